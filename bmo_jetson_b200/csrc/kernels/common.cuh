@@ -21,6 +21,10 @@ enum : int {
     kErrBadShape = 2,      // launch arguments inconsistent with the weight layout
     kErrReserved3 = 3,     // unused (no kernel raises it); kept so the other codes keep their bits
     kErrPeerTimeout = 4,   // a tensor-parallel peer's partial sums did not arrive within the wait bound
+    kErrNoPages = 5,       // paged plan: more pages needed than are free
+    kErrTableFull = 6,     // paged plan: a request would outgrow its row of the block table
+    kErrNoRoom = 7,        // paged plan: more new positions than the caller's lists hold
+    kErrBadIndex = 8,      // paged calls: a length, request, page or slot number out of range
 };
 
 // Upper bound on mbarrier polls before a wait gives up (~1-2 s with back-off).

@@ -1,0 +1,961 @@
+// paged_attention.cu -- attention of single tokens over the paged key-value
+// cache, the work of all rows split evenly over the GPU's warps and joined.
+//
+//   s_j = scale * q . k_j,  out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
+//
+// over the last `window` positions of a row.  One pass over the keys and
+// values: each warp keeps a running maximum, the sum of the weights and the
+// weighted sum of the values, and rescales them when the maximum grows.
+//
+// Every key and value is read once and used for a few query heads, so the
+// kernel is bound by memory; what has to be avoided is anything that keeps
+// loads from being in flight.  Rows go from global memory straight into the
+// registers in which the matrix instruction (mma.sync m16n8k16) takes its A
+// operand: the contraction runs over a permuted index, so a lane's 16
+// consecutive bytes are its fragment, and nothing is staged, transposed or
+// synchronised.  (tcgen05.mma would need the rows in shared memory in its
+// canonical layout, and 128 rows of which a decode step fills 2.)
+//   scores: A = 16 positions x 16 elements of K, B = q
+//   values: A = 16 elements x 16 positions of V^T, B = the weights
+// B has 8 columns.  An fp32 factor x takes two of them, hi = fp16(x) and
+// lo = fp16(x - hi), so products with fp16 keys and values keep about 22 bits
+// (x is brought into fp16's range by a power of two first) and are summed in
+// fp32 by the tensor core.
+//   fp16 cache: columns 2t, 2t + 1 are head t of a group of 4 (or 2 x 4).
+//   Q4_0 cache: columns 2t, 2t + 1 are block t of head_dim: q is masked to the
+//   block, so the score comes out as one integer-code sum per block, which
+//   the block's scale multiplies in fp32; and the weight of a value's block is
+//   p times that block's scale.  Codes n - 8 are exact in fp16.
+//
+// Work: a row's window is cut into tiles of kTile positions; (row, key head,
+// tile) in that order is a line of tiles of which every warp takes an equal,
+// contiguous part.  A head that lies within one warp's part is written at once.
+// Otherwise its pieces are joined in shared memory among the CTA's warps,
+// then through global memory by the last CTA to arrive, in the order of the
+// line, so the result does not depend on the order of arrival.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include <atomic>
+
+#include "../paged.h"
+#include "common.cuh"
+
+namespace bmo {
+namespace {
+
+constexpr int kPaWarps = 4;
+constexpr int kPaThreads = 32 * kPaWarps;
+constexpr float kLn2 = 0.6931471805599453f;
+// Weights are e^(s - m) * 2^7 in fp16; the maximum m is raised only when a
+// score passes it by more than 2^8, so a weight is below 2^15 and the sum
+// of its two parts is exact to 2^-25 of the largest weight's 2^7.
+constexpr float kSlack = 8.0f, kHead = 7.0f;
+
+__device__ __forceinline__ uint32_t pa_div(uint32_t n, const FastDiv &f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint4 ldg_stream16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+        : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldg_stream4(const void *p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 matrix of 16-bit elements held two a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t split_half(float x) {  // (hi, lo)
+    const __half hi = __float2half_rn(x);
+    const __half2 p = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+__device__ __forceinline__ uint32_t half_bits2(__half a, __half b) {
+    const __half2 p = __halves2half2(a, b);
+    return *reinterpret_cast<const uint32_t *>(&p);
+}
+
+// Codes 0..15 at bits 0-3 and 16-19 (or 4-7 and 20-23) of w as halves n - 8:
+// the code is placed in the mantissa of 1024 and the offset taken away.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
+    const uint32_t m = (w & 0x000f000fu) | 0x64006400u;
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&m), __float2half2_rn(1032.0f));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
+    const uint32_t m = (w & 0x00f000f0u) | 0x64006400u;
+    const __half2 h =
+        __hfma2(*reinterpret_cast<const __half2 *>(&m), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float act_load(const void *p, int act, long long i) {
+    if (act == BMO_ACT_F32) return static_cast<const float *>(p)[i];
+    if (act == BMO_ACT_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+}
+// 4 elements from i (a multiple of 4 elements from an aligned start if vec).
+__device__ __forceinline__ float4 act_load4(const void *p, int act, long long i, bool vec) {
+    if (!vec) return make_float4(act_load(p, act, i), act_load(p, act, i + 1), act_load(p, act, i + 2), act_load(p, act, i + 3));
+    if (act == BMO_ACT_F32) return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
+    const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
+    if (act == BMO_ACT_F16) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)),
+                     b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                       __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void act_store4(void *p, int act, long long i, float4 x, bool vec) {
+    if (act == BMO_ACT_F32) {
+        float *o = static_cast<float *>(p) + i;
+        if (vec) *reinterpret_cast<float4 *>(o) = x;
+        else o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
+        return;
+    }
+    uint16_t *o = static_cast<uint16_t *>(p) + i;
+    uint2 u;
+    if (act == BMO_ACT_F16) {
+        u.x = half_bits2(__float2half_rn(x.x), __float2half_rn(x.y));
+        u.y = half_bits2(__float2half_rn(x.z), __float2half_rn(x.w));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+        u.x = *reinterpret_cast<const uint32_t *>(&a);
+        u.y = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    if (vec) *reinterpret_cast<uint2 *>(o) = u;
+    else o[0] = u.x & 0xffff, o[1] = u.x >> 16, o[2] = u.y & 0xffff, o[3] = u.y >> 16;
+}
+
+// The power of two that brings amax into [2^10, 2^11), and its inverse
+// (both normal floats; amax 0, infinite or NaN gives some finite factor).
+__device__ __forceinline__ void range_factor(float amax, float &mul, float &inv) {
+    int ex = (__float_as_int(amax) >> 23) & 255;
+    ex = min(max(ex, 11), 254);
+    mul = __int_as_float((264 - ex) << 23);
+    inv = __int_as_float((ex - 10) << 23);
+}
+
+// Where a warp's lanes find the rows of 16 consecutive positions.  A layer
+// has fewer than 2^32 - 1 rows (checked by the entry point).
+constexpr uint32_t kNoRow = 0xffffffffu;  // not attended
+struct Pos16 {
+    uint32_t row[2];   // position g, g + 8 (scores)
+    uint32_t vrow[4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9
+};
+
+// A warp's walk through one row's pages: entries [b0, b0 + 32) of the row's
+// block table, one a lane.
+struct Pages {
+    const int *table;  // of the request
+    int b0, entry;
+};
+
+// ---- fp16 rows ----
+template <int HD_, int NB_>
+struct F16Rows {
+    static constexpr int HD = HD_, NB = NB_;
+    static constexpr int kMinCtas = NB == 1 ? 3 : 2;
+    static constexpr int kHeads = 4 * NB;          // query heads of a unit
+    static constexpr int kSub = HD == 128 ? 1 : 2; // 16-position parts of a tile
+    static constexpr int kO = HD / 16;
+    uint32_t q[NB][HD / 16][2];
+    float inv[NB];
+    uint4 kr[kSub][2][HD / 32], vr[kSub][4][HD / 64];
+
+    __device__ __forceinline__ void load_q(const PagedAttnArgs &a, int row, int head0, int n_heads, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int h = 4 * nb + (g >> 1);
+            float x[HD / 4];
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i) x[i] = 0.0f;
+            if (h < n_heads) {
+                const long long base = row * a.q_stride + static_cast<long long>(head0 + h) * HD + 8 * t;
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const float4 f = act_load4(a.q, a.act, base + 32 * c + 4 * u, a.q_vec);
+                        x[8 * c + 4 * u] = f.x * a.qscale, x[8 * c + 4 * u + 1] = f.y * a.qscale;
+                        x[8 * c + 4 * u + 2] = f.z * a.qscale, x[8 * c + 4 * u + 3] = f.w * a.qscale;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            float mul, iv;
+            range_factor(amax, mul, iv);
+            inv[nb] = __shfl_sync(0xffffffffu, iv, 8 * t);  // of head t, from lane (g = 2t, 0)
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {  // element pairs (2i, 2i + 1) of this lane
+                const float y0 = x[2 * i] * mul, y1 = x[2 * i + 1] * mul;
+                __half h0 = __float2half_rn(y0), h1 = __float2half_rn(y1);
+                if (g & 1) h0 = __float2half_rn(y0 - __half2float(h0)), h1 = __float2half_rn(y1 - __half2float(h1));
+                q[nb][i / 2][i % 2] = half_bits2(h0, h1);
+            }
+        }
+    }
+    __device__ __forceinline__ void load_k(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
+        const int t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const char *src = static_cast<const char *>(a.k) + static_cast<size_t>(p.row[i]) * (2 * HD) + 16 * t;
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c)
+                kr[s][i][c] = p.row[i] != kNoRow ? ldg_stream16(src + 64 * c) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void load_v(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
+        const int g = lane >> 2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const char *src = static_cast<const char *>(a.v) + static_cast<size_t>(p.vrow[i]) * (2 * HD) + 16 * g;
+#pragma unroll
+            for (int c = 0; c < HD / 64; ++c)
+                vr[s][i][c] = p.vrow[i] != kNoRow ? ldg_stream16(src + 128 * c) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    // sc[nb][i]: score (log2 units) of position g + 8 i for head (nb, t)
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) {
+                const uint4 x = kr[s][0][j], y = kr[s][1][j];
+                mma16816(c, x.x, y.x, x.y, y.y, q[nb][2 * j][0], q[nb][2 * j][1]);
+                mma16816(c, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
+            }
+            sc[nb][0] = (c[0] + c[1]) * inv[nb];
+            sc[nb][1] = (c[2] + c[3]) * inv[nb];
+        }
+    }
+    __device__ __forceinline__ bool value_range(int) { return false; }
+    __device__ __forceinline__ void raise_value_range(float (&)[NB][kO][4]) {}
+    __device__ __forceinline__ void reset() {}
+    __device__ __forceinline__ void values(int s, const float (&w)[NB][2], float (&o)[NB][kO][4]) {
+        uint32_t b[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            b[nb][0] = transpose8(split_half(w[nb][0]));
+            b[nb][1] = transpose8(split_half(w[nb][1]));
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c) {
+            const uint4 *v0 = &vr[s][0][c], *v1 = &vr[s][1][c], *v2 = &vr[s][2][c], *v3 = &vr[s][3][c];
+#define BMO_PV(j, f)                                                                              \
+    {                                                                                             \
+        const uint32_t a0 = __byte_perm(v0->f, v1->f, 0x5410), a1 = __byte_perm(v0->f, v1->f, 0x7632); \
+        const uint32_t a2 = __byte_perm(v2->f, v3->f, 0x5410), a3 = __byte_perm(v2->f, v3->f, 0x7632); \
+        _Pragma("unroll") for (int nb = 0; nb < NB; ++nb)                                         \
+            mma16816(o[nb][4 * c + j], a0, a1, a2, a3, b[nb][0], b[nb][1]);                       \
+    }
+            BMO_PV(0, x)
+            BMO_PV(1, y)
+            BMO_PV(2, z)
+            BMO_PV(3, w)
+#undef BMO_PV
+        }
+    }
+    // The lane's 8 consecutive elements [64 c + 8 g, + 8) of head (nb, t).
+    static constexpr int kRuns = HD / 64, kRunLen = 8;
+    __device__ __forceinline__ bool owns(int) const { return true; }
+    __device__ __forceinline__ static int head_of(int nb, int lane) { return 4 * nb + (lane & 3); }
+    __device__ __forceinline__ static int run_start(int run, int lane) { return 64 * run + 8 * (lane >> 2); }
+    __device__ __forceinline__ float element(const float (&o)[kO][4], int run, int i) const {
+        const float *c = o[4 * run + i / 2];
+        return i % 2 ? c[2] + c[3] : c[0] + c[1];
+    }
+};
+
+// ---- Q4_0 rows ----
+template <int HD_>
+struct Q4Rows {
+    static constexpr int HD = HD_, NB = 1;
+    static constexpr int kMinCtas = 3;
+    static constexpr int kHeads = 1;
+    static constexpr int kSub = 4;
+    static constexpr int kO = HD / 16;
+    static constexpr int kBlocks = HD / 32;       // <= 4: a column pair each
+    static constexpr int kKW = HD / 32;           // words of a key row a lane holds
+    static constexpr int kVW = HD / 64;           // words of a value row a lane holds
+    uint32_t q[HD / 16][2];
+    float inv;
+    float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
+    uint32_t kr[kSub][2][kKW], vr[kSub][4][kVW];
+    __half ks[kSub][2], vs[kSub][2];
+
+    __device__ __forceinline__ void load_q(const PagedAttnArgs &a, int row, int head0, int, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        // lane t holds words of block blk from byte `byte`; column pair g / 2 is block g / 2
+        const int blk = HD == 128 ? t : t >> 1, byte = HD == 128 ? 0 : 8 * (t & 1);
+        const bool mine = (g >> 1) == blk;
+        float lo[4 * kKW], hi[4 * kKW];  // elements byte + i and 16 + byte + i of the block
+        float amax = 0.0f;
+        const long long base = row * a.q_stride + static_cast<long long>(head0) * HD + 32 * blk + byte;
+#pragma unroll
+        for (int w = 0; w < kKW; ++w) {
+            const float4 x = act_load4(a.q, a.act, base + 4 * w, a.q_vec);
+            const float4 y = act_load4(a.q, a.act, base + 16 + 4 * w, a.q_vec);
+            lo[4 * w] = x.x * a.qscale, lo[4 * w + 1] = x.y * a.qscale;
+            lo[4 * w + 2] = x.z * a.qscale, lo[4 * w + 3] = x.w * a.qscale;
+            hi[4 * w] = y.x * a.qscale, hi[4 * w + 1] = y.y * a.qscale;
+            hi[4 * w + 2] = y.z * a.qscale, hi[4 * w + 3] = y.w * a.qscale;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * kKW; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float mul;
+        range_factor(amax, mul, inv);
+        auto part = [&](float x) {
+            const float y = mine ? x * mul : 0.0f;
+            const __half h = __float2half_rn(y);
+            return (g & 1) ? __float2half_rn(y - __half2float(h)) : h;
+        };
+#pragma unroll
+        for (int w = 0; w < kKW; ++w) {
+            q[2 * w][0] = half_bits2(part(lo[4 * w]), part(lo[4 * w + 2]));
+            q[2 * w][1] = half_bits2(part(hi[4 * w]), part(hi[4 * w + 2]));
+            q[2 * w + 1][0] = half_bits2(part(lo[4 * w + 1]), part(lo[4 * w + 3]));
+            q[2 * w + 1][1] = half_bits2(part(hi[4 * w + 1]), part(hi[4 * w + 3]));
+        }
+    }
+    __device__ __forceinline__ void load_k(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
+        const int t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool ok = p.row[i] != kNoRow;
+            const char *src = static_cast<const char *>(a.k) + static_cast<size_t>(p.row[i]) * (HD / 2) + 4 * kKW * t;
+            if constexpr (HD == 128) {
+                const uint4 x = ok ? ldg_stream16(src) : make_uint4(0, 0, 0, 0);
+                kr[s][i][0] = x.x, kr[s][i][1] = x.y, kr[s][i][2] = x.z, kr[s][i][3] = x.w;
+            } else {
+                const uint2 x = ok ? ldg_stream8(src) : make_uint2(0, 0);
+                kr[s][i][0] = x.x, kr[s][i][1] = x.y;
+            }
+            ks[s][i] = ok && t < kBlocks ? __ldg(a.k_scale + static_cast<size_t>(p.row[i]) * kBlocks + t) : __ushort_as_half(0);
+        }
+    }
+    __device__ __forceinline__ void load_v(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool ok = p.vrow[i] != kNoRow;
+            const char *src = static_cast<const char *>(a.v) + static_cast<size_t>(p.vrow[i]) * (HD / 2) + 4 * kVW * g;
+            if constexpr (HD == 128) {
+                const uint2 x = ok ? ldg_stream8(src) : make_uint2(0, 0);
+                vr[s][i][0] = x.x, vr[s][i][1] = x.y;
+            } else {
+                vr[s][i][0] = ok ? ldg_stream4(src) : 0;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            vs[s][i] = p.row[i] != kNoRow && t < kBlocks ? __ldg(a.v_scale + static_cast<size_t>(p.row[i]) * kBlocks + t) : __ushort_as_half(0);
+    }
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
+        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kKW; ++w) {
+            const uint32_t x = kr[s][0][w], y = kr[s][1][w];
+            mma16816(c, codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y), q[2 * w][0], q[2 * w][1]);
+            mma16816(c, codes_lo(x >> 8), codes_lo(y >> 8), codes_hi(x >> 8), codes_hi(y >> 8), q[2 * w + 1][0],
+                     q[2 * w + 1][1]);
+        }
+        sc[0][0] = (c[0] + c[1]) * __half2float(ks[s][0]);
+        sc[0][1] = (c[2] + c[3]) * __half2float(ks[s][1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 1);
+            sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 2);
+            sc[0][i] *= inv;
+        }
+    }
+    __device__ __forceinline__ void reset() { vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
+    // Whether a value scale of part s passes the bound of what a weight may be multiplied by.
+    __device__ __forceinline__ bool value_range(int s) {
+        return fabsf(__half2float(vs[s][0])) > vlim || fabsf(__half2float(vs[s][1])) > vlim;
+    }
+    __device__ __forceinline__ void raise_value_range(float (&o)[NB][kO][4]) {
+        float m = vlim;
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+            m = fmaxf(m, fmaxf(fabsf(__half2float(vs[s][0])), fabsf(__half2float(vs[s][1]))));
+        m = warp_max(m);
+        const int ex = min(((__float_as_int(m) >> 23) & 255) + 2, 127 + 18);  // a power of two above 2 m
+        const float lim = __int_as_float(ex << 23);
+        const float f = vlim * __int_as_float((254 - ex) << 23);
+        vlim = lim, vinv = __int_as_float((254 - ex) << 23);
+#pragma unroll
+        for (int j = 0; j < kO; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[0][j][i] *= f;
+    }
+    __device__ __forceinline__ void values(int s, const float (&w)[NB][2], float (&o)[NB][kO][4]) {
+        // w / vlim * scale <= 2^15
+        const uint32_t b0 = transpose8(split_half(w[0][0] * (__half2float(vs[s][0]) * vinv)));
+        const uint32_t b1 = transpose8(split_half(w[0][1] * (__half2float(vs[s][1]) * vinv)));
+#pragma unroll
+        for (int i = 0; i < kVW; ++i) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t x = __byte_perm(vr[s][0][i], vr[s][1][i], u ? 0x7632 : 0x5410);
+                const uint32_t y = __byte_perm(vr[s][2][i], vr[s][3][i], u ? 0x7632 : 0x5410);
+                mma16816(o[0][4 * i + 2 * u], codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y), b0, b1);
+                mma16816(o[0][4 * i + 2 * u + 1], codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8),
+                         codes_hi(y >> 8), b0, b1);
+            }
+        }
+    }
+    // Lane (g, t) holds bytes [4 kVW g, + 4 kVW) of the row: elements of block
+    // blk(g), low nibbles then high ones; the columns of that block are lane t == blk(g)'s.
+    static constexpr int kRuns = 2, kRunLen = 4 * kVW;
+    __device__ __forceinline__ bool owns(int lane) const { return (lane & 3) == (lane >> 2) * kBlocks / 8; }
+    __device__ __forceinline__ static int head_of(int, int) { return 0; }
+    __device__ __forceinline__ static int run_start(int run, int lane) {
+        const int g = lane >> 2;
+        return HD == 128 ? 32 * (g >> 1) + 8 * (g & 1) + 16 * run : 32 * (g >> 2) + 4 * (g & 3) + 16 * run;
+    }
+    __device__ __forceinline__ float element(const float (&o)[kO][4], int run, int i) const {
+        const float *c = o[i];
+        return (run ? c[2] + c[3] : c[0] + c[1]) * vlim;
+    }
+};
+
+// Two pieces a warp: one that began before its part of the line, one that goes on after it.
+template <int HD, int NH>
+struct PaSmem {
+    static constexpr int kPieces = 2 * kPaWarps;
+    float m[kPieces][NH], l[kPieces][NH];
+    float o[kPieces][NH][HD];
+    int seg[kPieces];    // row * units + unit, -1: none
+    int whole[kPieces];  // bit 0: begins at the head's first tile, bit 1: ends at its last
+    int join[2];         // this CTA is the last to arrive: global slot kind 0 / 1
+};
+
+constexpr int kJoinMax = 640;  // pieces a head can have: CTAs of a launch
+
+template <int HD, int NH>
+struct PaJoin {  // replaces the pieces when a CTA joins a head
+    float w[kJoinMax * NH];
+    float l[kJoinMax * NH];
+    float mm[NH], ll[NH];
+};
+
+__device__ __forceinline__ int pa_len(const PagedAttnArgs &a, int row, int &req, bool &bad) {
+    req = a.row_req ? a.row_req[row] : row;
+    if (req < 0 || req >= a.n_req) {
+        bad = true;
+        req = 0;
+        return 0;
+    }
+    int len = a.row_len ? a.row_len[row] : a.lens[req];
+    const int cap = static_cast<int>(a.max_blocks * a.page.d);
+    if (len < 0 || len > cap) {
+        bad = true;
+        len = len < 0 ? 0 : cap;
+    }
+    return len;
+}
+
+template <int HD, int NH>
+constexpr size_t kFixedSmem =
+    ((sizeof(PaSmem<HD, NH>) > sizeof(PaJoin<HD, NH>) ? sizeof(PaSmem<HD, NH>) : sizeof(PaJoin<HD, NH>)) + 15) / 16 * 16;
+
+// A piece in global memory: [heads][HD] sums, then the maxima and the weights' sums; 16-byte multiples.
+template <class R>
+constexpr int pa_piece_floats = (R::kHeads * (R::HD + 2) + 3) / 4 * 4;
+
+template <class R>
+__global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int HD = R::HD, NB = R::NB, NH = R::kHeads, kTile = 16 * R::kSub, kO = R::kO;
+    using Smem = PaSmem<HD, NH>;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    Smem &S = *reinterpret_cast<Smem *>(smem_raw);
+    int *ends = reinterpret_cast<int *>(smem_raw + kFixedSmem<HD, NH>);  // tiles of rows 0..r
+    __shared__ int scan_warp[kPaWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int group = a.n_heads / a.n_kv_heads;       // query heads of a key head
+    const int chunks = (group + NH - 1) / NH;         // units of a key head
+    const int units = a.n_kv_heads * chunks;
+    bool bad = false;
+
+    // ---- tiles of every row, summed ----
+    auto row_tiles = [&](int r, int &start, int &len) {
+        int req;
+        len = pa_len(a, r, req, bad);
+        start = a.window > 0 ? max(0, len - a.window) : 0;
+        return len > start ? (len + kTile - 1) / kTile - start / kTile : 0;
+    };
+    {
+        const int per_thread = (a.n_rows + kPaThreads - 1) / kPaThreads;
+        const int r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
+        int sum = 0, st, ln;
+        for (int r = r0; r < r1; ++r) {
+            sum += row_tiles(r, st, ln);
+            ends[r] = sum;
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += u;
+        }
+        if (lane == 31) scan_warp[warp] = inc;
+        if (tid < Smem::kPieces) S.seg[tid] = -1;
+        if (tid < 2) S.join[tid] = 0;
+        __syncthreads();
+        int before = inc - sum;
+        for (int w = 0; w < warp; ++w) before += scan_warp[w];
+        if (before)
+            for (int r = r0; r < r1; ++r) ends[r] += before;
+        __syncthreads();
+    }
+    if (bad) raise_error(a.status, kErrBadIndex);
+    const long long total = static_cast<long long>(ends[a.n_rows - 1]) * units;
+    const int n_warps = gridDim.x * kPaWarps;
+    const long long per = max(1ll, (total + n_warps - 1) / n_warps);
+    long long u = min(total, (static_cast<long long>(blockIdx.x) * kPaWarps + warp) * per);
+    const long long u_end = min(total, u + per);
+
+    // rows without a position
+    for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+        if (ends[r] != (r ? ends[r - 1] : 0)) continue;
+        for (int i = tid; i < a.n_heads * HD / 4; i += kPaThreads)
+            act_store4(a.out, a.act, r * a.out_stride + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f), a.out_vec);
+        if (a.lse)
+            for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
+    }
+
+    R R_;
+    while (u < u_end) {
+        // ---- the head that tile u belongs to ----
+        int row;
+        {
+            int lo = 0, hi = a.n_rows - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (static_cast<long long>(ends[mid]) * units > u) hi = mid;
+                else lo = mid + 1;
+            }
+            row = lo;
+        }
+        const int row0 = row ? ends[row - 1] : 0;
+        const int n_tiles = ends[row] - row0;
+        const long long rem = u - static_cast<long long>(row0) * units;
+        const int unit = static_cast<int>(rem / n_tiles);
+        const int tile0 = static_cast<int>(rem - static_cast<long long>(unit) * n_tiles);
+        const int tile1 = static_cast<int>(min(static_cast<long long>(n_tiles), tile0 + (u_end - u)));
+        u += tile1 - tile0;
+        int req, start, len;
+        len = pa_len(a, row, req, bad);
+        start = a.window > 0 ? max(0, len - a.window) : 0;
+        const int base_tile = start / kTile;
+        const int kh = unit / chunks, chunk = unit - kh * chunks;
+        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
+
+        Pages pg;
+        pg.table = a.table + static_cast<long long>(req) * a.max_blocks;
+        auto refill = [&](int b) {
+            pg.b0 = b;
+            pg.entry = b + lane < a.max_blocks ? pg.table[b + lane] : -1;
+        };
+        refill(static_cast<int>(pa_div(max(start, (base_tile + tile0) * kTile), a.page)));
+        // rows of the 16 positions from p0; those outside [start, len) and those of invalid pages: -1
+        auto locate = [&](int p0, Pos16 &P) {
+            const int first = max(p0, start), last = min(p0 + 15, len - 1);
+            if (first > last) {
+                P.row[0] = P.row[1] = P.vrow[0] = P.vrow[1] = P.vrow[2] = P.vrow[3] = kNoRow;
+                return;
+            }
+            const int b_first = pa_div(first, a.page), b_last = pa_div(last, a.page);
+            if (b_last >= pg.b0 + 32) refill(b_first);
+            if (b_first == b_last) {
+                const int page = __shfl_sync(0xffffffffu, pg.entry, b_first - pg.b0);
+                const bool ok = page >= 0 && page < a.n_pages;
+                bad |= !ok;
+                const uint32_t r0 = (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d - b_first * a.page.d;
+                auto at = [&](int p) { return ok && p >= first && p <= last ? r0 + p : kNoRow; };
+                P.row[0] = at(p0 + g), P.row[1] = at(p0 + g + 8);
+                P.vrow[0] = at(p0 + 2 * t), P.vrow[1] = at(p0 + 2 * t + 1);
+                P.vrow[2] = at(p0 + 2 * t + 8), P.vrow[3] = at(p0 + 2 * t + 9);
+            } else {
+                auto at = [&](int p) {
+                    const bool in = p >= first && p <= last;
+                    const int b = in ? static_cast<int>(pa_div(p, a.page)) : b_first;
+                    const int page = __shfl_sync(0xffffffffu, pg.entry, b - pg.b0);
+                    const bool ok = page >= 0 && page < a.n_pages;
+                    bad |= in && !ok;
+                    return in && ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + (p - b * a.page.d)
+                                    : kNoRow;
+                };
+                P.row[0] = at(p0 + g), P.row[1] = at(p0 + g + 8);
+                P.vrow[0] = at(p0 + 2 * t), P.vrow[1] = at(p0 + 2 * t + 1);
+                P.vrow[2] = at(p0 + 2 * t + 8), P.vrow[3] = at(p0 + 2 * t + 9);
+            }
+        };
+
+        float o[NB][kO][4], m[NB], l[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            m[nb] = -INFINITY, l[nb] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kO; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nb][j][i] = 0.0f;
+        }
+        R_.reset();
+        Pos16 P[R::kSub];
+        const int pbase = base_tile * kTile;
+#pragma unroll
+        for (int s = 0; s < R::kSub; ++s) {
+            locate(pbase + tile0 * kTile + 16 * s, P[s]);
+            R_.load_k(a, s, P[s], lane);
+        }
+        R_.load_q(a, row, head0, heads, lane);
+        for (int tile = tile0; tile < tile1; ++tile) {
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s) R_.load_v(a, s, P[s], lane);
+            float sc[R::kSub][NB][2];
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s) {
+                R_.scores(s, sc[s]);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    if (P[s].row[0] == kNoRow) sc[s][nb][0] = -INFINITY;
+                    if (P[s].row[1] == kNoRow) sc[s][nb][1] = -INFINITY;
+                }
+            }
+            if (tile + 1 < tile1) {
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) {
+                    locate(pbase + (tile + 1) * kTile + 16 * s, P[s]);
+                    R_.load_k(a, s, P[s], lane);
+                }
+            }
+            bool rise = false;
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) rise |= fmaxf(sc[s][nb][0], sc[s][nb][1]) > m[nb] + kSlack;
+            if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float x = m[nb];
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) x = fmaxf(x, fmaxf(sc[s][nb][0], sc[s][nb][1]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float f = x == -INFINITY ? 1.0f : ex2(m[nb] - x);
+                    m[nb] = x;
+                    l[nb] *= f;
+#pragma unroll
+                    for (int j = 0; j < kO; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[nb][j][i] *= f;
+                }
+            }
+            bool wide = false;
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s) wide |= R_.value_range(s);
+            if (__any_sync(0xffffffffu, wide)) R_.raise_value_range(o);
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s) {
+                float w[NB][2];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
+                    w[nb][0] = ex2(sc[s][nb][0] - ref);
+                    w[nb][1] = ex2(sc[s][nb][1] - ref);
+                    l[nb] += w[nb][0] + w[nb][1];
+                }
+                R_.values(s, w, o);
+            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], d);
+
+        // ---- a whole head goes out, a piece into shared memory ----
+        const bool begins = tile0 == 0, finishes = tile1 == n_tiles;
+        const int slot = 2 * warp + (begins ? 1 : 0);
+        if (!(begins && finishes) && lane == 0) {
+            S.seg[slot] = row * units + unit;
+            S.whole[slot] = (begins ? 1 : 0) | (finishes ? 2 : 0);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int h = R::head_of(nb, lane);
+            if (begins && finishes) {
+                if (h < heads) {
+                    const float f = l[nb] == 0.0f ? 0.0f : 1.0f / l[nb];
+                    if (R_.owns(lane)) {
+                        const long long out0 = row * a.out_stride + static_cast<long long>(head0 + h) * HD;
+#pragma unroll
+                        for (int run = 0; run < R::kRuns; ++run)
+#pragma unroll
+                            for (int i = 0; i < R::kRunLen; i += 4)
+                                act_store4(a.out, a.act, out0 + R::run_start(run, lane) + i,
+                                           make_float4(R_.element(o[nb], run, i) * f, R_.element(o[nb], run, i + 1) * f,
+                                                       R_.element(o[nb], run, i + 2) * f, R_.element(o[nb], run, i + 3) * f),
+                                           a.out_vec);
+                    }
+                    if (a.lse && g == 0 && (NH > 1 || t == 0))
+                        a.lse[static_cast<long long>(row) * a.n_heads + head0 + h] =
+                            l[nb] == 0.0f ? -INFINITY : (m[nb] - kHead + log2f(l[nb])) * kLn2;
+                }
+            } else {
+                if (R_.owns(lane)) {
+#pragma unroll
+                    for (int run = 0; run < R::kRuns; ++run)
+#pragma unroll
+                        for (int i = 0; i < R::kRunLen; i += 4)
+                            *reinterpret_cast<float4 *>(&S.o[slot][h][R::run_start(run, lane) + i]) =
+                                make_float4(R_.element(o[nb], run, i), R_.element(o[nb], run, i + 1),
+                                            R_.element(o[nb], run, i + 2), R_.element(o[nb], run, i + 3));
+                }
+                if (g == 0 && (NH > 1 || t == 0)) S.m[slot][h] = m[nb], S.l[slot][h] = l[nb];
+            }
+        }
+    }
+    if (bad) raise_error(a.status, kErrBadIndex);
+    __syncthreads();
+
+    // ---- pieces of one head within the CTA: joined by the warp that holds the first ----
+    const long long cta_tiles = per * kPaWarps;
+    constexpr int kPieceFloats = pa_piece_floats<R>;
+    for (int i = 2 * warp; i < 2 * warp + 2; ++i) {
+        const int seg = S.seg[i];
+        if (seg < 0) continue;
+        int before = i - 1;
+        while (before >= 0 && S.seg[before] < 0) --before;
+        if (before >= 0 && S.seg[before] == seg) continue;
+        int last = i;
+        for (int j = i + 1; j < Smem::kPieces; ++j)
+            if (S.seg[j] == seg) last = j;
+        const bool begins = S.whole[i] & 1, finishes = S.whole[last] & 2;
+        const int row = seg / units, unit = seg - row * units;
+        const int kh = unit / chunks, chunk = unit - kh * chunks;
+        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
+        float *dst = a.part + (2ll * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
+        for (int h = 0; h < heads; ++h) {
+            float M = -INFINITY, L = 0.0f;
+            for (int j = i; j <= last; ++j)
+                if (S.seg[j] == seg) M = fmaxf(M, S.m[j][h]);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int d = 4 * lane;
+            for (int j = i; j <= last; ++j) {
+                if (S.seg[j] != seg) continue;
+                const float f = S.m[j][h] == M ? 1.0f : ex2(S.m[j][h] - M);
+                L += f * S.l[j][h];
+                if (d < HD) {
+                    const float4 x = *reinterpret_cast<const float4 *>(&S.o[j][h][d]);
+                    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                }
+            }
+            if (begins && finishes) {
+                const float f = L == 0.0f ? 0.0f : 1.0f / L;
+                if (d < HD)
+                    act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0 + h) * HD + d,
+                               make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec);
+                if (a.lse && lane == 0)
+                    a.lse[static_cast<long long>(row) * a.n_heads + head0 + h] =
+                        L == 0.0f ? -INFINITY : (M - kHead + log2f(L)) * kLn2;
+            } else {
+                if (d < HD) __stcg(reinterpret_cast<float4 *>(dst + h * HD + d), acc);
+                if (lane == 0) {
+                    __stcg(dst + NH * HD + h, M);
+                    __stcg(dst + NH * HD + NH + h, L);
+                }
+            }
+        }
+        if (!(begins && finishes)) {
+            // the head's tiles on the line and the CTAs they lie in
+            const int row0 = row ? ends[row - 1] : 0, n_tiles = ends[row] - row0;
+            const long long first = static_cast<long long>(row0) * units + static_cast<long long>(unit) * n_tiles;
+            const int c0 = static_cast<int>(first / cta_tiles), c1 = static_cast<int>((first + n_tiles - 1) / cta_tiles);
+            __threadfence();
+            __syncwarp();
+            if (lane == 0 && atomicAdd(a.cnt + c0, 1) == c1 - c0) {
+                a.cnt[c0] = 0;
+                S.join[begins ? 1 : 0] = seg + 1;
+            }
+        }
+    }
+    __syncthreads();
+    const int joins[2] = {S.join[0], S.join[1]};
+    if (!joins[0] && !joins[1]) return;
+    __threadfence();
+
+    // ---- the last CTA to arrive joins the head's pieces, in line order ----
+    using Join = PaJoin<HD, NH>;
+    Join &J = *reinterpret_cast<Join *>(smem_raw);
+    __shared__ float4 red[kPaThreads];
+    for (int k = 0; k < 2; ++k) {
+        if (!joins[k]) continue;
+        __syncthreads();
+        const int seg = joins[k] - 1;
+        const int row = seg / units, unit = seg - row * units;
+        const int kh = unit / chunks, chunk = unit - kh * chunks;
+        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
+        const int row0 = row ? ends[row - 1] : 0, n_tiles = ends[row] - row0;
+        const long long first = static_cast<long long>(row0) * units + static_cast<long long>(unit) * n_tiles;
+        const int c0 = static_cast<int>(first / cta_tiles), c1 = static_cast<int>((first + n_tiles - 1) / cta_tiles);
+        const int n = c1 - c0 + 1;
+        auto piece = [&](int i) { return a.part + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * kPieceFloats; };
+        for (int i = tid; i < n * heads; i += kPaThreads) {
+            const int p = i / heads, h = i - p * heads;
+            const float *src = piece(p) + NH * HD + h;
+            J.w[i] = __ldcg(src);
+            J.l[i] = __ldcg(src + NH);
+        }
+        __syncthreads();
+        for (int h = warp; h < heads; h += kPaWarps) {
+            float M = -INFINITY, L = 0.0f;
+            for (int p = lane; p < n; p += 32) M = fmaxf(M, J.w[p * heads + h]);
+            M = warp_max(M);
+            for (int p = lane; p < n; p += 32) {
+                const float x = J.w[p * heads + h];
+                const float f = x == M ? 1.0f : ex2(x - M);
+                J.w[p * heads + h] = f;
+                L += f * J.l[p * heads + h];
+            }
+            L = warp_sum(L);
+            if (lane == 0) J.mm[h] = M, J.ll[h] = L;
+        }
+        __syncthreads();
+        const int cols = heads * HD / 4;  // float4 columns
+        const int parts = max(1, kPaThreads / cols);
+        for (int c = tid % cols, part = tid / cols; c < cols; c += kPaThreads) {
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            const int h = 4 * c / HD;
+            if (part < parts) {
+#pragma unroll 8
+                for (int p = part; p < n; p += parts) {
+                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(piece(p)) + c);
+                    const float f = J.w[p * heads + h];
+                    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                }
+            }
+            if (parts > 1) {
+                red[tid] = acc;
+                __syncthreads();
+                if (part == 0)
+                    for (int q = 1; q < parts; ++q) {
+                        const float4 x = red[q * cols + c];
+                        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+                    }
+            }
+            if (part == 0) {
+                const float f = J.ll[h] == 0.0f ? 0.0f : 1.0f / J.ll[h];
+                act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0) * HD + 4 * c,
+                           make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec);
+            }
+        }
+        if (a.lse && tid < heads)
+            a.lse[static_cast<long long>(row) * a.n_heads + head0 + tid] =
+                J.ll[tid] == 0.0f ? -INFINITY : (J.mm[tid] - kHead + log2f(J.ll[tid])) * kLn2;
+    }
+}
+
+constexpr int kMaxDevices = 64;
+
+// CTAs of a launch on the current device: all that are resident at once, at
+// most kJoinMax (0: the kernel cannot run here).
+template <class R>
+cudaError_t pa_grid(int &grid) {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices && (grid = known[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
+    constexpr int smem = static_cast<int>(kFixedSmem<R::HD, R::kHeads> + 4 * kPagedMaxRows);
+    e = cudaFuncSetAttribute(paged_attn_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    int sms = 0, per_sm = 0;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R>, kPaThreads, smem)) != cudaSuccess)
+        return e;
+    grid = sms * per_sm < kJoinMax ? sms * per_sm : kJoinMax;
+    if (grid <= 0) return cudaErrorInvalidConfiguration;
+    if (dev < kMaxDevices) known[dev].store(grid, std::memory_order_release);
+    return cudaSuccess;
+}
+
+template <class R>
+size_t pa_scratch(int grid) {
+    return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256 +
+           static_cast<size_t>(grid) * 2 * pa_piece_floats<R> * sizeof(float);
+}
+
+template <class R>
+cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cudaStream_t s) {
+    int grid = 0;
+    const cudaError_t e = pa_grid<R>(grid);
+    if (e != cudaSuccess) return e;
+    if (scratch_bytes < pa_scratch<R>(grid)) return cudaErrorInvalidValue;
+    a.cnt = static_cast<int *>(scratch);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
+    paged_attn_kernel<R><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <class F>
+auto pa_variant(int head_dim, int kv_type, int group, F f) {
+    if (kv_type == kKvQ4_0) return head_dim == 128 ? f(Q4Rows<128>{}) : f(Q4Rows<64>{});
+    // up to 4 query heads of a key head fill one B operand, up to 8 two of them
+    if (group <= 4) return head_dim == 128 ? f(F16Rows<128, 1>{}) : f(F16Rows<64, 1>{});
+    return head_dim == 128 ? f(F16Rows<128, 2>{}) : f(F16Rows<64, 2>{});
+}
+
+}  // namespace
+
+size_t paged_attention_scratch_bytes(int head_dim, int kv_type, int n_heads, int n_kv_heads) {
+    return pa_variant(head_dim, kv_type, n_heads / n_kv_heads, [&](auto r) -> size_t {
+        int grid = 0;
+        return pa_grid<decltype(r)>(grid) == cudaSuccess ? pa_scratch<decltype(r)>(grid) : 0;
+    });
+}
+
+cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, void *scratch, size_t scratch_bytes,
+                                   cudaStream_t s) {
+    return pa_variant(head_dim, kv_type, a.n_heads / a.n_kv_heads,
+                      [&](auto r) { return pa_launch<decltype(r)>(a, scratch, scratch_bytes, s); });
+}
+
+}  // namespace bmo

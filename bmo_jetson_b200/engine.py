@@ -155,6 +155,17 @@ def lib() -> ctypes.CDLL:
         [i, i, i, vp]
     L.bmo_k_tp_exchange.restype = i
     L.bmo_k_decode_attention.restype = i
+    ll = ctypes.c_longlong
+    L.bmo_k_paged_plan.argtypes = [vp, vp, i] + [vp] * 7
+    L.bmo_k_paged_plan.restype = i
+    L.bmo_k_paged_append.argtypes = [vp, i, i, vp, ll, vp, ll, vp, vp, f, vp, ll, i, vp, ll, i, vp, vp]
+    L.bmo_k_paged_append.restype = i
+    L.bmo_k_paged_read.argtypes = [vp, i, i, vp, vp, vp, i, vp, vp]
+    L.bmo_k_paged_read.restype = i
+    L.bmo_k_paged_attention_scratch_bytes.argtypes = [vp, i]
+    L.bmo_k_paged_attention_scratch_bytes.restype = sz
+    L.bmo_k_paged_attention.argtypes = [vp, i, i, vp, ll, i, vp, vp, f, vp, ll, vp, i, vp, vp, sz, vp]
+    L.bmo_k_paged_attention.restype = i
     _lib = L
     return L
 

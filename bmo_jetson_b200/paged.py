@@ -1,0 +1,220 @@
+"""Paged key-value cache over torch tensors (include/bmo_kernels.h, ``bmo_k_paged_*``).
+
+A server of many sessions keeps their keys and values in pages of one pool
+instead of one ring each: ``PageBook`` says which session ("request") has
+which pages and plans every step on the device, ``PagedKV`` holds the pages of
+all layers, appends rows, reads them back and attends over them.  The caller
+owns every tensor; calls run on torch's current stream and do not
+synchronise.
+
+    book = PageBook.empty(n_req, n_pages, page_size, max_blocks, window=512)
+    kv = PagedKV.empty(book, n_layers, n_kv_heads, head_dim)
+    book.plan(n_new, slot, pos, req, offsets)             # once a step
+    kv.append(layer, k, v, slot, pos=pos, q=q, q_out=q)   # each layer
+    kv.attention(layer, q, out)
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from .engine import KV_F16, KV_Q4_0, lib
+
+NO_PAGES, TABLE_FULL, NO_ROOM, BAD_INDEX = 1 << 5, 1 << 6, 1 << 7, 1 << 8
+_ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class _Book(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lens", "free_pages", "state")] + \
+               [(n, ctypes.c_int32) for n in ("n_req", "max_blocks", "n_pages", "page_size", "window")]
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("book", _Book)] + [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, ctypes.c_int32) for n in ("n_layers", "n_kv_heads", "head_dim", "kv_type")]
+
+
+def _call(device, fn, *args) -> None:
+    """Runs a library call on `device` and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc != 0:
+        raise RuntimeError(f"{fn.__name__} rc={rc}")
+
+
+def _ints(t: torch.Tensor, name: str, device, numel: Optional[int] = None) -> int:
+    """Address of a dense int32 tensor on `device`."""
+    if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor on {device}")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name}: {numel} entries, got {t.numel()}")
+    return t.data_ptr()
+
+
+def _status(t: Optional[torch.Tensor], device) -> Optional[int]:
+    return None if t is None else _ints(t, "status", device, 1)
+
+
+class PageBook:
+    """Block table [n_req, max_blocks], lengths [n_req], ring of free pages
+    [n_pages] and state [4] (first free entry, free pages, status bits, new
+    positions of the last step): int32 tensors on one GPU."""
+
+    def __init__(self, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, state: torch.Tensor, *,
+                 page_size: int, window: int = 0):
+        if table.dim() != 2 or table.device.type != "cuda":
+            raise ValueError("table: [n_req, max_blocks] on a GPU")
+        self.table, self.lens, self.free, self.state = table, lens, free, state
+        self.page_size, self.window, self.device = int(page_size), int(window), table.device
+        n_req, max_blocks = table.shape
+        self._c = _Book(_ints(table, "table", self.device), _ints(lens, "lens", self.device, n_req),
+                        _ints(free, "free", self.device), _ints(state, "state", self.device, 4), n_req, max_blocks,
+                        free.numel(), self.page_size, self.window)
+        self._ref = ctypes.byref(self._c)
+
+    @classmethod
+    def empty(cls, n_req: int, n_pages: int, page_size: int, max_blocks: int, window: int = 0,
+              device="cuda") -> "PageBook":
+        """A book of no positions, every page free."""
+        i32 = {"dtype": torch.int32, "device": device}
+        return cls(torch.full((n_req, max_blocks), -1, **i32), torch.zeros(n_req, **i32),
+                   torch.arange(n_pages, **i32), torch.tensor([0, n_pages, 0, 0], **i32), page_size=page_size,
+                   window=window)
+
+    def plan(self, n_new: torch.Tensor, slot: torch.Tensor, pos: torch.Tensor, req: torch.Tensor,
+             offsets: torch.Tensor, lens_out: Optional[torch.Tensor] = None,
+             state_out: Optional[torch.Tensor] = None) -> None:
+        """Plans a step (bmo_k_paged_plan): n_new[r] > 0 appends positions to
+        request r, 0 leaves it, < 0 ends it.  slot, pos, req [max_tokens] and
+        offsets [n_req + 1] receive the list of new positions; the new
+        lengths and state replace the book's unless lens_out / state_out are
+        given.  state[2] != 0 after it: the step was refused, nothing changed."""
+        d, n_req = self.device, self._c.n_req
+        n = slot.numel()
+        _call(
+            d, lib().bmo_k_paged_plan, self._ref, _ints(n_new, "n_new", d, n_req), n, _ints(slot, "slot", d), _ints(pos, "pos", d, n),
+            _ints(req, "req", d, n), _ints(offsets, "offsets", d, n_req + 1),
+            self._c.lens if lens_out is None else _ints(lens_out, "lens_out", d, n_req),
+            self._c.state if state_out is None else _ints(state_out, "state_out", d, 4))
+
+
+class PagedKV:
+    """Keys and values of all layers in the pages of `book`: fp16 tensors
+    [n_layers, n_pages, n_kv_heads, page_size, head_dim], or Q4_0 as uint8
+    nibble planes [..., head_dim / 2] with fp16 scales [..., head_dim / 32].
+    Attention calls of one PagedKV share a scratch buffer: keep them on one
+    stream or order them."""
+
+    def __init__(self, book: PageBook, k: torch.Tensor, v: torch.Tensor, *, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None):
+        q4 = k.dtype is torch.uint8
+        if k.dim() != 5 or k.dtype not in (torch.float16, torch.uint8):
+            raise ValueError("k: fp16 or uint8 [n_layers, n_pages, n_kv_heads, page_size, row]")
+        n_layers, n_pages, n_kv, page_size, row = k.shape
+        if n_pages != book.free.numel() or page_size != book.page_size:
+            raise ValueError("k: the book's pages")
+        head_dim = 2 * row if q4 else row
+        self.book, self.k, self.v, self.k_scale, self.v_scale = book, k, v, k_scale, v_scale
+        self.n_layers, self.n_kv_heads, self.head_dim = n_layers, n_kv, head_dim
+        self.kv_type = KV_Q4_0 if q4 else KV_F16
+        planes = [("k", k, k.shape, k.dtype), ("v", v, k.shape, k.dtype)]
+        if q4:
+            scales = k.shape[:-1] + (head_dim // 32,)
+            planes += [("k_scale", k_scale, scales, torch.float16), ("v_scale", v_scale, scales, torch.float16)]
+        for name, t, shape, dtype in planes:
+            if t is None or t.shape != shape or t.dtype is not dtype or t.device != book.device or not t.is_contiguous():
+                raise ValueError(f"{name}: a contiguous {dtype} tensor of {tuple(shape)} on {book.device}")
+        self._c = _Cache(book._c, k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q4 else None,
+                         v_scale.data_ptr() if q4 else None, n_layers, n_kv, head_dim, self.kv_type)
+        self._ref = ctypes.byref(self._c)
+        self._scratch = {}  # by query heads
+
+    @classmethod
+    def empty(cls, book: PageBook, n_layers: int, n_kv_heads: int, head_dim: int, kv_type: int = KV_F16) -> "PagedKV":
+        shape = (n_layers, book.free.numel(), n_kv_heads, book.page_size)
+        if kv_type == KV_F16:
+            k, v = (torch.zeros(shape + (head_dim,), dtype=torch.float16, device=book.device) for _ in range(2))
+            return cls(book, k, v)
+        k, v = (torch.zeros(shape + (head_dim // 2,), dtype=torch.uint8, device=book.device) for _ in range(2))
+        ks, vs = (torch.zeros(shape + (head_dim // 32,), dtype=torch.float16, device=book.device) for _ in range(2))
+        return cls(book, k, v, k_scale=ks, v_scale=vs)
+
+    def _rows(self, t: torch.Tensor, name: str, n: int, dtype, heads: int):
+        """(address, row stride) of [n, heads, head_dim] rows whose heads are dense."""
+        if t.dtype is not dtype or t.device != self.book.device or t.shape != (n, heads, self.head_dim):
+            raise ValueError(f"{name}: {dtype} of {(n, heads, self.head_dim)} on {self.book.device}")
+        s = t.stride()
+        if s[2] != 1 or (heads > 1 and s[1] != self.head_dim):
+            raise ValueError(f"{name}: the heads of a row are contiguous")
+        return t.data_ptr(), s[0]
+
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, *,
+               pos: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
+               q_out: Optional[torch.Tensor] = None, theta: float = 0.0,
+               status: Optional[torch.Tensor] = None) -> None:
+        """Stores k, v [n, n_kv_heads, head_dim] at slot[n] (bmo_k_paged_append);
+        theta > 0 rotates k, and q into q_out, by the positions pos[n]."""
+        n, d = slot.numel(), self.book.device
+        act = _ACT.get(k.dtype)
+        if act is None:
+            raise ValueError(f"k: float32, float16 or bfloat16, got {k.dtype}")
+        kp, ks = self._rows(k, "k", n, k.dtype, self.n_kv_heads)
+        vp, vs = self._rows(v, "v", n, k.dtype, self.n_kv_heads)
+        qp = qs = qop = qos = heads = 0
+        if q is not None:
+            heads = q.shape[1]
+            qp, qs = self._rows(q, "q", n, k.dtype, heads)
+            qop, qos = self._rows(q_out, "q_out", n, k.dtype, heads)
+        _call(d, lib().bmo_k_paged_append, self._ref, layer, n, kp, ks, vp, vs, _ints(slot, "slot", d),
+              None if pos is None else _ints(pos, "pos", d, n), theta, qp or None, qs, heads, qop or None, qos, act,
+              _status(status, d))
+
+    def read(self, layer: int, slot: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,
+             status: Optional[torch.Tensor] = None) -> None:
+        """Rows at slot[n] as k_out, v_out [n, n_kv_heads, head_dim] (bmo_k_paged_read)."""
+        n, d = slot.numel(), self.book.device
+        act = _ACT.get(k_out.dtype)
+        if act is None:
+            raise ValueError(f"k_out: float32, float16 or bfloat16, got {k_out.dtype}")
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if not t.is_contiguous():
+                raise ValueError(f"{name}: contiguous")
+        kp, _ = self._rows(k_out, "k_out", n, k_out.dtype, self.n_kv_heads)
+        vp, _ = self._rows(v_out, "v_out", n, k_out.dtype, self.n_kv_heads)
+        _call(d, lib().bmo_k_paged_read, self._ref, layer, n, _ints(slot, "slot", d), kp, vp, act, _status(status, d))
+
+    def attention(self, layer: int, q: torch.Tensor, out: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
+                  row_lens: Optional[torch.Tensor] = None, scale: float = 0.0, lse: Optional[torch.Tensor] = None,
+                  status: Optional[torch.Tensor] = None) -> None:
+        """Attention of q [n, n_heads, head_dim] into out (bmo_k_paged_attention).
+        Row i is a token of request rows[i] (default i) that attends to the first
+        row_lens[i] positions (default all); lse [n, n_heads] fp32."""
+        n, heads, _ = q.shape
+        d = self.book.device
+        act = _ACT.get(q.dtype)
+        if act is None:
+            raise ValueError(f"q: float32, float16 or bfloat16, got {q.dtype}")
+        qp, qs = self._rows(q, "q", n, q.dtype, heads)
+        op, os_ = self._rows(out, "out", n, q.dtype, heads)
+        lp = None
+        if lse is not None:
+            if lse.dtype is not torch.float32 or lse.shape != (n, heads) or lse.device != d or not lse.is_contiguous():
+                raise ValueError(f"lse: contiguous float32 of {(n, heads)}")
+            lp = lse.data_ptr()
+        sc = self._scratch.get(heads)
+        if sc is None:
+            with torch.cuda.device(d):
+                nbytes = lib().bmo_k_paged_attention_scratch_bytes(self._ref, heads)
+            if nbytes == 0:
+                raise ValueError(f"{heads} query heads over {self.n_kv_heads} key heads of {self.head_dim}")
+            sc = self._scratch[heads] = torch.zeros(nbytes, dtype=torch.uint8, device=d)
+            torch.cuda.current_stream(d).synchronize()  # later calls may be on another stream
+        _call(d, lib().bmo_k_paged_attention, self._ref, layer, n, qp, qs, heads,
+              None if rows is None else _ints(rows, "rows", d, n),
+              None if row_lens is None else _ints(row_lens, "row_lens", d, n), scale, op, os_, lp, act,
+              _status(status, d), sc.data_ptr(), sc.numel())

@@ -160,6 +160,105 @@ BMO_API int bmo_k_tp_exchange(const double *const *parts, unsigned long long *co
 BMO_API int bmo_k_sample_token(const float *logits_dev, int n, float temp, int top_k, int pause_rule,
                                uint32_t *rng_dev, int32_t *out_dev, void *stream);
 
+/* ---- paged key-value cache ----------------------------------------------
+ *
+ * A cache of any number of sessions ("requests") that share one pool of
+ * pages instead of owning a ring each.  A page holds page_size positions of
+ * every layer; a page of one layer is laid out as a ring of page_size slots
+ * (bmo_k_decode_attention): [n_layers][n_pages][n_kv_heads][page_size][head_dim]
+ * in fp16 (kv_type 0), or Q4_0 nibble planes (head_dim / 2 bytes a row) with
+ * fp16 scale planes [..][head_dim / 32] (kv_type 1).  Position p of request r
+ * is in page table[r][p / page_size] at slot p % page_size; a "slot number"
+ * is page * page_size + slot.  head_dim 64 or 128; page_size 1..65536;
+ * n_pages * page_size and max_blocks * page_size below 2^31.
+ * No counterpart in the reference, which decodes one session. */
+
+/* Element types of the activations of the paged calls (q, k, v, outputs). */
+enum { BMO_ACT_F32 = 0, BMO_ACT_F16 = 1, BMO_ACT_BF16 = 2 };
+
+/* Bits of the status words of the paged calls. */
+enum {
+    BMO_PAGED_NO_PAGES = 1 << 5,   /* plan: the step needs more pages than are free */
+    BMO_PAGED_TABLE_FULL = 1 << 6, /* plan: a request would outgrow max_blocks pages */
+    BMO_PAGED_NO_ROOM = 1 << 7,    /* plan: more new positions than max_tokens */
+    BMO_PAGED_BAD_INDEX = 1 << 8   /* a length, request, page or slot number out of range; the access was left out */
+};
+
+/* Which request has which pages.  All arrays are device memory. */
+typedef struct bmo_page_book {
+    int32_t *table;      /* [n_req][max_blocks] page of each block; entries outside a request's window are stale */
+    int32_t *lens;       /* [n_req] positions each request holds */
+    int32_t *free_pages; /* [n_pages] ring of page numbers */
+    int32_t *state;      /* [4]: first free entry of the ring, free pages, status bits, new positions of the step */
+    int32_t n_req, max_blocks, n_pages, page_size;
+    int32_t window; /* > 0: a token attends to the last `window` positions, its own included; 0: to all */
+} bmo_page_book;
+
+typedef struct bmo_paged_kv {
+    bmo_page_book book;
+    void *k, *v;             /* device, 16-byte aligned */
+    void *k_scale, *v_scale; /* kv_type 1 only */
+    int32_t n_layers, n_kv_heads, head_dim, kv_type;
+} bmo_paged_kv;
+
+/* Plans one step on the device: n_new_dev[r] > 0 appends that many positions
+ * to request r, 0 leaves it, < 0 ends it (its length becomes 0).  Pages for
+ * the new positions are taken from the ring of free pages in request order;
+ * pages that fall out of the window of the next step's tokens, and those of ended
+ * requests, are put at the ring's end.  A page given back in a step keeps its rows
+ * during the step: it can be taken again from the next plan on.  The new
+ * positions are listed request by request: entry i of slot_dev, pos_dev and
+ * req_dev [max_tokens] is its slot number, position and request (-1 past the
+ * last), offsets_dev [n_req + 1] is each request's first entry.
+ * lens_out_dev [n_req] and state_out_dev [4] receive the new lengths and
+ * state; they may be book->lens and book->state.  A step that cannot be
+ * served changes nothing but state_out[2], which says why
+ * (BMO_PAGED_* bits), and lists no positions.  n_req <= 65536. */
+BMO_API int bmo_k_paged_plan(const bmo_page_book *book, const int32_t *n_new_dev, int max_tokens, int32_t *slot_dev,
+                             int32_t *pos_dev, int32_t *req_dev, int32_t *offsets_dev, int32_t *lens_out_dev,
+                             int32_t *state_out_dev, void *stream);
+
+/* Stores n rows k_dev, v_dev [n][n_kv_heads][head_dim] (rows k_stride,
+ * v_stride elements apart, act_type BMO_ACT_*) at slot_dev[i] of `layer`;
+ * slot -1 leaves a row out.  theta > 0: k is rotated first by pos_dev[i]
+ * (interleaved pairs, angles and products as the exact-order decode step),
+ * and q_dev [n][n_heads][head_dim], if not NULL, is rotated into q_out_dev
+ * (which may be q_dev).  fp16 rounding and Q4_0 packing are the ring's.  Two
+ * rows of one call must not have the same slot.  status_dev (optional,
+ * device int) receives BMO_PAGED_BAD_INDEX for slots outside the cache. */
+BMO_API int bmo_k_paged_append(const bmo_paged_kv *cache, int layer, int n, const void *k_dev, long long k_stride,
+                               const void *v_dev, long long v_stride, const int32_t *slot_dev, const int32_t *pos_dev,
+                               float theta, const void *q_dev, long long q_stride, int n_heads, void *q_out_dev,
+                               long long q_out_stride, int act_type, int *status_dev, void *stream);
+
+/* Reads the rows at slot_dev[0, n) of `layer` back: k_out_dev, v_out_dev
+ * [n][n_kv_heads][head_dim], dense, in act_type; slot -1 and slots outside
+ * the cache read as zeros (the latter set BMO_PAGED_BAD_INDEX). */
+BMO_API int bmo_k_paged_read(const bmo_paged_kv *cache, int layer, int n, const int32_t *slot_dev, void *k_out_dev,
+                             void *v_out_dev, int act_type, int *status_dev, void *stream);
+
+/* Scratch bytes of bmo_k_paged_attention on the current device (0: the cache
+ * is not one it accepts). */
+BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, int n_heads);
+/* Attention of single tokens over the pages of `layer`: row i of q_dev
+ * [n_rows][n_heads][head_dim] attends to the last `window` (book.window; 0:
+ * all) of the first row_len_dev[i] positions of request row_req_dev[i].
+ * row_req_dev NULL: row i is request i; row_len_dev NULL: the request's
+ * length.  So several rows may be tokens of one request.  Query head h reads
+ * key head h / (n_heads / n_kv_heads); scale 0 means 1 / sqrt(head_dim).
+ * out_dev [n_rows][n_heads][head_dim] in act_type; lse_dev (optional, fp32
+ * [n_rows][n_heads]) receives log(sum(exp(score))).  A row of length 0 gives
+ * zeros and -inf.  Rows are q_stride, out_stride elements apart.  Slots
+ * past a request's length are never read.  Sums, maxima and products are fp32
+ * (each fp32 factor as two fp16 parts); the result is the same from call to
+ * call.  scratch_dev must be zero on the first call, is left reusable, and
+ * serves one call at a time.  n_rows <= 4096.  status_dev as above. */
+BMO_API int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, const void *q_dev,
+                                  long long q_stride, int n_heads, const int32_t *row_req_dev,
+                                  const int32_t *row_len_dev, float scale, void *out_dev, long long out_stride,
+                                  float *lse_dev, int act_type, int *status_dev, void *scratch_dev,
+                                  size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
