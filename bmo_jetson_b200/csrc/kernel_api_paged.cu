@@ -193,7 +193,9 @@ int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, cons
     if (n_rows == 0) return 0;
     // tile numbers of a call stay within 32 bits
     const long long positions = static_cast<long long>(b.max_blocks) * b.page_size;
-    if (n_rows * (positions / 16 + 1) > INT_MAX || static_cast<long long>(n_rows) * n_heads > INT_MAX / 2) return kInvalid;
+    if (n_rows * (positions / 16 + 1) > INT_MAX || n_heads * (positions / 16 + 1) > UINT_MAX ||
+        static_cast<long long>(n_rows) * n_heads > INT_MAX / 2)
+        return kInvalid;
     const int hd = cache->head_dim;
     if (!rows_ok(q_dev, n_rows, q_stride, n_heads, hd, elem) || !rows_ok(out_dev, n_rows, out_stride, n_heads, hd, elem) ||
         !scratch_dev || !aligned(scratch_dev, 16))

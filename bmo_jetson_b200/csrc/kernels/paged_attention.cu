@@ -86,6 +86,8 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
 // Transpose of an 8 x 8 matrix of 16-bit elements held two a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -192,39 +194,37 @@ struct F16Rows {
     float inv[NB];
     uint4 kr[kSub][2][HD / 32], vr[kSub][4][HD / 64];
 
-    __device__ __forceinline__ void load_q(const PagedAttnArgs &a, int row, int head0, int n_heads, int lane) {
+    // B fragments from the unit's queries qs[head][HD]; columns of heads past n_heads are zero.
+    __device__ __forceinline__ void load_q(const float *qs, int n_heads, float qscale, int lane) {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int h = 4 * nb + (g >> 1);
+            const float4 *src = reinterpret_cast<const float4 *>(qs + (h < n_heads ? h : 0) * HD + 8 * t);
             float x[HD / 4];
             float amax = 0.0f;
 #pragma unroll
-            for (int i = 0; i < HD / 4; ++i) x[i] = 0.0f;
-            if (h < n_heads) {
-                const long long base = row * a.q_stride + static_cast<long long>(head0 + h) * HD + 8 * t;
+            for (int c = 0; c < HD / 32; ++c)
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const float4 f = act_load4(a.q, a.act, base + 32 * c + 4 * u, a.q_vec);
-                        x[8 * c + 4 * u] = f.x * a.qscale, x[8 * c + 4 * u + 1] = f.y * a.qscale;
-                        x[8 * c + 4 * u + 2] = f.z * a.qscale, x[8 * c + 4 * u + 3] = f.w * a.qscale;
-                    }
-            }
+                for (int u = 0; u < 2; ++u) {
+                    const float4 f = src[8 * c + u];
+                    x[8 * c + 4 * u] = f.x, x[8 * c + 4 * u + 1] = f.y;
+                    x[8 * c + 4 * u + 2] = f.z, x[8 * c + 4 * u + 3] = f.w;
+                }
 #pragma unroll
             for (int i = 0; i < HD / 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
             float mul, iv;
             range_factor(amax, mul, iv);
-            inv[nb] = __shfl_sync(0xffffffffu, iv, 8 * t);  // of head t, from lane (g = 2t, 0)
+            inv[nb] = __shfl_sync(0xffffffffu, iv, 8 * t) * qscale;  // of head t, from lane (g = 2t, 0)
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {  // element pairs (2i, 2i + 1) of this lane
-                const float y0 = x[2 * i] * mul, y1 = x[2 * i + 1] * mul;
-                __half h0 = __float2half_rn(y0), h1 = __float2half_rn(y1);
-                if (g & 1) h0 = __float2half_rn(y0 - __half2float(h0)), h1 = __float2half_rn(y1 - __half2float(h1));
-                q[nb][i / 2][i % 2] = half_bits2(h0, h1);
+                const float y0 = h < n_heads ? x[2 * i] * mul : 0.0f, y1 = h < n_heads ? x[2 * i + 1] * mul : 0.0f;
+                __half2 h2 = __floats2half2_rn(y0, y1);
+                const float2 f = __half22float2(h2);
+                if (g & 1) h2 = __floats2half2_rn(y0 - f.x, y1 - f.y);
+                q[nb][i / 2][i % 2] = *reinterpret_cast<const uint32_t *>(&h2);
             }
         }
     }
@@ -266,28 +266,33 @@ struct F16Rows {
     __device__ __forceinline__ bool value_range(int) { return false; }
     __device__ __forceinline__ void raise_value_range(float (&)[NB][kO][4]) {}
     __device__ __forceinline__ void reset() {}
-    __device__ __forceinline__ void values(int s, const float (&w)[NB][2], float (&o)[NB][kO][4]) {
-        uint32_t b[NB][2];
+    // Adds the weighted values of the tile.  The tensor core's sum of a tile
+    // starts from zero and is added in fp32: its own running sum is not rounded to nearest.
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
+        uint32_t b[kSub][NB][2];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            b[nb][0] = transpose8(split_half(w[nb][0]));
-            b[nb][1] = transpose8(split_half(w[nb][1]));
-        }
+        for (int s = 0; s < kSub; ++s)
 #pragma unroll
-        for (int c = 0; c < HD / 64; ++c) {
-            const uint4 *v0 = &vr[s][0][c], *v1 = &vr[s][1][c], *v2 = &vr[s][2][c], *v3 = &vr[s][3][c];
-#define BMO_PV(j, f)                                                                              \
-    {                                                                                             \
-        const uint32_t a0 = __byte_perm(v0->f, v1->f, 0x5410), a1 = __byte_perm(v0->f, v1->f, 0x7632); \
-        const uint32_t a2 = __byte_perm(v2->f, v3->f, 0x5410), a3 = __byte_perm(v2->f, v3->f, 0x7632); \
-        _Pragma("unroll") for (int nb = 0; nb < NB; ++nb)                                         \
-            mma16816(o[nb][4 * c + j], a0, a1, a2, a3, b[nb][0], b[nb][1]);                       \
-    }
-            BMO_PV(0, x)
-            BMO_PV(1, y)
-            BMO_PV(2, z)
-            BMO_PV(3, w)
-#undef BMO_PV
+            for (int nb = 0; nb < NB; ++nb) {
+                b[s][nb][0] = transpose8(split_half(w[s][nb][0]));
+                b[s][nb][1] = transpose8(split_half(w[s][nb][1]));
+            }
+#pragma unroll
+        for (int j = 0; j < kO; ++j) {
+            float sum[NB][4] = {};
+#pragma unroll
+            for (int s = 0; s < kSub; ++s) {
+                const uint32_t v0 = word(vr[s][0][j / 4], j % 4), v1 = word(vr[s][1][j / 4], j % 4),
+                               v2 = word(vr[s][2][j / 4], j % 4), v3 = word(vr[s][3][j / 4], j % 4);
+                const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
+                const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) mma16816(sum[nb], a0, a1, a2, a3, b[s][nb][0], b[s][nb][1]);
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[nb][j][i] += sum[nb][i];
         }
     }
     // The lane's 8 consecutive elements [64 c + 8 g, + 8) of head (nb, t).
@@ -307,7 +312,7 @@ struct Q4Rows {
     static constexpr int HD = HD_, NB = 1;
     static constexpr int kMinCtas = 3;
     static constexpr int kHeads = 1;
-    static constexpr int kSub = 4;
+    static constexpr int kSub = 2;
     static constexpr int kO = HD / 16;
     static constexpr int kBlocks = HD / 32;       // <= 4: a column pair each
     static constexpr int kKW = HD / 32;           // words of a key row a lane holds
@@ -318,22 +323,19 @@ struct Q4Rows {
     uint32_t kr[kSub][2][kKW], vr[kSub][4][kVW];
     __half ks[kSub][2], vs[kSub][2];
 
-    __device__ __forceinline__ void load_q(const PagedAttnArgs &a, int row, int head0, int, int lane) {
+    __device__ __forceinline__ void load_q(const float *qs, int, float qscale, int lane) {
         const int g = lane >> 2, t = lane & 3;
         // lane t holds words of block blk from byte `byte`; column pair g / 2 is block g / 2
         const int blk = HD == 128 ? t : t >> 1, byte = HD == 128 ? 0 : 8 * (t & 1);
         const bool mine = (g >> 1) == blk;
         float lo[4 * kKW], hi[4 * kKW];  // elements byte + i and 16 + byte + i of the block
         float amax = 0.0f;
-        const long long base = row * a.q_stride + static_cast<long long>(head0) * HD + 32 * blk + byte;
+        const float4 *src = reinterpret_cast<const float4 *>(qs + 32 * blk + byte);
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
-            const float4 x = act_load4(a.q, a.act, base + 4 * w, a.q_vec);
-            const float4 y = act_load4(a.q, a.act, base + 16 + 4 * w, a.q_vec);
-            lo[4 * w] = x.x * a.qscale, lo[4 * w + 1] = x.y * a.qscale;
-            lo[4 * w + 2] = x.z * a.qscale, lo[4 * w + 3] = x.w * a.qscale;
-            hi[4 * w] = y.x * a.qscale, hi[4 * w + 1] = y.y * a.qscale;
-            hi[4 * w + 2] = y.z * a.qscale, hi[4 * w + 3] = y.w * a.qscale;
+            const float4 x = src[w], y = src[4 + w];
+            lo[4 * w] = x.x, lo[4 * w + 1] = x.y, lo[4 * w + 2] = x.z, lo[4 * w + 3] = x.w;
+            hi[4 * w] = y.x, hi[4 * w + 1] = y.y, hi[4 * w + 2] = y.z, hi[4 * w + 3] = y.w;
         }
 #pragma unroll
         for (int i = 0; i < 4 * kKW; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
@@ -341,6 +343,7 @@ struct Q4Rows {
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float mul;
         range_factor(amax, mul, inv);
+        inv *= qscale;
         auto part = [&](float x) {
             const float y = mine ? x * mul : 0.0f;
             const __half h = __float2half_rn(y);
@@ -425,19 +428,27 @@ struct Q4Rows {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[0][j][i] *= f;
     }
-    __device__ __forceinline__ void values(int s, const float (&w)[NB][2], float (&o)[NB][kO][4]) {
-        // w / vlim * scale <= 2^15
-        const uint32_t b0 = transpose8(split_half(w[0][0] * (__half2float(vs[s][0]) * vinv)));
-        const uint32_t b1 = transpose8(split_half(w[0][1] * (__half2float(vs[s][1]) * vinv)));
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
+        uint32_t b[kSub][2];
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)  // w * scale / vlim <= 2^15
+                b[s][i] = transpose8(split_half(w[s][0][i] * (__half2float(vs[s][i]) * vinv)));
 #pragma unroll
         for (int i = 0; i < kVW; ++i) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t x = __byte_perm(vr[s][0][i], vr[s][1][i], u ? 0x7632 : 0x5410);
-                const uint32_t y = __byte_perm(vr[s][2][i], vr[s][3][i], u ? 0x7632 : 0x5410);
-                mma16816(o[0][4 * i + 2 * u], codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y), b0, b1);
-                mma16816(o[0][4 * i + 2 * u + 1], codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8),
-                         codes_hi(y >> 8), b0, b1);
+                float even[4] = {}, odd[4] = {};
+#pragma unroll
+                for (int s = 0; s < kSub; ++s) {
+                    const uint32_t x = __byte_perm(vr[s][0][i], vr[s][1][i], u ? 0x7632 : 0x5410);
+                    const uint32_t y = __byte_perm(vr[s][2][i], vr[s][3][i], u ? 0x7632 : 0x5410);
+                    mma16816(even, codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y), b[s][0], b[s][1]);
+                    mma16816(odd, codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8), b[s][0], b[s][1]);
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[0][4 * i + 2 * u][c] += even[c], o[0][4 * i + 2 * u + 1][c] += odd[c];
             }
         }
     }
@@ -460,21 +471,43 @@ struct Q4Rows {
 template <int HD, int NH>
 struct PaSmem {
     static constexpr int kPieces = 2 * kPaWarps;
+    float buf[kPaWarps][NH * HD];            // a warp's queries, then its outputs
+    float bm[kPaWarps][NH], bl[kPaWarps][NH];
     float m[kPieces][NH], l[kPieces][NH];
-    float o[kPieces][NH][HD];
+    float o[kPieces][NH * HD];
+    float4 red[kPaThreads];
+    float red_m[kPaThreads], red_l[kPaThreads];
     int seg[kPieces];    // row * units + unit, -1: none
     int whole[kPieces];  // bit 0: begins at the head's first tile, bit 1: ends at its last
-    int join[2];         // this CTA is the last to arrive: global slot kind 0 / 1
+    int join[2];         // 1 + the head that this CTA, last to arrive, joins
 };
 
-constexpr int kJoinMax = 640;  // pieces a head can have: CTAs of a launch
+constexpr int kMaxGrid = 640;
 
-template <int HD, int NH>
-struct PaJoin {  // replaces the pieces when a CTA joins a head
-    float w[kJoinMax * NH];
-    float l[kJoinMax * NH];
-    float mm[NH], ll[NH];
+// Running join of pieces (m, l, o): sums relative to the maximum so far.
+struct Joined {
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    __device__ __forceinline__ void scale_to(float top) {
+        const float f = m == top ? 1.0f : ex2(m - top);
+        m = top;
+        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+    }
+    __device__ __forceinline__ void add(float pm, float pl, float4 po) {  // pm <= m
+        const float f = pm == m ? 1.0f : ex2(pm - m);
+        l += f * pl, o.x += f * po.x, o.y += f * po.y, o.z += f * po.z, o.w += f * po.w;
+    }
 };
+
+__device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m - kHead + log2f(l)) * kLn2; }
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+// Release of the CTA's earlier writes (ordered by a barrier before it) and acquire of the others'.
+__device__ __forceinline__ int arrive(int *p) {
+    int v;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ int pa_len(const PagedAttnArgs &a, int row, int &req, bool &bad) {
     req = a.row_req ? a.row_req[row] : row;
@@ -493,8 +526,7 @@ __device__ __forceinline__ int pa_len(const PagedAttnArgs &a, int row, int &req,
 }
 
 template <int HD, int NH>
-constexpr size_t kFixedSmem =
-    ((sizeof(PaSmem<HD, NH>) > sizeof(PaJoin<HD, NH>) ? sizeof(PaSmem<HD, NH>) : sizeof(PaJoin<HD, NH>)) + 15) / 16 * 16;
+constexpr size_t kFixedSmem = (sizeof(PaSmem<HD, NH>) + 15) / 16 * 16;
 
 // A piece in global memory: [heads][HD] sums, then the maxima and the weights' sums; 16-byte multiples.
 template <class R>
@@ -548,9 +580,25 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     if (bad) raise_error(a.status, kErrBadIndex);
     const long long total = static_cast<long long>(ends[a.n_rows - 1]) * units;
     const int n_warps = gridDim.x * kPaWarps;
-    const long long per = max(1ll, (total + n_warps - 1) / n_warps);
+    const long long per = total >> 32 ? (total + n_warps - 1) / n_warps
+                                      : max(1u, (static_cast<uint32_t>(total) + n_warps - 1) / n_warps);
     long long u = min(total, (static_cast<long long>(blockIdx.x) * kPaWarps + warp) * per);
     const long long u_end = min(total, u + per);
+    // of a head: its query heads, its tiles on the line, and the CTAs these lie in
+    struct Head {
+        int row, head0, heads, kh, row0, n_tiles;
+    };
+    auto head_of_seg = [&](int row, int unit) {
+        Head h;
+        h.row = row;
+        h.kh = chunks == 1 ? unit : unit / chunks;
+        const int chunk = unit - h.kh * chunks;
+        h.head0 = h.kh * group + chunk * NH;
+        h.heads = min(NH, group - chunk * NH);
+        h.row0 = row ? ends[row - 1] : 0;
+        h.n_tiles = ends[row] - h.row0;
+        return h;
+    };
 
     // rows without a position
     for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
@@ -576,17 +624,17 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         }
         const int row0 = row ? ends[row - 1] : 0;
         const int n_tiles = ends[row] - row0;
-        const long long rem = u - static_cast<long long>(row0) * units;
-        const int unit = static_cast<int>(rem / n_tiles);
-        const int tile0 = static_cast<int>(rem - static_cast<long long>(unit) * n_tiles);
+        const uint32_t rem = static_cast<uint32_t>(u - static_cast<long long>(row0) * units);
+        const int unit = rem / n_tiles;
+        const int tile0 = rem - unit * n_tiles;
         const int tile1 = static_cast<int>(min(static_cast<long long>(n_tiles), tile0 + (u_end - u)));
         u += tile1 - tile0;
+        const Head hd = head_of_seg(row, unit);
+        const int kh = hd.kh, head0 = hd.head0, heads = hd.heads;
         int req, start, len;
         len = pa_len(a, row, req, bad);
         start = a.window > 0 ? max(0, len - a.window) : 0;
         const int base_tile = start / kTile;
-        const int kh = unit / chunks, chunk = unit - kh * chunks;
-        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
 
         Pages pg;
         pg.table = a.table + static_cast<long long>(req) * a.max_blocks;
@@ -595,6 +643,12 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             pg.entry = b + lane < a.max_blocks ? pg.table[b + lane] : -1;
         };
         refill(static_cast<int>(pa_div(max(start, (base_tile + tile0) * kTile), a.page)));
+        float *buf = S.buf[warp];
+        __syncwarp();
+        for (int i = lane; i < heads * HD / 4; i += 32)
+            *reinterpret_cast<float4 *>(buf + 4 * i) =
+                act_load4(a.q, a.act, row * a.q_stride + static_cast<long long>(head0) * HD + 4 * i, a.q_vec);
+        __syncwarp();
         // rows of the 16 positions from p0; those outside [start, len) and those of invalid pages: -1
         auto locate = [&](int p0, Pos16 &P) {
             const int first = max(p0, start), last = min(p0 + 15, len - 1);
@@ -646,7 +700,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             locate(pbase + tile0 * kTile + 16 * s, P[s]);
             R_.load_k(a, s, P[s], lane);
         }
-        R_.load_q(a, row, head0, heads, lane);
+        R_.load_q(buf, heads, a.qscale, lane);
         for (int tile = tile0; tile < tile1; ++tile) {
 #pragma unroll
             for (int s = 0; s < R::kSub; ++s) R_.load_v(a, s, P[s], lane);
@@ -694,209 +748,179 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             for (int s = 0; s < R::kSub; ++s) wide |= R_.value_range(s);
             if (__any_sync(0xffffffffu, wide)) R_.raise_value_range(o);
 #pragma unroll
-            for (int s = 0; s < R::kSub; ++s) {
-                float w[NB][2];
+            for (int nb = 0; nb < NB; ++nb) {
+                const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
-                    w[nb][0] = ex2(sc[s][nb][0] - ref);
-                    w[nb][1] = ex2(sc[s][nb][1] - ref);
-                    l[nb] += w[nb][0] + w[nb][1];
+                for (int s = 0; s < R::kSub; ++s) {
+                    sc[s][nb][0] = ex2(sc[s][nb][0] - ref);
+                    sc[s][nb][1] = ex2(sc[s][nb][1] - ref);
+                    l[nb] += sc[s][nb][0] + sc[s][nb][1];
                 }
-                R_.values(s, w, o);
             }
+            R_.values(sc, o);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], d);
 
-        // ---- a whole head goes out, a piece into shared memory ----
-        const bool begins = tile0 == 0, finishes = tile1 == n_tiles;
+        // ---- a piece stays in shared memory, a whole head goes out through it ----
+        const bool begins = tile0 == 0, finishes = tile1 == n_tiles, whole = begins && finishes;
         const int slot = 2 * warp + (begins ? 1 : 0);
-        if (!(begins && finishes) && lane == 0) {
+        if (!whole && lane == 0) {
             S.seg[slot] = row * units + unit;
             S.whole[slot] = (begins ? 1 : 0) | (finishes ? 2 : 0);
         }
+        float *dst = whole ? buf : S.o[slot], *dst_m = whole ? S.bm[warp] : S.m[slot], *dst_l = whole ? S.bl[warp] : S.l[slot];
+        __syncwarp();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int h = R::head_of(nb, lane);
-            if (begins && finishes) {
-                if (h < heads) {
-                    const float f = l[nb] == 0.0f ? 0.0f : 1.0f / l[nb];
-                    if (R_.owns(lane)) {
-                        const long long out0 = row * a.out_stride + static_cast<long long>(head0 + h) * HD;
+            if (h >= heads) continue;
+            if (R_.owns(lane)) {
 #pragma unroll
-                        for (int run = 0; run < R::kRuns; ++run)
+                for (int run = 0; run < R::kRuns; ++run)
 #pragma unroll
-                            for (int i = 0; i < R::kRunLen; i += 4)
-                                act_store4(a.out, a.act, out0 + R::run_start(run, lane) + i,
-                                           make_float4(R_.element(o[nb], run, i) * f, R_.element(o[nb], run, i + 1) * f,
-                                                       R_.element(o[nb], run, i + 2) * f, R_.element(o[nb], run, i + 3) * f),
-                                           a.out_vec);
-                    }
-                    if (a.lse && g == 0 && (NH > 1 || t == 0))
-                        a.lse[static_cast<long long>(row) * a.n_heads + head0 + h] =
-                            l[nb] == 0.0f ? -INFINITY : (m[nb] - kHead + log2f(l[nb])) * kLn2;
-                }
-            } else {
-                if (R_.owns(lane)) {
-#pragma unroll
-                    for (int run = 0; run < R::kRuns; ++run)
-#pragma unroll
-                        for (int i = 0; i < R::kRunLen; i += 4)
-                            *reinterpret_cast<float4 *>(&S.o[slot][h][R::run_start(run, lane) + i]) =
-                                make_float4(R_.element(o[nb], run, i), R_.element(o[nb], run, i + 1),
-                                            R_.element(o[nb], run, i + 2), R_.element(o[nb], run, i + 3));
-                }
-                if (g == 0 && (NH > 1 || t == 0)) S.m[slot][h] = m[nb], S.l[slot][h] = l[nb];
+                    for (int i = 0; i < R::kRunLen; i += 4)
+                        *reinterpret_cast<float4 *>(dst + h * HD + R::run_start(run, lane) + i) =
+                            make_float4(R_.element(o[nb], run, i), R_.element(o[nb], run, i + 1),
+                                        R_.element(o[nb], run, i + 2), R_.element(o[nb], run, i + 3));
             }
+            if (g == 0 && (NH > 1 || t == 0)) dst_m[h] = m[nb], dst_l[h] = l[nb];
+        }
+        __syncwarp();
+        if (whole) {
+            for (int i = lane; i < heads * HD / 4; i += 32) {
+                const float4 x = *reinterpret_cast<const float4 *>(buf + 4 * i);
+                const float f = inverse_of(dst_l[4 * i / HD]);
+                act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0) * HD + 4 * i,
+                           make_float4(x.x * f, x.y * f, x.z * f, x.w * f), a.out_vec);
+            }
+            if (a.lse && lane < heads)
+                a.lse[static_cast<long long>(row) * a.n_heads + head0 + lane] = lse_of(dst_m[lane], dst_l[lane]);
         }
     }
     if (bad) raise_error(a.status, kErrBadIndex);
     __syncthreads();
 
-    // ---- pieces of one head within the CTA: joined by the warp that holds the first ----
-    const long long cta_tiles = per * kPaWarps;
+    // ---- the CTA's pieces of one head, joined; one that other CTAs hold too goes to global memory ----
     constexpr int kPieceFloats = pa_piece_floats<R>;
-    for (int i = 2 * warp; i < 2 * warp + 2; ++i) {
+    const long long cta_tiles = per * kPaWarps;
+    auto cta_of = [&](long long tile) {
+        return static_cast<int>(tile >> 32 || cta_tiles >> 32 ? tile / cta_tiles
+                                                              : static_cast<uint32_t>(tile) / static_cast<uint32_t>(cta_tiles));
+    };
+    auto finish = [&](const Head &h, int c, const Joined &j) {  // column c: 4 elements
+        const float f = inverse_of(j.l);
+        act_store4(a.out, a.act, h.row * a.out_stride + static_cast<long long>(h.head0) * HD + 4 * c,
+                   make_float4(j.o.x * f, j.o.y * f, j.o.z * f, j.o.w * f), a.out_vec);
+        if (a.lse && 4 * c % HD == 0)
+            a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + 4 * c / HD] = lse_of(j.m, j.l);
+    };
+    int open[2] = {0, 0};  // 1 + heads of which this CTA has a part: one that began earlier, one that begins here
+    for (int i = 0; i < Smem::kPieces;) {
         const int seg = S.seg[i];
-        if (seg < 0) continue;
-        int before = i - 1;
-        while (before >= 0 && S.seg[before] < 0) --before;
-        if (before >= 0 && S.seg[before] == seg) continue;
-        int last = i;
-        for (int j = i + 1; j < Smem::kPieces; ++j)
-            if (S.seg[j] == seg) last = j;
-        const bool begins = S.whole[i] & 1, finishes = S.whole[last] & 2;
-        const int row = seg / units, unit = seg - row * units;
-        const int kh = unit / chunks, chunk = unit - kh * chunks;
-        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
-        float *dst = a.part + (2ll * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
-        for (int h = 0; h < heads; ++h) {
-            float M = -INFINITY, L = 0.0f;
-            for (int j = i; j <= last; ++j)
-                if (S.seg[j] == seg) M = fmaxf(M, S.m[j][h]);
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int d = 4 * lane;
-            for (int j = i; j <= last; ++j) {
-                if (S.seg[j] != seg) continue;
-                const float f = S.m[j][h] == M ? 1.0f : ex2(S.m[j][h] - M);
-                L += f * S.l[j][h];
-                if (d < HD) {
-                    const float4 x = *reinterpret_cast<const float4 *>(&S.o[j][h][d]);
-                    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+        int last = i, next = i + 1;
+        if (seg >= 0)
+            for (; next < Smem::kPieces && (S.seg[next] == seg || S.seg[next] < 0); ++next)
+                if (S.seg[next] == seg) last = next;
+        if (seg >= 0) {
+            const bool begins = S.whole[i] & 1, finishes = S.whole[last] & 2;
+            const Head h = head_of_seg(seg / units, seg % units);
+            float *dst = a.part + (2ll * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
+            for (int c = tid; c < h.heads * HD / 4; c += kPaThreads) {
+                const int hh = 4 * c / HD;
+                Joined j;
+                for (int k = i; k <= last; ++k)
+                    if (S.seg[k] == seg) j.m = fmaxf(j.m, S.m[k][hh]);
+                for (int k = i; k <= last; ++k)
+                    if (S.seg[k] == seg) j.add(S.m[k][hh], S.l[k][hh], *reinterpret_cast<const float4 *>(&S.o[k][4 * c]));
+                if (begins && finishes) {
+                    finish(h, c, j);
+                } else {
+                    __stcg(reinterpret_cast<float4 *>(dst + 4 * c), j.o);
+                    if (4 * c % HD == 0) {
+                        __stcg(dst + NH * HD + hh, j.m);
+                        __stcg(dst + NH * HD + NH + hh, j.l);
+                    }
                 }
             }
-            if (begins && finishes) {
-                const float f = L == 0.0f ? 0.0f : 1.0f / L;
-                if (d < HD)
-                    act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0 + h) * HD + d,
-                               make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec);
-                if (a.lse && lane == 0)
-                    a.lse[static_cast<long long>(row) * a.n_heads + head0 + h] =
-                        L == 0.0f ? -INFINITY : (M - kHead + log2f(L)) * kLn2;
-            } else {
-                if (d < HD) __stcg(reinterpret_cast<float4 *>(dst + h * HD + d), acc);
-                if (lane == 0) {
-                    __stcg(dst + NH * HD + h, M);
-                    __stcg(dst + NH * HD + NH + h, L);
-                }
-            }
+            if (!(begins && finishes)) open[begins ? 1 : 0] = seg + 1;
         }
-        if (!(begins && finishes)) {
-            // the head's tiles on the line and the CTAs they lie in
-            const int row0 = row ? ends[row - 1] : 0, n_tiles = ends[row] - row0;
-            const long long first = static_cast<long long>(row0) * units + static_cast<long long>(unit) * n_tiles;
-            const int c0 = static_cast<int>(first / cta_tiles), c1 = static_cast<int>((first + n_tiles - 1) / cta_tiles);
-            __threadfence();
-            __syncwarp();
-            if (lane == 0 && atomicAdd(a.cnt + c0, 1) == c1 - c0) {
-                a.cnt[c0] = 0;
-                S.join[begins ? 1 : 0] = seg + 1;
-            }
+        i = next;
+    }
+    if (!open[0] && !open[1]) return;
+    __syncthreads();
+    auto first_tile = [&](const Head &h, int seg) {
+        return static_cast<long long>(h.row0) * units + static_cast<long long>(seg % units) * h.n_tiles;
+    };
+    if (tid < 2 && open[tid]) {
+        const int seg = open[tid] - 1;
+        const Head h = head_of_seg(seg / units, seg % units);
+        const long long first = first_tile(h, seg);
+        const int c0 = cta_of(first), c1 = cta_of(first + h.n_tiles - 1);
+        if (arrive(a.cnt + c0) == c1 - c0) {
+            a.cnt[c0] = 0;
+            S.join[tid] = seg + 1;
         }
     }
     __syncthreads();
-    const int joins[2] = {S.join[0], S.join[1]};
-    if (!joins[0] && !joins[1]) return;
-    __threadfence();
 
     // ---- the last CTA to arrive joins the head's pieces, in line order ----
-    using Join = PaJoin<HD, NH>;
-    Join &J = *reinterpret_cast<Join *>(smem_raw);
-    __shared__ float4 red[kPaThreads];
     for (int k = 0; k < 2; ++k) {
-        if (!joins[k]) continue;
-        __syncthreads();
-        const int seg = joins[k] - 1;
-        const int row = seg / units, unit = seg - row * units;
-        const int kh = unit / chunks, chunk = unit - kh * chunks;
-        const int head0 = kh * group + chunk * NH, heads = min(NH, group - chunk * NH);
-        const int row0 = row ? ends[row - 1] : 0, n_tiles = ends[row] - row0;
-        const long long first = static_cast<long long>(row0) * units + static_cast<long long>(unit) * n_tiles;
-        const int c0 = static_cast<int>(first / cta_tiles), c1 = static_cast<int>((first + n_tiles - 1) / cta_tiles);
-        const int n = c1 - c0 + 1;
-        auto piece = [&](int i) { return a.part + (2ll * (c0 + i) + (i == 0 ? 1 : 0)) * kPieceFloats; };
-        for (int i = tid; i < n * heads; i += kPaThreads) {
-            const int p = i / heads, h = i - p * heads;
-            const float *src = piece(p) + NH * HD + h;
-            J.w[i] = __ldcg(src);
-            J.l[i] = __ldcg(src + NH);
-        }
-        __syncthreads();
-        for (int h = warp; h < heads; h += kPaWarps) {
-            float M = -INFINITY, L = 0.0f;
-            for (int p = lane; p < n; p += 32) M = fmaxf(M, J.w[p * heads + h]);
-            M = warp_max(M);
-            for (int p = lane; p < n; p += 32) {
-                const float x = J.w[p * heads + h];
-                const float f = x == M ? 1.0f : ex2(x - M);
-                J.w[p * heads + h] = f;
-                L += f * J.l[p * heads + h];
-            }
-            L = warp_sum(L);
-            if (lane == 0) J.mm[h] = M, J.ll[h] = L;
-        }
-        __syncthreads();
-        const int cols = heads * HD / 4;  // float4 columns
-        const int parts = max(1, kPaThreads / cols);
-        for (int c = tid % cols, part = tid / cols; c < cols; c += kPaThreads) {
-            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            const int h = 4 * c / HD;
+        const int seg = S.join[k] - 1;
+        if (seg < 0) continue;
+        const Head h = head_of_seg(seg / units, seg % units);
+        const long long first = first_tile(h, seg);
+        const int c0 = cta_of(first), n = cta_of(first + h.n_tiles - 1) - c0 + 1;
+        const int cols = h.heads * HD / 4;
+        const int parts = max(1, kPaThreads / cols);  // threads that share a column's pieces
+        const int part = tid / cols;
+        for (int c = tid - part * cols; c < cols; c += kPaThreads) {
+            const int hh = 4 * c / HD;
+            Joined j;
             if (part < parts) {
-#pragma unroll 8
-                for (int p = part; p < n; p += parts) {
-                    const float4 x = __ldcg(reinterpret_cast<const float4 *>(piece(p)) + c);
-                    const float f = J.w[p * heads + h];
-                    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                for (int p0 = part; p0 < n; p0 += 8 * parts) {
+                    float pm[8], pl[8];
+                    float4 po[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int p = p0 + i * parts;
+                        const float *src = a.part + (2ll * (c0 + (p < n ? p : 0)) + (p == 0 || p >= n ? 1 : 0)) * kPieceFloats;
+                        pm[i] = __ldcg(src + NH * HD + hh);
+                        pl[i] = __ldcg(src + NH * HD + NH + hh);
+                        po[i] = __ldcg(reinterpret_cast<const float4 *>(src + 4 * c));
+                    }
+                    float top = j.m;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (p0 + i * parts < n) top = fmaxf(top, pm[i]);
+                    j.scale_to(top);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (p0 + i * parts < n) j.add(pm[i], pl[i], po[i]);
                 }
             }
-            if (parts > 1) {
-                red[tid] = acc;
+            if (parts > 1) {  // one column a thread: every thread is here once
+                S.red[tid] = j.o, S.red_m[tid] = j.m, S.red_l[tid] = j.l;
                 __syncthreads();
-                if (part == 0)
-                    for (int q = 1; q < parts; ++q) {
-                        const float4 x = red[q * cols + c];
-                        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
-                    }
+                if (part == 0) {
+                    float top = j.m;
+                    for (int q = 1; q < parts; ++q) top = fmaxf(top, S.red_m[q * cols + c]);
+                    j.scale_to(top);
+                    for (int q = 1; q < parts; ++q) j.add(S.red_m[q * cols + c], S.red_l[q * cols + c], S.red[q * cols + c]);
+                }
+                __syncthreads();
             }
-            if (part == 0) {
-                const float f = J.ll[h] == 0.0f ? 0.0f : 1.0f / J.ll[h];
-                act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0) * HD + 4 * c,
-                           make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f), a.out_vec);
-            }
+            if (part == 0) finish(h, c, j);
         }
-        if (a.lse && tid < heads)
-            a.lse[static_cast<long long>(row) * a.n_heads + head0 + tid] =
-                J.ll[tid] == 0.0f ? -INFINITY : (J.mm[tid] - kHead + log2f(J.ll[tid])) * kLn2;
     }
 }
 
 constexpr int kMaxDevices = 64;
 
 // CTAs of a launch on the current device: all that are resident at once, at
-// most kJoinMax (0: the kernel cannot run here).
+// most kMaxGrid (0: the kernel cannot run here).
 template <class R>
 cudaError_t pa_grid(int &grid) {
     static std::atomic<int> known[kMaxDevices];
@@ -911,7 +935,7 @@ cudaError_t pa_grid(int &grid) {
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
     if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R>, kPaThreads, smem)) != cudaSuccess)
         return e;
-    grid = sms * per_sm < kJoinMax ? sms * per_sm : kJoinMax;
+    grid = sms * per_sm < kMaxGrid ? sms * per_sm : kMaxGrid;
     if (grid <= 0) return cudaErrorInvalidConfiguration;
     if (dev < kMaxDevices) known[dev].store(grid, std::memory_order_release);
     return cudaSuccess;

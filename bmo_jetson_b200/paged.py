@@ -26,6 +26,11 @@ NO_PAGES, TABLE_FULL, NO_ROOM, BAD_INDEX = 1 << 5, 1 << 6, 1 << 7, 1 << 8
 _ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+# the current stream's handle, without making a Stream object (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _Book(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lens", "free_pages", "state")] + \
                [(n, ctypes.c_int32) for n in ("n_req", "max_blocks", "n_pages", "page_size", "window")]
@@ -39,10 +44,10 @@ class _Cache(ctypes.Structure):
 def _call(device, fn, *args) -> None:
     """Runs a library call on `device` and its current stream."""
     if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, _raw_stream(device.index))
     if rc != 0:
         raise RuntimeError(f"{fn.__name__} rc={rc}")
 
