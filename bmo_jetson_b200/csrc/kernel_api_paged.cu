@@ -40,10 +40,6 @@ bool rows_ok(const void *p, int n, long long stride, int heads, int head_dim, si
     return p && aligned(p, elem) && (n <= 1 || stride >= static_cast<long long>(heads) * head_dim);
 }
 
-bool allows4(const void *p, int n, long long stride, size_t elem) {
-    return aligned(p, 4 * elem) && (n <= 1 || stride % 4 == 0);
-}
-
 // Element offset of `layer` in the caches.
 long long layer_rows(const bmo_paged_kv *c, int layer) {
     return static_cast<long long>(layer) * c->book.n_pages * c->n_kv_heads * c->book.page_size;
@@ -191,11 +187,9 @@ int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, cons
     const bmo_page_book &b = cache->book;
     if (!row_req_dev && n_rows > b.n_req) return kInvalid;
     if (n_rows == 0) return 0;
-    // tile numbers of a call stay within 32 bits
-    const long long positions = static_cast<long long>(b.max_blocks) * b.page_size;
-    if (n_rows * (positions / 16 + 1) > INT_MAX || n_heads * (positions / 16 + 1) > UINT_MAX ||
-        static_cast<long long>(n_rows) * n_heads > INT_MAX / 2)
-        return kInvalid;
+    // the kernel numbers the call's tiles (16 positions or more of a head) in 31 bits
+    const long long tiles = static_cast<long long>(b.max_blocks) * b.page_size / 16 + 1;
+    if (n_heads > 65536 || tiles * n_rows > INT_MAX / n_heads) return kInvalid;
     const int hd = cache->head_dim;
     if (!rows_ok(q_dev, n_rows, q_stride, n_heads, hd, elem) || !rows_ok(out_dev, n_rows, out_stride, n_heads, hd, elem) ||
         !scratch_dev || !aligned(scratch_dev, 16))
@@ -223,13 +217,10 @@ int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, cons
     a.n_rows = n_rows;
     a.n_heads = n_heads;
     a.n_kv_heads = cache->n_kv_heads;
-    a.act = act_type;
-    a.q_vec = allows4(q_dev, n_rows, q_stride, elem);
-    a.out_vec = allows4(out_dev, n_rows, out_stride, elem);
     const double sc = scale != 0.0f ? scale : 1.0 / std::sqrt(static_cast<double>(hd));
     a.qscale = static_cast<float>(sc * 1.4426950408889634);
     a.status = status_dev;
-    return static_cast<int>(launch_paged_attention(a, hd, cache->kv_type, scratch_dev, scratch_bytes,
+    return static_cast<int>(launch_paged_attention(a, hd, cache->kv_type, act_type, scratch_dev, scratch_bytes,
                                                    static_cast<cudaStream_t>(stream)));
 }
 

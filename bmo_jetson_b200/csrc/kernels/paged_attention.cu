@@ -119,43 +119,20 @@ __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-__device__ __forceinline__ float act_load(const void *p, int act, long long i) {
-    if (act == BMO_ACT_F32) return static_cast<const float *>(p)[i];
-    if (act == BMO_ACT_F16) return __half2float(static_cast<const __half *>(p)[i]);
-    return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
+// Activations are read and written an element a lane: a warp's accesses are
+// whole lines whatever the rows' alignment, and the code stays short.  (These kernels
+// run for a few microseconds and fetch their code cold on every SM.)
+template <int ACT>
+__device__ __forceinline__ float act_load(const void *p, long long i) {
+    if constexpr (ACT == BMO_ACT_F32) return static_cast<const float *>(p)[i];
+    else if constexpr (ACT == BMO_ACT_F16) return __half2float(static_cast<const __half *>(p)[i]);
+    else return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
 }
-// 4 elements from i (a multiple of 4 elements from an aligned start if vec).
-__device__ __forceinline__ float4 act_load4(const void *p, int act, long long i, bool vec) {
-    if (!vec) return make_float4(act_load(p, act, i), act_load(p, act, i + 1), act_load(p, act, i + 2), act_load(p, act, i + 3));
-    if (act == BMO_ACT_F32) return *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i);
-    const uint2 u = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + i);
-    if (act == BMO_ACT_F16) {
-        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)),
-                     b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                       __uint_as_float(u.y & 0xffff0000u));
-}
-__device__ __forceinline__ void act_store4(void *p, int act, long long i, float4 x, bool vec) {
-    if (act == BMO_ACT_F32) {
-        float *o = static_cast<float *>(p) + i;
-        if (vec) *reinterpret_cast<float4 *>(o) = x;
-        else o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
-        return;
-    }
-    uint16_t *o = static_cast<uint16_t *>(p) + i;
-    uint2 u;
-    if (act == BMO_ACT_F16) {
-        u.x = half_bits2(__float2half_rn(x.x), __float2half_rn(x.y));
-        u.y = half_bits2(__float2half_rn(x.z), __float2half_rn(x.w));
-    } else {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-        u.x = *reinterpret_cast<const uint32_t *>(&a);
-        u.y = *reinterpret_cast<const uint32_t *>(&b);
-    }
-    if (vec) *reinterpret_cast<uint2 *>(o) = u;
-    else o[0] = u.x & 0xffff, o[1] = u.x >> 16, o[2] = u.y & 0xffff, o[3] = u.y >> 16;
+template <int ACT>
+__device__ __forceinline__ void act_store(void *p, long long i, float x) {
+    if constexpr (ACT == BMO_ACT_F32) static_cast<float *>(p)[i] = x;
+    else if constexpr (ACT == BMO_ACT_F16) static_cast<__half *>(p)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16 *>(p)[i] = __float2bfloat16_rn(x);
 }
 
 // The power of two that brings amax into [2^10, 2^11), and its inverse
@@ -173,13 +150,6 @@ constexpr uint32_t kNoRow = 0xffffffffu;  // not attended
 struct Pos16 {
     uint32_t row[2];   // position g, g + 8 (scores)
     uint32_t vrow[4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9
-};
-
-// A warp's walk through one row's pages: entries [b0, b0 + 32) of the row's
-// block table, one a lane.
-struct Pages {
-    const int *table;  // of the request
-    int b0, entry;
 };
 
 // ---- fp16 rows ----
@@ -252,15 +222,15 @@ struct F16Rows {
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two shorter chains
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) {
                 const uint4 x = kr[s][0][j], y = kr[s][1][j];
                 mma16816(c, x.x, y.x, x.y, y.y, q[nb][2 * j][0], q[nb][2 * j][1]);
-                mma16816(c, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
+                mma16816(d, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
             }
-            sc[nb][0] = (c[0] + c[1]) * inv[nb];
-            sc[nb][1] = (c[2] + c[3]) * inv[nb];
+            sc[nb][0] = ((c[0] + d[0]) + (c[1] + d[1])) * inv[nb];
+            sc[nb][1] = ((c[2] + d[2]) + (c[3] + d[3])) * inv[nb];
         }
     }
     __device__ __forceinline__ bool value_range(int) { return false; }
@@ -467,6 +437,12 @@ struct Q4Rows {
     }
 };
 
+// A key head's share of a row on the line of tiles: up to NH query heads.
+struct Head {
+    int row, head0, heads;     // query heads [head0, head0 + heads) of a row
+    uint32_t first, n_tiles;   // its tiles on the line
+};
+
 // Two pieces a warp: one that began before its part of the line, one that goes on after it.
 template <int HD, int NH>
 struct PaSmem {
@@ -475,32 +451,19 @@ struct PaSmem {
     float bm[kPaWarps][NH], bl[kPaWarps][NH];
     float m[kPieces][NH], l[kPieces][NH];
     float o[kPieces][NH * HD];
-    float4 red[kPaThreads];
-    float red_m[kPaThreads], red_l[kPaThreads];
-    int seg[kPieces];    // row * units + unit, -1: none
-    int whole[kPieces];  // bit 0: begins at the head's first tile, bit 1: ends at its last
-    int join[2];         // 1 + the head that this CTA, last to arrive, joins
+    Head head[kPieces];
+    int whole[kPieces];  // -1: no piece; bit 0: begins at the head's first tile, bit 1: ends at its last
+    int scan[kPaWarps];
+    Head join_head[2];
+    int join_n[2], join_c0[2];  // pieces that this CTA, last to arrive, joins; the first one's CTA
 };
 
 constexpr int kMaxGrid = 640;
 
-// Running join of pieces (m, l, o): sums relative to the maximum so far.
-struct Joined {
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    __device__ __forceinline__ void scale_to(float top) {
-        const float f = m == top ? 1.0f : ex2(m - top);
-        m = top;
-        l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
-    }
-    __device__ __forceinline__ void add(float pm, float pl, float4 po) {  // pm <= m
-        const float f = pm == m ? 1.0f : ex2(pm - m);
-        l += f * pl, o.x += f * po.x, o.y += f * po.y, o.z += f * po.z, o.w += f * po.w;
-    }
-};
-
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m - kHead + log2f(l)) * kLn2; }
-__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+__device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : __frcp_rn(l); }
+
+constexpr int kJoinBatch = 8;  // pieces requested at a time
 
 // Release of the CTA's earlier writes (ordered by a barrier before it) and acquire of the others'.
 __device__ __forceinline__ int arrive(int *p) {
@@ -532,156 +495,129 @@ constexpr size_t kFixedSmem = (sizeof(PaSmem<HD, NH>) + 15) / 16 * 16;
 template <class R>
 constexpr int pa_piece_floats = (R::kHeads * (R::HD + 2) + 3) / 4 * 4;
 
-template <class R>
+template <class R, int ACT>
 __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int HD = R::HD, NB = R::NB, NH = R::kHeads, kTile = 16 * R::kSub, kO = R::kO;
     using Smem = PaSmem<HD, NH>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem &S = *reinterpret_cast<Smem *>(smem_raw);
-    int *ends = reinterpret_cast<int *>(smem_raw + kFixedSmem<HD, NH>);  // tiles of rows 0..r
-    __shared__ int scan_warp[kPaWarps];
+    uint32_t *ends = reinterpret_cast<uint32_t *>(smem_raw + kFixedSmem<HD, NH>);  // tiles of rows 0..r
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int group = a.n_heads / a.n_kv_heads;       // query heads of a key head
-    const int chunks = (group + NH - 1) / NH;         // units of a key head
-    const int units = a.n_kv_heads * chunks;
+    const int group = a.group;        // query heads of a key head
+    const uint32_t units = a.units.d;  // of a row: key heads x groups of NH query heads
     bool bad = false;
 
     // ---- tiles of every row, summed ----
-    auto row_tiles = [&](int r, int &start, int &len) {
+    auto row_tiles = [&](int r) -> uint32_t {
         int req;
-        len = pa_len(a, r, req, bad);
-        start = a.window > 0 ? max(0, len - a.window) : 0;
+        const int len = pa_len(a, r, req, bad);
+        const int start = a.window > 0 ? max(0, len - a.window) : 0;
         return len > start ? (len + kTile - 1) / kTile - start / kTile : 0;
     };
-    {
-        const int per_thread = (a.n_rows + kPaThreads - 1) / kPaThreads;
-        const int r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
-        int sum = 0, st, ln;
-        for (int r = r0; r < r1; ++r) {
-            sum += row_tiles(r, st, ln);
-            ends[r] = sum;
-        }
-        int inc = sum;
+    if (lane < 2) S.whole[2 * warp + lane] = -1;
+    if (tid < 2) S.join_n[tid] = 0;
+    uint32_t my_end = 0;  // up to 32 rows: tiles of rows 0..lane, in every warp
+    if (a.n_rows <= 32) {
+        my_end = lane < a.n_rows ? row_tiles(lane) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += u;
+            const uint32_t x = __shfl_up_sync(0xffffffffu, my_end, o);
+            if (lane >= o) my_end += x;
         }
-        if (lane == 31) scan_warp[warp] = inc;
-        if (tid < Smem::kPieces) S.seg[tid] = -1;
-        if (tid < 2) S.join[tid] = 0;
+    } else {
+        const int per_thread = (a.n_rows + kPaThreads - 1) / kPaThreads;
+        const int r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
+        uint32_t sum = 0;
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+            sum += row_tiles(r);
+            ends[r] = sum;
+        }
+        uint32_t inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += x;
+        }
+        if (lane == 31) S.scan[warp] = inc;
         __syncthreads();
-        int before = inc - sum;
-        for (int w = 0; w < warp; ++w) before += scan_warp[w];
+        uint32_t before = inc - sum;
+#pragma unroll
+        for (int w = 0; w < kPaWarps - 1; ++w) before += w < warp ? S.scan[w] : 0;
         if (before)
+#pragma unroll 1
             for (int r = r0; r < r1; ++r) ends[r] += before;
         __syncthreads();
     }
     if (bad) raise_error(a.status, kErrBadIndex);
-    const long long total = static_cast<long long>(ends[a.n_rows - 1]) * units;
-    const int n_warps = gridDim.x * kPaWarps;
-    const long long per = total >> 32 ? (total + n_warps - 1) / n_warps
-                                      : max(1u, (static_cast<uint32_t>(total) + n_warps - 1) / n_warps);
-    long long u = min(total, (static_cast<long long>(blockIdx.x) * kPaWarps + warp) * per);
-    const long long u_end = min(total, u + per);
-    // of a head: its query heads, its tiles on the line, and the CTAs these lie in
-    struct Head {
-        int row, head0, heads, kh, row0, n_tiles;
-    };
-    auto head_of_seg = [&](int row, int unit) {
-        Head h;
-        h.row = row;
-        h.kh = chunks == 1 ? unit : unit / chunks;
-        const int chunk = unit - h.kh * chunks;
-        h.head0 = h.kh * group + chunk * NH;
-        h.heads = min(NH, group - chunk * NH);
-        h.row0 = row ? ends[row - 1] : 0;
-        h.n_tiles = ends[row] - h.row0;
-        return h;
-    };
+    const bool few = a.n_rows <= 32;
+    auto end_of = [&](int r) { return few ? __shfl_sync(0xffffffffu, my_end, r) : ends[r]; };
+    const uint32_t total = end_of(a.n_rows - 1) * units;  // below 2^31 (checked by the entry point)
+    const uint32_t per = max(1u, (total + gridDim.x * kPaWarps - 1) / (gridDim.x * kPaWarps));
+    const uint32_t me = blockIdx.x * kPaWarps + warp;
+    uint32_t u = static_cast<uint32_t>(min(static_cast<unsigned long long>(total), static_cast<unsigned long long>(me) * per));
+    const uint32_t u_end = u + min(per, total - u);
 
     // rows without a position
+#pragma unroll 1
     for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
-        if (ends[r] != (r ? ends[r - 1] : 0)) continue;
-        for (int i = tid; i < a.n_heads * HD / 4; i += kPaThreads)
-            act_store4(a.out, a.act, r * a.out_stride + 4 * i, make_float4(0.0f, 0.0f, 0.0f, 0.0f), a.out_vec);
+        const uint32_t e0 = end_of(max(r - 1, 0)), e1 = end_of(r);
+        if (e1 != (r ? e0 : 0)) continue;
+#pragma unroll 1
+        for (int i = tid; i < a.n_heads * HD; i += kPaThreads) act_store<ACT>(a.out, r * a.out_stride + i, 0.0f);
         if (a.lse)
+#pragma unroll 1
             for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
     }
 
     R R_;
+    float *buf = S.buf[warp];
+#pragma unroll 1
     while (u < u_end) {
         // ---- the head that tile u belongs to ----
+        const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
         int row;
-        {
+        if (few) {
+            row = __popc(__ballot_sync(0xffffffffu, lane < a.n_rows && my_end <= q));
+        } else {
             int lo = 0, hi = a.n_rows - 1;
+#pragma unroll 1
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
-                if (static_cast<long long>(ends[mid]) * units > u) hi = mid;
+                if (ends[mid] > q) hi = mid;
                 else lo = mid + 1;
             }
             row = lo;
         }
-        const int row0 = row ? ends[row - 1] : 0;
-        const int n_tiles = ends[row] - row0;
-        const uint32_t rem = static_cast<uint32_t>(u - static_cast<long long>(row0) * units);
-        const int unit = rem / n_tiles;
-        const int tile0 = rem - unit * n_tiles;
-        const int tile1 = static_cast<int>(min(static_cast<long long>(n_tiles), tile0 + (u_end - u)));
+        const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
+        const uint32_t row0 = row ? row_prev : 0;
+        Head hd;
+        hd.row = row;
+        hd.n_tiles = row_end - row0;
+        const uint32_t unit = (u - row0 * units) / hd.n_tiles;
+        hd.first = row0 * units + unit * hd.n_tiles;
+        const int tile0 = u - hd.first;
+        const int tile1 = min(hd.n_tiles, tile0 + (u_end - u));
         u += tile1 - tile0;
-        const Head hd = head_of_seg(row, unit);
-        const int kh = hd.kh, head0 = hd.head0, heads = hd.heads;
-        int req, start, len;
-        len = pa_len(a, row, req, bad);
-        start = a.window > 0 ? max(0, len - a.window) : 0;
-        const int base_tile = start / kTile;
+        const int kh = pa_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
+        hd.head0 = kh * group + chunk * NH;
+        hd.heads = min(NH, group - chunk * NH);
+        int req;
+        const int len = pa_len(a, row, req, bad);
+        const int start = a.window > 0 ? max(0, len - a.window) : 0;
+        const int pbase = start / kTile * kTile;
 
-        Pages pg;
-        pg.table = a.table + static_cast<long long>(req) * a.max_blocks;
-        auto refill = [&](int b) {
-            pg.b0 = b;
-            pg.entry = b + lane < a.max_blocks ? pg.table[b + lane] : -1;
-        };
-        refill(static_cast<int>(pa_div(max(start, (base_tile + tile0) * kTile), a.page)));
-        float *buf = S.buf[warp];
+        // entries [b0, b0 + 32) of the row of the block table, one a lane
+        const int *table = a.table + static_cast<long long>(req) * a.max_blocks;
+        int b0 = pa_div(max(start, pbase + tile0 * kTile), a.page);
+        int entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
         __syncwarp();
-        for (int i = lane; i < heads * HD / 4; i += 32)
-            *reinterpret_cast<float4 *>(buf + 4 * i) =
-                act_load4(a.q, a.act, row * a.q_stride + static_cast<long long>(head0) * HD + 4 * i, a.q_vec);
+        const long long q0 = row * a.q_stride + static_cast<long long>(hd.head0) * HD + lane;
+#pragma unroll 1
+        for (int h = 0; h < hd.heads; ++h)
+#pragma unroll
+            for (int i = 0; i < HD; i += 32) buf[h * HD + i + lane] = act_load<ACT>(a.q, q0 + h * HD + i);
         __syncwarp();
-        // rows of the 16 positions from p0; those outside [start, len) and those of invalid pages: -1
-        auto locate = [&](int p0, Pos16 &P) {
-            const int first = max(p0, start), last = min(p0 + 15, len - 1);
-            if (first > last) {
-                P.row[0] = P.row[1] = P.vrow[0] = P.vrow[1] = P.vrow[2] = P.vrow[3] = kNoRow;
-                return;
-            }
-            const int b_first = pa_div(first, a.page), b_last = pa_div(last, a.page);
-            if (b_last >= pg.b0 + 32) refill(b_first);
-            if (b_first == b_last) {
-                const int page = __shfl_sync(0xffffffffu, pg.entry, b_first - pg.b0);
-                const bool ok = page >= 0 && page < a.n_pages;
-                bad |= !ok;
-                const uint32_t r0 = (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d - b_first * a.page.d;
-                auto at = [&](int p) { return ok && p >= first && p <= last ? r0 + p : kNoRow; };
-                P.row[0] = at(p0 + g), P.row[1] = at(p0 + g + 8);
-                P.vrow[0] = at(p0 + 2 * t), P.vrow[1] = at(p0 + 2 * t + 1);
-                P.vrow[2] = at(p0 + 2 * t + 8), P.vrow[3] = at(p0 + 2 * t + 9);
-            } else {
-                auto at = [&](int p) {
-                    const bool in = p >= first && p <= last;
-                    const int b = in ? static_cast<int>(pa_div(p, a.page)) : b_first;
-                    const int page = __shfl_sync(0xffffffffu, pg.entry, b - pg.b0);
-                    const bool ok = page >= 0 && page < a.n_pages;
-                    bad |= in && !ok;
-                    return in && ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + (p - b * a.page.d)
-                                    : kNoRow;
-                };
-                P.row[0] = at(p0 + g), P.row[1] = at(p0 + g + 8);
-                P.vrow[0] = at(p0 + 2 * t), P.vrow[1] = at(p0 + 2 * t + 1);
-                P.vrow[2] = at(p0 + 2 * t + 8), P.vrow[3] = at(p0 + 2 * t + 9);
-            }
-        };
 
         float o[NB][kO][4], m[NB], l[NB];
 #pragma unroll
@@ -693,34 +629,51 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 for (int i = 0; i < 4; ++i) o[nb][j][i] = 0.0f;
         }
         R_.reset();
+        R_.load_q(buf, hd.heads, a.qscale, lane);
         Pos16 P[R::kSub];
-        const int pbase = base_tile * kTile;
-#pragma unroll
-        for (int s = 0; s < R::kSub; ++s) {
-            locate(pbase + tile0 * kTile + 16 * s, P[s]);
-            R_.load_k(a, s, P[s], lane);
-        }
-        R_.load_q(buf, heads, a.qscale, lane);
-        for (int tile = tile0; tile < tile1; ++tile) {
-#pragma unroll
-            for (int s = 0; s < R::kSub; ++s) R_.load_v(a, s, P[s], lane);
+        // Step `tile` uses the keys requested in the step before, requests its
+        // own values and the next tile's keys; the first step only requests keys.
+#pragma unroll 1
+        for (int tile = tile0 - 1; tile < tile1; ++tile) {
             float sc[R::kSub][NB][2];
+            if (tile >= tile0) {
 #pragma unroll
-            for (int s = 0; s < R::kSub; ++s) {
-                R_.scores(s, sc[s]);
+                for (int s = 0; s < R::kSub; ++s) R_.load_v(a, s, P[s], lane);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    if (P[s].row[0] == kNoRow) sc[s][nb][0] = -INFINITY;
-                    if (P[s].row[1] == kNoRow) sc[s][nb][1] = -INFINITY;
+                for (int s = 0; s < R::kSub; ++s) {
+                    R_.scores(s, sc[s]);
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        if (P[s].row[0] == kNoRow) sc[s][nb][0] = -INFINITY;
+                        if (P[s].row[1] == kNoRow) sc[s][nb][1] = -INFINITY;
+                    }
                 }
             }
             if (tile + 1 < tile1) {
+                // lane i finds the row of the tile's position i (mod 16), the others read it from there
+                const int p0 = pbase + (tile + 1) * kTile;
+                const int last = min(p0 + kTile, len) - 1;
+                if (static_cast<int>(pa_div(last, a.page)) >= b0 + 32) {
+                    b0 = pa_div(max(p0, start), a.page);
+                    entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
+                }
+                const int p = p0 + (lane & (kTile - 1));
+                const bool in = p >= start && p <= last;
+                const int b = in ? pa_div(p, a.page) : b0;
+                const int page = __shfl_sync(0xffffffffu, entry, b - b0);
+                const bool ok = page >= 0 && page < a.n_pages;
+                bad |= in && !ok;
+                const uint32_t r = in && ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p : kNoRow;
 #pragma unroll
                 for (int s = 0; s < R::kSub; ++s) {
-                    locate(pbase + (tile + 1) * kTile + 16 * s, P[s]);
+                    P[s].row[0] = __shfl_sync(0xffffffffu, r, 16 * s + g);
+                    P[s].row[1] = __shfl_sync(0xffffffffu, r, 16 * s + g + 8);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) P[s].vrow[i] = __shfl_sync(0xffffffffu, r, 16 * s + 2 * t + (i & 1) + 4 * (i & 2));
                     R_.load_k(a, s, P[s], lane);
                 }
             }
+            if (tile < tile0) continue;
             bool rise = false;
 #pragma unroll
             for (int s = 0; s < R::kSub; ++s)
@@ -765,10 +718,10 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             for (int d = 4; d < 32; d <<= 1) l[nb] += __shfl_xor_sync(0xffffffffu, l[nb], d);
 
         // ---- a piece stays in shared memory, a whole head goes out through it ----
-        const bool begins = tile0 == 0, finishes = tile1 == n_tiles, whole = begins && finishes;
+        const bool begins = tile0 == 0, finishes = tile1 == static_cast<int>(hd.n_tiles), whole = begins && finishes;
         const int slot = 2 * warp + (begins ? 1 : 0);
         if (!whole && lane == 0) {
-            S.seg[slot] = row * units + unit;
+            S.head[slot] = hd;
             S.whole[slot] = (begins ? 1 : 0) | (finishes ? 2 : 0);
         }
         float *dst = whole ? buf : S.o[slot], *dst_m = whole ? S.bm[warp] : S.m[slot], *dst_l = whole ? S.bl[warp] : S.l[slot];
@@ -776,7 +729,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int h = R::head_of(nb, lane);
-            if (h >= heads) continue;
+            if (h >= hd.heads) continue;
             if (R_.owns(lane)) {
 #pragma unroll
                 for (int run = 0; run < R::kRuns; ++run)
@@ -790,130 +743,140 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         }
         __syncwarp();
         if (whole) {
-            for (int i = lane; i < heads * HD / 4; i += 32) {
-                const float4 x = *reinterpret_cast<const float4 *>(buf + 4 * i);
-                const float f = inverse_of(dst_l[4 * i / HD]);
-                act_store4(a.out, a.act, row * a.out_stride + static_cast<long long>(head0) * HD + 4 * i,
-                           make_float4(x.x * f, x.y * f, x.z * f, x.w * f), a.out_vec);
+            const long long out0 = row * a.out_stride + static_cast<long long>(hd.head0) * HD + lane;
+#pragma unroll 1
+            for (int h = 0; h < hd.heads; ++h) {
+                const float f = inverse_of(dst_l[h]);
+#pragma unroll
+                for (int i = 0; i < HD; i += 32) act_store<ACT>(a.out, out0 + h * HD + i, buf[h * HD + i + lane] * f);
             }
-            if (a.lse && lane < heads)
-                a.lse[static_cast<long long>(row) * a.n_heads + head0 + lane] = lse_of(dst_m[lane], dst_l[lane]);
+            if (a.lse && lane < hd.heads)
+                a.lse[static_cast<long long>(row) * a.n_heads + hd.head0 + lane] = lse_of(dst_m[lane], dst_l[lane]);
         }
     }
     if (bad) raise_error(a.status, kErrBadIndex);
     __syncthreads();
 
-    // ---- the CTA's pieces of one head, joined; one that other CTAs hold too goes to global memory ----
+    // ---- pieces of one head, joined ----
+    // A head's pieces in the CTA follow one another and end at the one that
+    // finishes the head, or at the last.  What other CTAs hold too goes to
+    // global memory; the last CTA to arrive puts all its parts back into the
+    // slots and comes through here once more.
     constexpr int kPieceFloats = pa_piece_floats<R>;
-    const long long cta_tiles = per * kPaWarps;
-    auto cta_of = [&](long long tile) {
-        return static_cast<int>(tile >> 32 || cta_tiles >> 32 ? tile / cta_tiles
-                                                              : static_cast<uint32_t>(tile) / static_cast<uint32_t>(cta_tiles));
-    };
-    auto finish = [&](const Head &h, int c, const Joined &j) {  // column c: 4 elements
-        const float f = inverse_of(j.l);
-        act_store4(a.out, a.act, h.row * a.out_stride + static_cast<long long>(h.head0) * HD + 4 * c,
-                   make_float4(j.o.x * f, j.o.y * f, j.o.z * f, j.o.w * f), a.out_vec);
-        if (a.lse && 4 * c % HD == 0)
-            a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + 4 * c / HD] = lse_of(j.m, j.l);
-    };
-    int open[2] = {0, 0};  // 1 + heads of which this CTA has a part: one that began earlier, one that begins here
-    for (int i = 0; i < Smem::kPieces;) {
-        const int seg = S.seg[i];
-        int last = i, next = i + 1;
-        if (seg >= 0)
-            for (; next < Smem::kPieces && (S.seg[next] == seg || S.seg[next] < 0); ++next)
-                if (S.seg[next] == seg) last = next;
-        if (seg >= 0) {
-            const bool begins = S.whole[i] & 1, finishes = S.whole[last] & 2;
-            const Head h = head_of_seg(seg / units, seg % units);
-            float *dst = a.part + (2ll * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
-            for (int c = tid; c < h.heads * HD / 4; c += kPaThreads) {
-                const int hh = 4 * c / HD;
-                Joined j;
-                for (int k = i; k <= last; ++k)
-                    if (S.seg[k] == seg) j.m = fmaxf(j.m, S.m[k][hh]);
-                for (int k = i; k <= last; ++k)
-                    if (S.seg[k] == seg) j.add(S.m[k][hh], S.l[k][hh], *reinterpret_cast<const float4 *>(&S.o[k][4 * c]));
-                if (begins && finishes) {
-                    finish(h, c, j);
+    int joining = -1;  // 0, 1: the slots hold that head's parts
+    for (;;) {
+        const int w = lane < Smem::kPieces ? S.whole[lane] : -1;
+        uint32_t left = __ballot_sync(0xffffffffu, w >= 0);
+        const uint32_t begin_bits = __ballot_sync(0xffffffffu, w >= 0 && (w & 1)),
+                       finish_bits = __ballot_sync(0xffffffffu, w >= 0 && (w & 2));
+        const uint32_t all = left;
+        int open[2] = {-1, -1};  // first slot of a head that began in an earlier CTA, of one that begins here
+#pragma unroll 1
+        while (left) {
+            const int first = __ffs(left) - 1;
+            const uint32_t ends_at = finish_bits >> first << first;
+            const int last = ends_at ? __ffs(ends_at) - 1 : 31 - __clz(left);
+            left = left >> last >> 1 << last << 1;
+            const bool begins = begin_bits >> first & 1, complete = begins && ends_at;
+            const Head h = S.head[first];
+            float *dst = a.part + (2 * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
+#pragma unroll 1
+            for (int e = tid; e < h.heads * HD; e += kPaThreads) {
+                const int hh = e / HD;
+                float top = -INFINITY, l = 0.0f, x = 0.0f;
+#pragma unroll 1
+                for (int k = first; k <= last; ++k)
+                    if (all >> k & 1) top = fmaxf(top, S.m[k][hh]);
+#pragma unroll 1
+                for (int k = first; k <= last; ++k)
+                    if (all >> k & 1) {
+                        const float f = S.m[k][hh] == top ? 1.0f : ex2(S.m[k][hh] - top);
+                        l += f * S.l[k][hh];
+                        x += f * S.o[k][e];
+                    }
+                if (complete) {
+                    act_store<ACT>(a.out, h.row * a.out_stride + static_cast<long long>(h.head0) * HD + e, x * inverse_of(l));
+                    if (a.lse && e % HD == 0)
+                        a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + hh] = lse_of(top, l);
                 } else {
-                    __stcg(reinterpret_cast<float4 *>(dst + 4 * c), j.o);
-                    if (4 * c % HD == 0) {
-                        __stcg(dst + NH * HD + hh, j.m);
-                        __stcg(dst + NH * HD + NH + hh, j.l);
+                    __stcg(dst + e, x);
+                    if (e % HD == 0) {
+                        __stcg(dst + NH * HD + hh, top);
+                        __stcg(dst + NH * HD + NH + hh, l);
                     }
                 }
             }
-            if (!(begins && finishes)) open[begins ? 1 : 0] = seg + 1;
+            if (!complete) open[begins ? 1 : 0] = first;
         }
-        i = next;
-    }
-    if (!open[0] && !open[1]) return;
-    __syncthreads();
-    auto first_tile = [&](const Head &h, int seg) {
-        return static_cast<long long>(h.row0) * units + static_cast<long long>(seg % units) * h.n_tiles;
-    };
-    if (tid < 2 && open[tid]) {
-        const int seg = open[tid] - 1;
-        const Head h = head_of_seg(seg / units, seg % units);
-        const long long first = first_tile(h, seg);
-        const int c0 = cta_of(first), c1 = cta_of(first + h.n_tiles - 1);
-        if (arrive(a.cnt + c0) == c1 - c0) {
-            a.cnt[c0] = 0;
-            S.join[tid] = seg + 1;
+        if (joining < 0) {
+            if (open[0] < 0 && open[1] < 0) return;
+            __syncthreads();
+            if (tid < 2 && open[tid] >= 0) {
+                const Head h = S.head[open[tid]];
+                const uint32_t cta_tiles = per * kPaWarps;
+                const int c0 = h.first / cta_tiles, c1 = (h.first + h.n_tiles - 1) / cta_tiles;
+                if (arrive(a.cnt + c0) == c1 - c0) {
+                    a.cnt[c0] = 0;
+                    S.join_n[tid] = c1 - c0 + 1;
+                    S.join_c0[tid] = c0;
+                }
+            }
+            // the heads move to where a second pass finds them
+            if (tid == 2 && open[0] >= 0) S.join_head[0] = S.head[open[0]];
+            if (tid == 3 && open[1] >= 0) S.join_head[1] = S.head[open[1]];
         }
-    }
-    __syncthreads();
+        __syncthreads();
+        do {
+            if (++joining == 2) return;
+        } while (!S.join_n[joining]);
 
-    // ---- the last CTA to arrive joins the head's pieces, in line order ----
-    for (int k = 0; k < 2; ++k) {
-        const int seg = S.join[k] - 1;
-        if (seg < 0) continue;
-        const Head h = head_of_seg(seg / units, seg % units);
-        const long long first = first_tile(h, seg);
-        const int c0 = cta_of(first), n = cta_of(first + h.n_tiles - 1) - c0 + 1;
-        const int cols = h.heads * HD / 4;
-        const int parts = max(1, kPaThreads / cols);  // threads that share a column's pieces
+        // ---- the last CTA to arrive: every part of the slots' columns joins a share of the pieces, in line order ----
+        const int n = S.join_n[joining], c0 = S.join_c0[joining];
+        const Head h = S.join_head[joining];
+        const int cols = h.heads * (HD / 4);                   // of 4 elements
+        const int parts = min(max(1, kPaThreads / cols), n);   // <= 8
         const int part = tid / cols;
-        for (int c = tid - part * cols; c < cols; c += kPaThreads) {
-            const int hh = 4 * c / HD;
-            Joined j;
-            if (part < parts) {
-                for (int p0 = part; p0 < n; p0 += 8 * parts) {
-                    float pm[8], pl[8];
-                    float4 po[8];
+        if (tid < Smem::kPieces) S.whole[tid] = tid < parts ? (tid == 0 ? 1 : 0) | (tid == parts - 1 ? 2 : 0) : -1;
+        if (tid == 0) S.head[0] = h;
+        if (part < parts) {
+#pragma unroll 1
+            for (int c = tid - part * cols; c < cols; c += kPaThreads) {
+                const int hh = c / (HD / 4);
+                float top = -INFINITY, l = 0.0f;
+                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                for (int p0 = part; p0 < n; p0 += kJoinBatch * parts) {
+                    float pm[kJoinBatch], pl[kJoinBatch];
+                    float4 po[kJoinBatch];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < kJoinBatch; ++i) {
                         const int p = p0 + i * parts;
-                        const float *src = a.part + (2ll * (c0 + (p < n ? p : 0)) + (p == 0 || p >= n ? 1 : 0)) * kPieceFloats;
-                        pm[i] = __ldcg(src + NH * HD + hh);
-                        pl[i] = __ldcg(src + NH * HD + NH + hh);
-                        po[i] = __ldcg(reinterpret_cast<const float4 *>(src + 4 * c));
+                        pm[i] = -INFINITY, pl[i] = 0.0f, po[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (p < n) {
+                            const float *src = a.part + (2 * (c0 + p) + (p == 0 ? 1 : 0)) * kPieceFloats;
+                            pm[i] = __ldcg(src + NH * HD + hh);
+                            pl[i] = __ldcg(src + NH * HD + NH + hh);
+                            po[i] = __ldcg(reinterpret_cast<const float4 *>(src + 4 * c));
+                        }
                     }
-                    float top = j.m;
+                    float now = top;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (p0 + i * parts < n) top = fmaxf(top, pm[i]);
-                    j.scale_to(top);
+                    for (int i = 0; i < kJoinBatch; ++i) now = fmaxf(now, pm[i]);
+                    const float f = top == now ? 1.0f : ex2(top - now);
+                    top = now;
+                    l *= f, o.x *= f, o.y *= f, o.z *= f, o.w *= f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (p0 + i * parts < n) j.add(pm[i], pl[i], po[i]);
+                    for (int i = 0; i < kJoinBatch; ++i) {
+                        const float w = pm[i] == top ? 1.0f : ex2(pm[i] - top);
+                        l += w * pl[i];
+                        o.x += w * po[i].x, o.y += w * po[i].y, o.z += w * po[i].z, o.w += w * po[i].w;
+                    }
                 }
+                *reinterpret_cast<float4 *>(&S.o[part][4 * c]) = o;
+                if (c % (HD / 4) == 0) S.m[part][hh] = top, S.l[part][hh] = l;
             }
-            if (parts > 1) {  // one column a thread: every thread is here once
-                S.red[tid] = j.o, S.red_m[tid] = j.m, S.red_l[tid] = j.l;
-                __syncthreads();
-                if (part == 0) {
-                    float top = j.m;
-                    for (int q = 1; q < parts; ++q) top = fmaxf(top, S.red_m[q * cols + c]);
-                    j.scale_to(top);
-                    for (int q = 1; q < parts; ++q) j.add(S.red_m[q * cols + c], S.red_l[q * cols + c], S.red[q * cols + c]);
-                }
-                __syncthreads();
-            }
-            if (part == 0) finish(h, c, j);
         }
+        __syncthreads();
     }
 }
 
@@ -921,7 +884,7 @@ constexpr int kMaxDevices = 64;
 
 // CTAs of a launch on the current device: all that are resident at once, at
 // most kMaxGrid (0: the kernel cannot run here).
-template <class R>
+template <class R, int ACT>
 cudaError_t pa_grid(int &grid) {
     static std::atomic<int> known[kMaxDevices];
     int dev = 0;
@@ -929,11 +892,12 @@ cudaError_t pa_grid(int &grid) {
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices && (grid = known[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
     constexpr int smem = static_cast<int>(kFixedSmem<R::HD, R::kHeads> + 4 * kPagedMaxRows);
-    e = cudaFuncSetAttribute(paged_attn_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(paged_attn_kernel<R, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     int sms = 0, per_sm = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R>, kPaThreads, smem)) != cudaSuccess)
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R, ACT>, kPaThreads, smem)) !=
+        cudaSuccess)
         return e;
     grid = sms * per_sm < kMaxGrid ? sms * per_sm : kMaxGrid;
     if (grid <= 0) return cudaErrorInvalidConfiguration;
@@ -942,20 +906,21 @@ cudaError_t pa_grid(int &grid) {
 }
 
 template <class R>
-size_t pa_scratch(int grid) {
-    return (static_cast<size_t>(grid) * 4 + 255) / 256 * 256 +
-           static_cast<size_t>(grid) * 2 * pa_piece_floats<R> * sizeof(float);
-}
+constexpr size_t kScratch = (4 * kMaxGrid + 255) / 256 * 256 + sizeof(float) * kMaxGrid * 2 * pa_piece_floats<R>;
 
-template <class R>
+template <class R, int ACT>
 cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cudaStream_t s) {
     int grid = 0;
-    const cudaError_t e = pa_grid<R>(grid);
+    const cudaError_t e = pa_grid<R, ACT>(grid);
     if (e != cudaSuccess) return e;
-    if (scratch_bytes < pa_scratch<R>(grid)) return cudaErrorInvalidValue;
+    if (scratch_bytes < kScratch<R>) return cudaErrorInvalidValue;
+    a.group = a.n_heads / a.n_kv_heads;
+    const int chunks = (a.group + R::kHeads - 1) / R::kHeads;
+    a.chunks = make_fast_div(chunks);
+    a.units = make_fast_div(a.n_kv_heads * chunks);
     a.cnt = static_cast<int *>(scratch);
-    a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (static_cast<size_t>(grid) * 4 + 255) / 256 * 256);
-    paged_attn_kernel<R><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
+    a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
+    paged_attn_kernel<R, ACT><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -970,16 +935,17 @@ auto pa_variant(int head_dim, int kv_type, int group, F f) {
 }  // namespace
 
 size_t paged_attention_scratch_bytes(int head_dim, int kv_type, int n_heads, int n_kv_heads) {
-    return pa_variant(head_dim, kv_type, n_heads / n_kv_heads, [&](auto r) -> size_t {
-        int grid = 0;
-        return pa_grid<decltype(r)>(grid) == cudaSuccess ? pa_scratch<decltype(r)>(grid) : 0;
-    });
+    return pa_variant(head_dim, kv_type, n_heads / n_kv_heads, [](auto r) { return kScratch<decltype(r)>; });
 }
 
-cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, void *scratch, size_t scratch_bytes,
-                                   cudaStream_t s) {
-    return pa_variant(head_dim, kv_type, a.n_heads / a.n_kv_heads,
-                      [&](auto r) { return pa_launch<decltype(r)>(a, scratch, scratch_bytes, s); });
+cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, int act, void *scratch,
+                                   size_t scratch_bytes, cudaStream_t s) {
+    return pa_variant(head_dim, kv_type, a.n_heads / a.n_kv_heads, [&](auto r) {
+        using R = decltype(r);
+        if (act == BMO_ACT_F32) return pa_launch<R, BMO_ACT_F32>(a, scratch, scratch_bytes, s);
+        if (act == BMO_ACT_F16) return pa_launch<R, BMO_ACT_F16>(a, scratch, scratch_bytes, s);
+        return pa_launch<R, BMO_ACT_BF16>(a, scratch, scratch_bytes, s);
+    });
 }
 
 }  // namespace bmo

@@ -15,7 +15,7 @@ constexpr int kPagedMaxReq = 65536;       // requests of one plan
 constexpr int kPagedMaxRows = 4096;       // rows of one attention call (their tile counts sit in shared memory)
 constexpr int kPagedMaxPageSize = 65536;
 
-// n / d for 0 <= n < 2^31 by one multiply: q = (umulhi(n, mul) + n) >> shift.
+// n / d for 0 <= n < 2^31 by one multiply: q = (umulhi(n, mul) + n) >> shift;
 struct FastDiv {
     uint32_t d, mul, shift;
 };
@@ -69,17 +69,16 @@ struct PagedAttnArgs {
     int n_req, max_blocks, n_pages, window;
     FastDiv page;
     int n_rows, n_heads, n_kv_heads;
-    int act;
-    int q_vec, out_vec;              // rows of q / out allow 4-element accesses
+    int group;                       // query heads of a key head (this and the next set by the launcher)
+    FastDiv units, chunks;           // units of a row, of a key head
     float qscale;                    // score scale * log2(e)
     int *status;
     // split rows: two partial results per CTA, one arrival counter per CTA
     float *part;
     int *cnt;
 };
-cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, void *scratch, size_t scratch_bytes,
-                                   cudaStream_t s);
-// 0 when the device cannot run it.
+cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, int act, void *scratch,
+                                   size_t scratch_bytes, cudaStream_t s);
 size_t paged_attention_scratch_bytes(int head_dim, int kv_type, int n_heads, int n_kv_heads);
 
 }  // namespace bmo

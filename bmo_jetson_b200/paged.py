@@ -213,8 +213,7 @@ class PagedKV:
             lp = lse.data_ptr()
         sc = self._scratch.get(heads)
         if sc is None:
-            with torch.cuda.device(d):
-                nbytes = lib().bmo_k_paged_attention_scratch_bytes(self._ref, heads)
+            nbytes = lib().bmo_k_paged_attention_scratch_bytes(self._ref, heads)
             if nbytes == 0:
                 raise ValueError(f"{heads} query heads over {self.n_kv_heads} key heads of {self.head_dim}")
             sc = self._scratch[heads] = torch.zeros(nbytes, dtype=torch.uint8, device=d)

@@ -237,8 +237,7 @@ BMO_API int bmo_k_paged_append(const bmo_paged_kv *cache, int layer, int n, cons
 BMO_API int bmo_k_paged_read(const bmo_paged_kv *cache, int layer, int n, const int32_t *slot_dev, void *k_out_dev,
                              void *v_out_dev, int act_type, int *status_dev, void *stream);
 
-/* Scratch bytes of bmo_k_paged_attention on the current device (0: the cache
- * is not one it accepts). */
+/* Scratch bytes of bmo_k_paged_attention (0: the cache is not one it accepts). */
 BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, int n_heads);
 /* Attention of single tokens over the pages of `layer`: row i of q_dev
  * [n_rows][n_heads][head_dim] attends to the last `window` (book.window; 0:
@@ -252,7 +251,8 @@ BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, in
  * past a request's length are never read.  Sums, maxima and products are fp32
  * (each fp32 factor as two fp16 parts); the result is the same from call to
  * call.  scratch_dev must be zero on the first call, is left reusable, and
- * serves one call at a time.  n_rows <= 4096.  status_dev as above. */
+ * serves one call at a time.  n_rows <= 4096, and n_rows * n_heads *
+ * (max_blocks * page_size / 16 + 1) below 2^31.  status_dev as above. */
 BMO_API int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, const void *q_dev,
                                   long long q_stride, int n_heads, const int32_t *row_req_dev,
                                   const int32_t *row_len_dev, float scale, void *out_dev, long long out_stride,
