@@ -188,7 +188,7 @@ int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, cons
     if (!row_req_dev && n_rows > b.n_req) return kInvalid;
     if (n_rows == 0) return 0;
     // the kernel numbers the call's tiles (16 positions or more of a head) in 31 bits
-    const long long tiles = static_cast<long long>(b.max_blocks) * b.page_size / 16 + 1;
+    const long long tiles = static_cast<long long>(b.max_blocks) * b.page_size / 16 + 4;
     if (n_heads > 65536 || tiles * n_rows > INT_MAX / n_heads) return kInvalid;
     const int hd = cache->head_dim;
     if (!rows_ok(q_dev, n_rows, q_stride, n_heads, hd, elem) || !rows_ok(out_dev, n_rows, out_stride, n_heads, hd, elem) ||

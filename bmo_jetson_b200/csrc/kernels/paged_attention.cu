@@ -144,9 +144,8 @@ __device__ __forceinline__ void range_factor(float amax, float &mul, float &inv)
     inv = __int_as_float((ex - 10) << 23);
 }
 
-// Where a warp's lanes find the rows of 16 consecutive positions.  A layer
-// has fewer than 2^32 - 1 rows (checked by the entry point).
-constexpr uint32_t kNoRow = 0xffffffffu;  // not attended
+// Where a lane finds its rows of 16 consecutive positions, numbered within the
+// layer (fewer than 2^32, checked by the entry point).
 struct Pos16 {
     uint32_t row[2];   // position g, g + 8 (scores)
     uint32_t vrow[4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9
@@ -157,6 +156,7 @@ template <int HD_, int NB_>
 struct F16Rows {
     static constexpr int HD = HD_, NB = NB_;
     static constexpr int kMinCtas = NB == 1 ? 3 : 2;
+    static constexpr int kHeadCost = 1;
     static constexpr int kHeads = 4 * NB;          // query heads of a unit
     static constexpr int kSub = HD == 128 ? 1 : 2; // 16-position parts of a tile
     static constexpr int kO = HD / 16;
@@ -198,25 +198,22 @@ struct F16Rows {
             }
         }
     }
-    __device__ __forceinline__ void load_k(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
-        const int t = lane & 3;
+    const char *kp, *vp;  // the lane's bytes of row 0
+    __device__ __forceinline__ F16Rows(const PagedAttnArgs &a, int lane)
+        : kp(static_cast<const char *>(a.k) + 16 * (lane & 3)), vp(static_cast<const char *>(a.v) + 16 * (lane >> 2)) {}
+    __device__ __forceinline__ void load_k(int s, const Pos16 &p) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const char *src = static_cast<const char *>(a.k) + static_cast<size_t>(p.row[i]) * (2 * HD) + 16 * t;
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int c = 0; c < HD / 32; ++c)
-                kr[s][i][c] = p.row[i] != kNoRow ? ldg_stream16(src + 64 * c) : make_uint4(0, 0, 0, 0);
-        }
+                kr[s][i][c] = ldg_stream16(kp + static_cast<size_t>(p.row[i]) * (2 * HD) + 64 * c);
     }
-    __device__ __forceinline__ void load_v(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
-        const int g = lane >> 2;
+    __device__ __forceinline__ void load_v(int s, const Pos16 &p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const char *src = static_cast<const char *>(a.v) + static_cast<size_t>(p.vrow[i]) * (2 * HD) + 16 * g;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
-                vr[s][i][c] = p.vrow[i] != kNoRow ? ldg_stream16(src + 128 * c) : make_uint4(0, 0, 0, 0);
-        }
+                vr[s][i][c] = ldg_stream16(vp + static_cast<size_t>(p.vrow[i]) * (2 * HD) + 128 * c);
     }
     // sc[nb][i]: score (log2 units) of position g + 8 i for head (nb, t)
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
@@ -281,6 +278,7 @@ template <int HD_>
 struct Q4Rows {
     static constexpr int HD = HD_, NB = 1;
     static constexpr int kMinCtas = 3;
+    static constexpr int kHeadCost = 2;
     static constexpr int kHeads = 1;
     static constexpr int kSub = 2;
     static constexpr int kO = HD / 16;
@@ -288,7 +286,7 @@ struct Q4Rows {
     static constexpr int kKW = HD / 32;           // words of a key row a lane holds
     static constexpr int kVW = HD / 64;           // words of a value row a lane holds
     uint32_t q[HD / 16][2];
-    float inv;
+    float inv, bias[2];
     float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
     uint32_t kr[kSub][2][kKW], vr[kSub][4][kVW];
     __half ks[kSub][2], vs[kSub][2];
@@ -314,63 +312,76 @@ struct Q4Rows {
         float mul;
         range_factor(amax, mul, inv);
         inv *= qscale;
-        auto part = [&](float x) {
+        float sum = 0.0f;
+        auto part = [&](float x, float weight) {
             const float y = mine ? x * mul : 0.0f;
-            const __half h = __float2half_rn(y);
-            return (g & 1) ? __float2half_rn(y - __half2float(h)) : h;
+            __half h = __float2half_rn(y);
+            if (g & 1) h = __float2half_rn(y - __half2float(h));
+            sum += weight * __half2float(h);
+            return h;
         };
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
-            q[2 * w][0] = half_bits2(part(lo[4 * w]), part(lo[4 * w + 2]));
-            q[2 * w][1] = half_bits2(part(hi[4 * w]), part(hi[4 * w + 2]));
-            q[2 * w + 1][0] = half_bits2(part(lo[4 * w + 1]), part(lo[4 * w + 3]));
-            q[2 * w + 1][1] = half_bits2(part(hi[4 * w + 1]), part(hi[4 * w + 3]));
+            q[2 * w][0] = half_bits2(part(lo[4 * w], 1.0f), part(lo[4 * w + 2], 1.0f));
+            q[2 * w][1] = half_bits2(part(0.0625f * hi[4 * w], 16.0f), part(0.0625f * hi[4 * w + 2], 16.0f));
+            q[2 * w + 1][0] = half_bits2(part(lo[4 * w + 1], 1.0f), part(lo[4 * w + 3], 1.0f));
+            q[2 * w + 1][1] = half_bits2(part(0.0625f * hi[4 * w + 1], 16.0f), part(0.0625f * hi[4 * w + 3], 16.0f));
         }
+        // of columns 2t, 2t + 1: from a lane that holds block t
+        if (HD == 64) sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        const int from = HD == 128 ? 9 * t : 8 * t + (2 * t & 3);
+        bias[0] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum, from);      // -8 * 2^-24
+        bias[1] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum, from + 4);
     }
-    __device__ __forceinline__ void load_k(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
-        const int t = lane & 3;
+    const char *kp, *vp;        // the lane's bytes of row 0
+    const __half *ksp, *vsp;    // its block's scales
+    __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, int lane)
+        : kp(static_cast<const char *>(a.k) + 4 * kKW * (lane & 3)), vp(static_cast<const char *>(a.v) + 4 * kVW * (lane >> 2)),
+          ksp(a.k_scale + (lane & 3) % kBlocks), vsp(a.v_scale + (lane & 3) % kBlocks) {}
+    __device__ __forceinline__ void load_k(int s, const Pos16 &p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool ok = p.row[i] != kNoRow;
-            const char *src = static_cast<const char *>(a.k) + static_cast<size_t>(p.row[i]) * (HD / 2) + 4 * kKW * t;
+            const char *src = kp + static_cast<size_t>(p.row[i]) * (HD / 2);
             if constexpr (HD == 128) {
-                const uint4 x = ok ? ldg_stream16(src) : make_uint4(0, 0, 0, 0);
+                const uint4 x = ldg_stream16(src);
                 kr[s][i][0] = x.x, kr[s][i][1] = x.y, kr[s][i][2] = x.z, kr[s][i][3] = x.w;
             } else {
-                const uint2 x = ok ? ldg_stream8(src) : make_uint2(0, 0);
+                const uint2 x = ldg_stream8(src);
                 kr[s][i][0] = x.x, kr[s][i][1] = x.y;
             }
-            ks[s][i] = ok && t < kBlocks ? __ldg(a.k_scale + static_cast<size_t>(p.row[i]) * kBlocks + t) : __ushort_as_half(0);
+            ks[s][i] = __ldg(ksp + static_cast<size_t>(p.row[i]) * kBlocks);
         }
     }
-    __device__ __forceinline__ void load_v(const PagedAttnArgs &a, int s, const Pos16 &p, int lane) {
-        const int g = lane >> 2, t = lane & 3;
+    __device__ __forceinline__ void load_v(int s, const Pos16 &p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool ok = p.vrow[i] != kNoRow;
-            const char *src = static_cast<const char *>(a.v) + static_cast<size_t>(p.vrow[i]) * (HD / 2) + 4 * kVW * g;
+            const char *src = vp + static_cast<size_t>(p.vrow[i]) * (HD / 2);
             if constexpr (HD == 128) {
-                const uint2 x = ok ? ldg_stream8(src) : make_uint2(0, 0);
+                const uint2 x = ldg_stream8(src);
                 vr[s][i][0] = x.x, vr[s][i][1] = x.y;
             } else {
-                vr[s][i][0] = ok ? ldg_stream4(src) : 0;
+                vr[s][i][0] = ldg_stream4(src);
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            vs[s][i] = p.row[i] != kNoRow && t < kBlocks ? __ldg(a.v_scale + static_cast<size_t>(p.row[i]) * kBlocks + t) : __ushort_as_half(0);
+        for (int i = 0; i < 2; ++i) vs[s][i] = __ldg(vsp + static_cast<size_t>(p.row[i]) * kBlocks);
     }
+    // A: codes n as subnormal halves, n 2^-24 (low nibbles) and 16 n 2^-24 (high
+    // nibbles, whose q is divided by 16), so a code costs half a mask; the sums
+    // start at -8 sum q, which makes them those of n - 8.  (Not done for the values: there the
+    // offset would be summed over all positions and cost digits.)
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
-        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float c[4] = {bias[0], bias[1], bias[0], bias[1]}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two shorter chains
+        constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
-            const uint32_t x = kr[s][0][w], y = kr[s][1][w];
-            mma16816(c, codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y), q[2 * w][0], q[2 * w][1]);
-            mma16816(c, codes_lo(x >> 8), codes_lo(y >> 8), codes_hi(x >> 8), codes_hi(y >> 8), q[2 * w + 1][0],
-                     q[2 * w + 1][1]);
+            const uint32_t x = kr[s][0][w], y = kr[s][1][w], x8 = x >> 8, y8 = y >> 8;
+            mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
+            mma16816(d, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
         }
-        sc[0][0] = (c[0] + c[1]) * __half2float(ks[s][0]);
-        sc[0][1] = (c[2] + c[3]) * __half2float(ks[s][1]);
+        // lanes past the row's blocks hold zero sums
+        sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (__half2float(ks[s][0]) * 16777216.0f);
+        sc[0][1] = ((c[2] + d[2]) + (c[3] + d[3])) * (__half2float(ks[s][1]) * 16777216.0f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 1);
@@ -404,7 +415,7 @@ struct Q4Rows {
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int i = 0; i < 2; ++i)  // w * scale / vlim <= 2^15
-                b[s][i] = transpose8(split_half(w[s][0][i] * (__half2float(vs[s][i]) * vinv)));
+                b[s][i] = transpose8(split_half(w[s][0][i] * (__half2float(vs[s][i]) * vinv)));  // columns of no block: unused
 #pragma unroll
         for (int i = 0; i < kVW; ++i) {
 #pragma unroll
@@ -501,22 +512,22 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     using Smem = PaSmem<HD, NH>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem &S = *reinterpret_cast<Smem *>(smem_raw);
-    uint32_t *ends = reinterpret_cast<uint32_t *>(smem_raw + kFixedSmem<HD, NH>);  // tiles of rows 0..r
+    uint32_t *ends = reinterpret_cast<uint32_t *>(smem_raw + kFixedSmem<HD, NH>);  // of rows 0..r
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.group;        // query heads of a key head
     const uint32_t units = a.units.d;  // of a row: key heads x groups of NH query heads
     bool bad = false;
 
-    // ---- tiles of every row, summed ----
+    // ---- tiles of every row, summed; a head counts kHeadCost tiles more, for what it costs besides ----
     auto row_tiles = [&](int r) -> uint32_t {
         int req;
         const int len = pa_len(a, r, req, bad);
         const int start = a.window > 0 ? max(0, len - a.window) : 0;
-        return len > start ? (len + kTile - 1) / kTile - start / kTile : 0;
+        return len > start ? (len + kTile - 1) / kTile - start / kTile + R::kHeadCost : 0;
     };
     if (lane < 2) S.whole[2 * warp + lane] = -1;
     if (tid < 2) S.join_n[tid] = 0;
-    uint32_t my_end = 0;  // up to 32 rows: tiles of rows 0..lane, in every warp
+    uint32_t my_end = 0;  // up to 32 rows: of rows 0..lane, in every warp
     if (a.n_rows <= 32) {
         my_end = lane < a.n_rows ? row_tiles(lane) : 0;
 #pragma unroll
@@ -570,7 +581,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
     }
 
-    R R_;
+    R R_(a, lane);
     float *buf = S.buf[warp];
 #pragma unroll 1
     while (u < u_end) {
@@ -591,14 +602,17 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         }
         const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
         const uint32_t row0 = row ? row_prev : 0;
+        // [0, kHeadCost) of a head stands for its other costs, then come its tiles
+        const uint32_t span = row_end - row0;
+        const uint32_t unit = (u - row0 * units) / span;
+        const uint32_t from = u - row0 * units - unit * span, to = min(span, from + (u_end - u));
+        u += to - from;
+        const int tile0 = max(static_cast<int>(from) - R::kHeadCost, 0), tile1 = static_cast<int>(to) - R::kHeadCost;
+        if (tile1 <= tile0) continue;
         Head hd;
         hd.row = row;
-        hd.n_tiles = row_end - row0;
-        const uint32_t unit = (u - row0 * units) / hd.n_tiles;
-        hd.first = row0 * units + unit * hd.n_tiles;
-        const int tile0 = u - hd.first;
-        const int tile1 = min(hd.n_tiles, tile0 + (u_end - u));
-        u += tile1 - tile0;
+        hd.n_tiles = span - R::kHeadCost;
+        hd.first = row0 * units + unit * span + R::kHeadCost;
         const int kh = pa_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
         hd.head0 = kh * group + chunk * NH;
         hd.heads = min(NH, group - chunk * NH);
@@ -631,22 +645,27 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         R_.reset();
         R_.load_q(buf, hd.heads, a.qscale, lane);
         Pos16 P[R::kSub];
+        constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << kTile) - 1;
+        uint32_t there = 0;  // positions attended to of the tile whose keys are requested
         // Step `tile` uses the keys requested in the step before, requests its
         // own values and the next tile's keys; the first step only requests keys.
 #pragma unroll 1
         for (int tile = tile0 - 1; tile < tile1; ++tile) {
+            const uint32_t now = there;
             float sc[R::kSub][NB][2];
-            if (tile >= tile0) {
+            if (now) {
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.load_v(a, s, P[s], lane);
+                for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) {
-                    R_.scores(s, sc[s]);
+                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
+                if (now != kAll) {
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        if (P[s].row[0] == kNoRow) sc[s][nb][0] = -INFINITY;
-                        if (P[s].row[1] == kNoRow) sc[s][nb][1] = -INFINITY;
-                    }
+                    for (int s = 0; s < R::kSub; ++s)
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                if (!(now >> (16 * s + 8 * i + g) & 1)) sc[s][nb][i] = -INFINITY;
                 }
             }
             if (tile + 1 < tile1) {
@@ -663,17 +682,26 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 const int page = __shfl_sync(0xffffffffu, entry, b - b0);
                 const bool ok = page >= 0 && page < a.n_pages;
                 bad |= in && !ok;
-                const uint32_t r = in && ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p : kNoRow;
+                uint32_t r = (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p;
+                there = __ballot_sync(0xffffffffu, in && ok) & kAll;
+                if (there) {
+                    // a position that is left out reads a row that is not, with weight 0
+                    if (there != kAll) {
+                        const uint32_t other = __shfl_sync(0xffffffffu, r, __ffs(there) - 1);
+                        r = in && ok ? r : other;
+                    }
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) {
-                    P[s].row[0] = __shfl_sync(0xffffffffu, r, 16 * s + g);
-                    P[s].row[1] = __shfl_sync(0xffffffffu, r, 16 * s + g + 8);
+                    for (int s = 0; s < R::kSub; ++s) {
+                        P[s].row[0] = __shfl_sync(0xffffffffu, r, 16 * s + g);
+                        P[s].row[1] = __shfl_sync(0xffffffffu, r, 16 * s + g + 8);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) P[s].vrow[i] = __shfl_sync(0xffffffffu, r, 16 * s + 2 * t + (i & 1) + 4 * (i & 2));
-                    R_.load_k(a, s, P[s], lane);
+                        for (int i = 0; i < 4; ++i)
+                            P[s].vrow[i] = __shfl_sync(0xffffffffu, r, 16 * s + 2 * t + (i & 1) + 4 * (i & 2));
+                        R_.load_k(s, P[s]);
+                    }
                 }
             }
-            if (tile < tile0) continue;
+            if (!now) continue;
             bool rise = false;
 #pragma unroll
             for (int s = 0; s < R::kSub; ++s)
@@ -924,24 +952,29 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     return cudaGetLastError();
 }
 
+template <class R>
+struct PaVariant {
+    using Rows = R;
+};
+
 template <class F>
 auto pa_variant(int head_dim, int kv_type, int group, F f) {
-    if (kv_type == kKvQ4_0) return head_dim == 128 ? f(Q4Rows<128>{}) : f(Q4Rows<64>{});
+    if (kv_type == kKvQ4_0) return head_dim == 128 ? f(PaVariant<Q4Rows<128>>{}) : f(PaVariant<Q4Rows<64>>{});
     // up to 4 query heads of a key head fill one B operand, up to 8 two of them
-    if (group <= 4) return head_dim == 128 ? f(F16Rows<128, 1>{}) : f(F16Rows<64, 1>{});
-    return head_dim == 128 ? f(F16Rows<128, 2>{}) : f(F16Rows<64, 2>{});
+    if (group <= 4) return head_dim == 128 ? f(PaVariant<F16Rows<128, 1>>{}) : f(PaVariant<F16Rows<64, 1>>{});
+    return head_dim == 128 ? f(PaVariant<F16Rows<128, 2>>{}) : f(PaVariant<F16Rows<64, 2>>{});
 }
 
 }  // namespace
 
 size_t paged_attention_scratch_bytes(int head_dim, int kv_type, int n_heads, int n_kv_heads) {
-    return pa_variant(head_dim, kv_type, n_heads / n_kv_heads, [](auto r) { return kScratch<decltype(r)>; });
+    return pa_variant(head_dim, kv_type, n_heads / n_kv_heads, [](auto r) { return kScratch<typename decltype(r)::Rows>; });
 }
 
 cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, int act, void *scratch,
                                    size_t scratch_bytes, cudaStream_t s) {
     return pa_variant(head_dim, kv_type, a.n_heads / a.n_kv_heads, [&](auto r) {
-        using R = decltype(r);
+        using R = typename decltype(r)::Rows;
         if (act == BMO_ACT_F32) return pa_launch<R, BMO_ACT_F32>(a, scratch, scratch_bytes, s);
         if (act == BMO_ACT_F16) return pa_launch<R, BMO_ACT_F16>(a, scratch, scratch_bytes, s);
         return pa_launch<R, BMO_ACT_BF16>(a, scratch, scratch_bytes, s);

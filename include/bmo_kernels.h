@@ -252,7 +252,7 @@ BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, in
  * (each fp32 factor as two fp16 parts); the result is the same from call to
  * call.  scratch_dev must be zero on the first call, is left reusable, and
  * serves one call at a time.  n_rows <= 4096, and n_rows * n_heads *
- * (max_blocks * page_size / 16 + 1) below 2^31.  status_dev as above. */
+ * (max_blocks * page_size / 16 + 4) below 2^31.  status_dev as above. */
 BMO_API int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, const void *q_dev,
                                   long long q_stride, int n_heads, const int32_t *row_req_dev,
                                   const int32_t *row_len_dev, float scale, void *out_dev, long long out_stride,
