@@ -78,12 +78,26 @@ __device__ __forceinline__ uint32_t ldg_stream4(const void *p) {
     return v;
 }
 
+// c += A B, and c = A B + start.
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1, float start0, float start1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %10, %11};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(start0), "f"(start1));
+}
+// c = A B if first, else c += A B (first known at compile time).
+__device__ __forceinline__ void mma16816(float (&c)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    if (first) mma16816(c, a0, a1, a2, a3, b0, b1, 0.0f, 0.0f);
+    else mma16816(c, a0, a1, a2, a3, b0, b1);
 }
 
 __device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
@@ -144,6 +158,32 @@ __device__ __forceinline__ void range_factor(float amax, float &mul, float &inv)
     inv = __int_as_float((ex - 10) << 23);
 }
 
+// 4 elements of a query head, split: times `weight` and the power of two that
+// brings the head into fp16's range; inv: that power's inverse.
+struct QueryPart {
+    __half hi[4], lo[4];
+    float inv;
+};
+template <int ACT, int HD>
+__device__ __forceinline__ void query_load(const void *src, long long at, int lane, float (&x)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = 4 * lane < HD ? act_load<ACT>(src, at + 4 * lane + i) : 0.0f;
+}
+__device__ __forceinline__ QueryPart query_part(const float (&x)[4], float weight = 1.0f) {
+    const float amax = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
+    QueryPart p;
+    float mul;
+    range_factor(amax, mul, p.inv);
+    mul *= weight;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = x[i] * mul;
+        p.hi[i] = __float2half_rn(y);
+        p.lo[i] = __float2half_rn(y - __half2float(p.hi[i]));
+    }
+    return p;
+}
+
 // Where a lane finds its rows of 16 consecutive positions, numbered within the
 // layer (fewer than 2^32, checked by the entry point).
 struct Pos16 {
@@ -164,37 +204,43 @@ struct F16Rows {
     float inv[NB];
     uint4 kr[kSub][2][HD / 32], vr[kSub][4][HD / 64];
 
-    // B fragments from the unit's queries qs[head][HD]; columns of heads past n_heads are zero.
-    __device__ __forceinline__ void load_q(const float *qs, int n_heads, float qscale, int lane) {
+    // B fragments of the unit's queries (element q0 of q): a lane splits 4
+    // elements of a head at a time into buf[head][hi, lo][HD] (halves), from where
+    // each lane's fragments are 16-byte words.  Columns of heads past n_heads are zero.
+    template <int ACT>
+    __device__ __forceinline__ void load_q(const void *src, long long q0, int n_heads, float qscale, float *buf, int lane) {
         const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) inv[nb] = 1.0f;
+#pragma unroll 1
+        for (int h0 = 0; h0 < n_heads; h0 += 4) {
+            float x[4][4];  // four heads' loads in flight
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (h0 + j < n_heads) query_load<ACT, HD>(src, q0 + (h0 + j) * HD, lane, x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (h0 + j >= n_heads) continue;
+                const QueryPart p = query_part(x[j]);
+                if (4 * lane < HD) {
+                    uint2 *dst = reinterpret_cast<uint2 *>(buf + (h0 + j) * HD) + lane;
+                    dst[0] = make_uint2(half_bits2(p.hi[0], p.hi[1]), half_bits2(p.hi[2], p.hi[3]));
+                    dst[HD / 4] = make_uint2(half_bits2(p.lo[0], p.lo[1]), half_bits2(p.lo[2], p.lo[3]));
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+                    if (h0 == 4 * nb && j == t) inv[nb] = p.inv * qscale;
+            }
+        }
+        __syncwarp();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int h = 4 * nb + (g >> 1);
-            const float4 *src = reinterpret_cast<const float4 *>(qs + (h < n_heads ? h : 0) * HD + 8 * t);
-            float x[HD / 4];
-            float amax = 0.0f;
+            const uint4 *frag = reinterpret_cast<const uint4 *>(buf + (h < n_heads ? h : 0) * HD) + (g & 1) * (HD / 8) + t;
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const float4 f = src[8 * c + u];
-                    x[8 * c + 4 * u] = f.x, x[8 * c + 4 * u + 1] = f.y;
-                    x[8 * c + 4 * u + 2] = f.z, x[8 * c + 4 * u + 3] = f.w;
-                }
-#pragma unroll
-            for (int i = 0; i < HD / 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            float mul, iv;
-            range_factor(amax, mul, iv);
-            inv[nb] = __shfl_sync(0xffffffffu, iv, 8 * t) * qscale;  // of head t, from lane (g = 2t, 0)
-#pragma unroll
-            for (int i = 0; i < HD / 8; ++i) {  // element pairs (2i, 2i + 1) of this lane
-                const float y0 = h < n_heads ? x[2 * i] * mul : 0.0f, y1 = h < n_heads ? x[2 * i + 1] * mul : 0.0f;
-                __half2 h2 = __floats2half2_rn(y0, y1);
-                const float2 f = __half22float2(h2);
-                if (g & 1) h2 = __floats2half2_rn(y0 - f.x, y1 - f.y);
-                q[nb][i / 2][i % 2] = *reinterpret_cast<const uint32_t *>(&h2);
+            for (int c = 0; c < HD / 32; ++c) {
+                const uint4 u = h < n_heads ? frag[4 * c] : make_uint4(0, 0, 0, 0);
+                q[nb][2 * c][0] = u.x, q[nb][2 * c][1] = u.y, q[nb][2 * c + 1][0] = u.z, q[nb][2 * c + 1][1] = u.w;
             }
         }
     }
@@ -219,12 +265,12 @@ struct F16Rows {
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two shorter chains
+            float c[4], d[4];  // two shorter chains
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) {
                 const uint4 x = kr[s][0][j], y = kr[s][1][j];
-                mma16816(c, x.x, y.x, x.y, y.y, q[nb][2 * j][0], q[nb][2 * j][1]);
-                mma16816(d, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
+                mma16816(c, j == 0, x.x, y.x, x.y, y.y, q[nb][2 * j][0], q[nb][2 * j][1]);
+                mma16816(d, j == 0, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
             }
             sc[nb][0] = ((c[0] + d[0]) + (c[1] + d[1])) * inv[nb];
             sc[nb][1] = ((c[2] + d[2]) + (c[3] + d[3])) * inv[nb];
@@ -246,7 +292,7 @@ struct F16Rows {
             }
 #pragma unroll
         for (int j = 0; j < kO; ++j) {
-            float sum[NB][4] = {};
+            float sum[NB][4];
 #pragma unroll
             for (int s = 0; s < kSub; ++s) {
                 const uint32_t v0 = word(vr[s][0][j / 4], j % 4), v1 = word(vr[s][1][j / 4], j % 4),
@@ -254,7 +300,7 @@ struct F16Rows {
                 const uint32_t a0 = __byte_perm(v0, v1, 0x5410), a1 = __byte_perm(v0, v1, 0x7632);
                 const uint32_t a2 = __byte_perm(v2, v3, 0x5410), a3 = __byte_perm(v2, v3, 0x7632);
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) mma16816(sum[nb], a0, a1, a2, a3, b[s][nb][0], b[s][nb][1]);
+                for (int nb = 0; nb < NB; ++nb) mma16816(sum[nb], s == 0, a0, a1, a2, a3, b[s][nb][0], b[s][nb][1]);
             }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -291,47 +337,46 @@ struct Q4Rows {
     uint32_t kr[kSub][2][kKW], vr[kSub][4][kVW];
     __half ks[kSub][2], vs[kSub][2];
 
-    __device__ __forceinline__ void load_q(const float *qs, int, float qscale, int lane) {
+    // B fragments of the query: a lane splits 4 elements, elements 16..31 of a
+    // block divided by 16, and puts them where the lanes that hold their codes
+    // find their fragments as 16-byte words: buf[block][hi, lo][16] (pairs of halves).
+    template <int ACT>
+    __device__ __forceinline__ void load_q(const void *src, long long q0, int, float qscale, float *buf, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        // lane t holds words of block blk from byte `byte`; column pair g / 2 is block g / 2
-        const int blk = HD == 128 ? t : t >> 1, byte = HD == 128 ? 0 : 8 * (t & 1);
+        uint32_t *frag = reinterpret_cast<uint32_t *>(buf);
+        const int i = lane & 7;  // elements 4i.. of block lane / 8
+        float e[4];
+        query_load<ACT, HD>(src, q0, lane, e);
+        const QueryPart x = query_part(e, i < 4 ? 1.0f : 0.0625f);
+        inv = x.inv * qscale;
+        const float weight = i < 4 ? 1.0f : 16.0f;
+        float sum_hi = weight * ((__half2float(x.hi[0]) + __half2float(x.hi[1])) + (__half2float(x.hi[2]) + __half2float(x.hi[3])));
+        float sum_lo = weight * ((__half2float(x.lo[0]) + __half2float(x.lo[1])) + (__half2float(x.lo[2]) + __half2float(x.lo[3])));
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, d);
+            sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, d);
+        }
+        if (4 * lane < HD) {
+            // word 4 (i % 4): codes of bytes 4 (i % 4).. : elements 0, 2 then 1, 3; low nibbles before high ones
+            uint32_t *dst = frag + (lane >> 3) * 32 + 4 * (i & 3) + (i >> 2);
+            dst[0] = half_bits2(x.hi[0], x.hi[2]), dst[2] = half_bits2(x.hi[1], x.hi[3]);
+            dst[16] = half_bits2(x.lo[0], x.lo[2]), dst[18] = half_bits2(x.lo[1], x.lo[3]);
+        }
+        // the sums of columns 2t, 2t + 1 start at -8 2^-24 sum q of block t
+        bias[0] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum_hi, (8 * t) & 31);
+        bias[1] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum_lo, (8 * t) & 31);
+        if (t >= kBlocks) bias[0] = bias[1] = 0.0f;
+        __syncwarp();
+        // lane t holds bytes 4 w.. of block blk, w in [w0, w0 + kKW); column pair g / 2 is block g / 2
+        const int blk = HD == 128 ? t : t >> 1, w0 = HD == 128 ? 0 : 2 * (t & 1);
         const bool mine = (g >> 1) == blk;
-        float lo[4 * kKW], hi[4 * kKW];  // elements byte + i and 16 + byte + i of the block
-        float amax = 0.0f;
-        const float4 *src = reinterpret_cast<const float4 *>(qs + 32 * blk + byte);
+        const uint4 *words = reinterpret_cast<const uint4 *>(frag + blk * 32 + (g & 1) * 16) + w0;
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
-            const float4 x = src[w], y = src[4 + w];
-            lo[4 * w] = x.x, lo[4 * w + 1] = x.y, lo[4 * w + 2] = x.z, lo[4 * w + 3] = x.w;
-            hi[4 * w] = y.x, hi[4 * w + 1] = y.y, hi[4 * w + 2] = y.z, hi[4 * w + 3] = y.w;
+            const uint4 u = mine ? words[w] : make_uint4(0, 0, 0, 0);
+            q[2 * w][0] = u.x, q[2 * w][1] = u.y, q[2 * w + 1][0] = u.z, q[2 * w + 1][1] = u.w;
         }
-#pragma unroll
-        for (int i = 0; i < 4 * kKW; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        float mul;
-        range_factor(amax, mul, inv);
-        inv *= qscale;
-        float sum = 0.0f;
-        auto part = [&](float x, float weight) {
-            const float y = mine ? x * mul : 0.0f;
-            __half h = __float2half_rn(y);
-            if (g & 1) h = __float2half_rn(y - __half2float(h));
-            sum += weight * __half2float(h);
-            return h;
-        };
-#pragma unroll
-        for (int w = 0; w < kKW; ++w) {
-            q[2 * w][0] = half_bits2(part(lo[4 * w], 1.0f), part(lo[4 * w + 2], 1.0f));
-            q[2 * w][1] = half_bits2(part(0.0625f * hi[4 * w], 16.0f), part(0.0625f * hi[4 * w + 2], 16.0f));
-            q[2 * w + 1][0] = half_bits2(part(lo[4 * w + 1], 1.0f), part(lo[4 * w + 3], 1.0f));
-            q[2 * w + 1][1] = half_bits2(part(0.0625f * hi[4 * w + 1], 16.0f), part(0.0625f * hi[4 * w + 3], 16.0f));
-        }
-        // of columns 2t, 2t + 1: from a lane that holds block t
-        if (HD == 64) sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        const int from = HD == 128 ? 9 * t : 8 * t + (2 * t & 3);
-        bias[0] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum, from);      // -8 * 2^-24
-        bias[1] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum, from + 4);
     }
     const char *kp, *vp;        // the lane's bytes of row 0
     const __half *ksp, *vsp;    // its block's scales
@@ -371,13 +416,14 @@ struct Q4Rows {
     // start at -8 sum q, which makes them those of n - 8.  (Not done for the values: there the
     // offset would be summed over all positions and cost digits.)
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
-        float c[4] = {bias[0], bias[1], bias[0], bias[1]}, d[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two shorter chains
+        float c[4], d[4];  // two shorter chains
         constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
             const uint32_t x = kr[s][0][w], y = kr[s][1][w], x8 = x >> 8, y8 = y >> 8;
-            mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
-            mma16816(d, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
+            if (w == 0) mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[0][0], q[0][1], bias[0], bias[1]);
+            else mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
+            mma16816(d, w == 0, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
         }
         // lanes past the row's blocks hold zero sums
         sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (__half2float(ks[s][0]) * 16777216.0f);
@@ -420,13 +466,13 @@ struct Q4Rows {
         for (int i = 0; i < kVW; ++i) {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float even[4] = {}, odd[4] = {};
+                float even[4], odd[4];
 #pragma unroll
                 for (int s = 0; s < kSub; ++s) {
                     const uint32_t x = __byte_perm(vr[s][0][i], vr[s][1][i], u ? 0x7632 : 0x5410);
                     const uint32_t y = __byte_perm(vr[s][2][i], vr[s][3][i], u ? 0x7632 : 0x5410);
-                    mma16816(even, codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y), b[s][0], b[s][1]);
-                    mma16816(odd, codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8), b[s][0], b[s][1]);
+                    mma16816(even, s == 0, codes_lo(x), codes_hi(x), codes_lo(y), codes_hi(y), b[s][0], b[s][1]);
+                    mma16816(odd, s == 0, codes_lo(x >> 8), codes_hi(x >> 8), codes_lo(y >> 8), codes_hi(y >> 8), b[s][0], b[s][1]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[0][4 * i + 2 * u][c] += even[c], o[0][4 * i + 2 * u + 1][c] += odd[c];
@@ -474,7 +520,7 @@ constexpr int kMaxGrid = 640;
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m - kHead + log2f(l)) * kLn2; }
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : __frcp_rn(l); }
 
-constexpr int kJoinBatch = 8;  // pieces requested at a time
+constexpr int kJoinBatch = 16;  // pieces requested at a time
 
 // Release of the CTA's earlier writes (ordered by a barrier before it) and acquire of the others'.
 __device__ __forceinline__ int arrive(int *p) {
@@ -625,14 +671,6 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const int *table = a.table + static_cast<long long>(req) * a.max_blocks;
         int b0 = pa_div(max(start, pbase + tile0 * kTile), a.page);
         int entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
-        __syncwarp();
-        const long long q0 = row * a.q_stride + static_cast<long long>(hd.head0) * HD + lane;
-#pragma unroll 1
-        for (int h = 0; h < hd.heads; ++h)
-#pragma unroll
-            for (int i = 0; i < HD; i += 32) buf[h * HD + i + lane] = act_load<ACT>(a.q, q0 + h * HD + i);
-        __syncwarp();
-
         float o[NB][kO][4], m[NB], l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -643,7 +681,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 for (int i = 0; i < 4; ++i) o[nb][j][i] = 0.0f;
         }
         R_.reset();
-        R_.load_q(buf, hd.heads, a.qscale, lane);
+        __syncwarp();  // the last head's outputs have been read from buf
+        R_.template load_q<ACT>(a.q, row * a.q_stride + static_cast<long long>(hd.head0) * HD, hd.heads, a.qscale, buf, lane);
         Pos16 P[R::kSub];
         constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << kTile) - 1;
         uint32_t there = 0;  // positions attended to of the tile whose keys are requested
