@@ -37,6 +37,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../paged.h"
 #include "common.cuh"
@@ -109,10 +110,13 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ uint32_t split_half(float x) {  // (hi, lo)
-    const __half hi = __float2half_rn(x);
-    const __half2 p = __halves2half2(hi, __float2half_rn(x - __half2float(hi)));
-    return *reinterpret_cast<const uint32_t *>(&p);
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t &px, uint32_t &py) {  // (hi, lo) of x, of y
+    const __half2 hi = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(hi);
+    const __half2 lo = __floats2half2_rn(x - f.x, y - f.y);
+    const uint32_t h = *reinterpret_cast<const uint32_t *>(&hi), l = *reinterpret_cast<const uint32_t *>(&lo);
+    px = __byte_perm(h, l, 0x5410);
+    py = __byte_perm(h, l, 0x7632);
 }
 __device__ __forceinline__ uint32_t half_bits2(__half a, __half b) {
     const __half2 p = __halves2half2(a, b);
@@ -122,12 +126,14 @@ __device__ __forceinline__ uint32_t half_bits2(__half a, __half b) {
 // Codes 0..15 at bits 0-3 and 16-19 (or 4-7 and 20-23) of w as halves n - 8:
 // the code is placed in the mantissa of 1024 and the offset taken away.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
-    const uint32_t m = (w & 0x000f000fu) | 0x64006400u;
+    uint32_t m;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(m) : "r"(w));  // (w & mask) | 1024.0
     const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&m), __float2half2_rn(1032.0f));
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ uint32_t codes_hi(uint32_t w) {
-    const uint32_t m = (w & 0x00f000f0u) | 0x64006400u;
+    uint32_t m;
+    asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(m) : "r"(w));
     const __half2 h =
         __hfma2(*reinterpret_cast<const __half2 *>(&m), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -184,12 +190,27 @@ __device__ __forceinline__ QueryPart query_part(const float (&x)[4], float weigh
     return p;
 }
 
-// Where a lane finds its rows of 16 consecutive positions, numbered within the
-// layer (fewer than 2^32, checked by the entry point).
-struct Pos16 {
-    uint32_t row[2];   // position g, g + 8 (scores)
-    uint32_t vrow[4];  // positions 2t, 2t + 1, 2t + 8, 2t + 9
+// Rows of 16 consecutive positions of a layer, numbered from 0 (fewer than
+// 2^32, checked by the entry point).  Pages of a multiple of 16 positions:
+// one number, of position 0.  Other page sizes: each lane's own rows, each
+// less the position's number, so that the addresses are formed the same way.
+template <bool kAligned>
+struct Pos16;
+template <>
+struct Pos16<true> {
+    uint32_t first;
+    __device__ __forceinline__ long long key(int) const { return first; }
+    __device__ __forceinline__ long long value(int) const { return first; }
 };
+template <>
+struct Pos16<false> {
+    long long k[2], v[4];
+    __device__ __forceinline__ long long key(int i) const { return k[i]; }
+    __device__ __forceinline__ long long value(int i) const { return v[i]; }
+};
+// Position that a lane holds: i-th of its keys, of its values.
+__device__ __forceinline__ int key_pos(int lane, int i) { return (lane >> 2) + 8 * i; }
+__device__ __forceinline__ int value_pos(int lane, int i) { return 2 * (lane & 3) + (i & 1) + 4 * (i & 2); }
 
 // ---- fp16 rows ----
 template <int HD_, int NB_>
@@ -244,22 +265,34 @@ struct F16Rows {
             }
         }
     }
-    const char *kp, *vp;  // the lane's bytes of row 0
+    const char *kp, *vp;  // the lane's bytes of positions g and 2t, were they in rows g and 2t
     __device__ __forceinline__ F16Rows(const PagedAttnArgs &a, int lane)
-        : kp(static_cast<const char *>(a.k) + 16 * (lane & 3)), vp(static_cast<const char *>(a.v) + 16 * (lane >> 2)) {}
-    __device__ __forceinline__ void load_k(int s, const Pos16 &p) {
+        : kp(static_cast<const char *>(a.k) + 2 * HD * (lane >> 2) + 16 * (lane & 3)),
+          vp(static_cast<const char *>(a.v) + 4 * HD * (lane & 3) + 16 * (lane >> 2)) {}
+    template <class P>
+    __device__ __forceinline__ void load_k(int s, const P &p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int c = 0; c < HD / 32; ++c)
-                kr[s][i][c] = ldg_stream16(kp + static_cast<size_t>(p.row[i]) * (2 * HD) + 64 * c);
+            for (int c = 0; c < HD / 32; ++c) kr[s][i][c] = ldg_stream16(kp + p.key(i) * (2 * HD) + 16 * HD * i + 64 * c);
     }
-    __device__ __forceinline__ void load_v(int s, const Pos16 &p) {
+    template <class P>
+    __device__ __forceinline__ void load_v(int s, const P &p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
-                vr[s][i][c] = ldg_stream16(vp + static_cast<size_t>(p.vrow[i]) * (2 * HD) + 128 * c);
+                vr[s][i][c] = ldg_stream16(vp + p.value(i) * (2 * HD) + 2 * HD * value_pos(0, i) + 128 * c);
+    }
+    // Values of positions that are left out (bit 0 in `there`) must not meet their weight 0 as NaN.
+    __device__ __forceinline__ void clear_values(uint32_t there, int lane) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!(there >> (16 * s + value_pos(lane, i)) & 1))
+#pragma unroll
+                    for (int c = 0; c < HD / 64; ++c) vr[s][i][c] = make_uint4(0, 0, 0, 0);
     }
     // sc[nb][i]: score (log2 units) of position g + 8 i for head (nb, t)
     __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
@@ -287,8 +320,9 @@ struct F16Rows {
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                b[s][nb][0] = transpose8(split_half(w[s][nb][0]));
-                b[s][nb][1] = transpose8(split_half(w[s][nb][1]));
+                split_half2(w[s][nb][0], w[s][nb][1], b[s][nb][0], b[s][nb][1]);
+                b[s][nb][0] = transpose8(b[s][nb][0]);
+                b[s][nb][1] = transpose8(b[s][nb][1]);
             }
 #pragma unroll
         for (int j = 0; j < kO; ++j) {
@@ -378,15 +412,18 @@ struct Q4Rows {
             q[2 * w][0] = u.x, q[2 * w][1] = u.y, q[2 * w + 1][0] = u.z, q[2 * w + 1][1] = u.w;
         }
     }
-    const char *kp, *vp;        // the lane's bytes of row 0
-    const __half *ksp, *vsp;    // its block's scales
+    const char *kp, *vp;        // the lane's bytes of positions g and 2t, were they in rows g and 2t
+    const __half *ksp, *vsp;    // scales of its block of position g
     __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, int lane)
-        : kp(static_cast<const char *>(a.k) + 4 * kKW * (lane & 3)), vp(static_cast<const char *>(a.v) + 4 * kVW * (lane >> 2)),
-          ksp(a.k_scale + (lane & 3) % kBlocks), vsp(a.v_scale + (lane & 3) % kBlocks) {}
-    __device__ __forceinline__ void load_k(int s, const Pos16 &p) {
+        : kp(static_cast<const char *>(a.k) + HD / 2 * (lane >> 2) + 4 * kKW * (lane & 3)),
+          vp(static_cast<const char *>(a.v) + HD * (lane & 3) + 4 * kVW * (lane >> 2)),
+          ksp(a.k_scale + kBlocks * (lane >> 2) + (lane & 3) % kBlocks),
+          vsp(a.v_scale + kBlocks * (lane >> 2) + (lane & 3) % kBlocks) {}
+    template <class P>
+    __device__ __forceinline__ void load_k(int s, const P &p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const char *src = kp + static_cast<size_t>(p.row[i]) * (HD / 2);
+            const char *src = kp + p.key(i) * (HD / 2) + 4 * HD * i;
             if constexpr (HD == 128) {
                 const uint4 x = ldg_stream16(src);
                 kr[s][i][0] = x.x, kr[s][i][1] = x.y, kr[s][i][2] = x.z, kr[s][i][3] = x.w;
@@ -394,13 +431,14 @@ struct Q4Rows {
                 const uint2 x = ldg_stream8(src);
                 kr[s][i][0] = x.x, kr[s][i][1] = x.y;
             }
-            ks[s][i] = __ldg(ksp + static_cast<size_t>(p.row[i]) * kBlocks);
+            ks[s][i] = __ldg(ksp + p.key(i) * kBlocks + 8 * kBlocks * i);
         }
     }
-    __device__ __forceinline__ void load_v(int s, const Pos16 &p) {
+    template <class P>
+    __device__ __forceinline__ void load_v(int s, const P &p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const char *src = vp + static_cast<size_t>(p.vrow[i]) * (HD / 2);
+            const char *src = vp + p.value(i) * (HD / 2) + HD / 2 * value_pos(0, i);
             if constexpr (HD == 128) {
                 const uint2 x = ldg_stream8(src);
                 vr[s][i][0] = x.x, vr[s][i][1] = x.y;
@@ -409,7 +447,15 @@ struct Q4Rows {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) vs[s][i] = __ldg(vsp + static_cast<size_t>(p.row[i]) * kBlocks);
+        for (int i = 0; i < 2; ++i) vs[s][i] = __ldg(vsp + p.key(i) * kBlocks + 8 * kBlocks * i);
+    }
+    // Scales of positions that are left out must not meet their weight 0 as NaN (codes are always finite).
+    __device__ __forceinline__ void clear_values(uint32_t there, int lane) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (!(there >> (16 * s + key_pos(lane, i)) & 1)) vs[s][i] = __ushort_as_half(0);
     }
     // A: codes n as subnormal halves, n 2^-24 (low nibbles) and 16 n 2^-24 (high
     // nibbles, whose q is divided by 16), so a code costs half a mask; the sums
@@ -458,10 +504,11 @@ struct Q4Rows {
     __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
         uint32_t b[kSub][2];
 #pragma unroll
-        for (int s = 0; s < kSub; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)  // w * scale / vlim <= 2^15
-                b[s][i] = transpose8(split_half(w[s][0][i] * (__half2float(vs[s][i]) * vinv)));  // columns of no block: unused
+        for (int s = 0; s < kSub; ++s) {  // w * scale / vlim <= 2^15; columns of no block are not used
+            split_half2(w[s][0][0] * (__half2float(vs[s][0]) * vinv), w[s][0][1] * (__half2float(vs[s][1]) * vinv), b[s][0], b[s][1]);
+            b[s][0] = transpose8(b[s][0]);
+            b[s][1] = transpose8(b[s][1]);
+        }
 #pragma unroll
         for (int i = 0; i < kVW; ++i) {
 #pragma unroll
@@ -552,7 +599,7 @@ constexpr size_t kFixedSmem = (sizeof(PaSmem<HD, NH>) + 15) / 16 * 16;
 template <class R>
 constexpr int pa_piece_floats = (R::kHeads * (R::HD + 2) + 3) / 4 * 4;
 
-template <class R, int ACT>
+template <class R, int ACT, bool kAligned>
 __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
     constexpr int HD = R::HD, NB = R::NB, NH = R::kHeads, kTile = 16 * R::kSub, kO = R::kO;
     using Smem = PaSmem<HD, NH>;
@@ -669,8 +716,15 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
 
         // entries [b0, b0 + 32) of the row of the block table, one a lane
         const int *table = a.table + static_cast<long long>(req) * a.max_blocks;
-        int b0 = pa_div(max(start, pbase + tile0 * kTile), a.page);
-        int entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
+        const int from_pos = kAligned ? pbase + tile0 * kTile : max(start, pbase + tile0 * kTile);
+        int block = pa_div(from_pos, a.page);         // of the next 16 positions
+        uint32_t offset = from_pos - block * a.page.d;  // of these in their page
+        int b0, entry;
+        auto refill = [&] {
+            b0 = block;
+            entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
+        };
+        refill();
         float o[NB][kO][4], m[NB], l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -683,7 +737,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         R_.reset();
         __syncwarp();  // the last head's outputs have been read from buf
         R_.template load_q<ACT>(a.q, row * a.q_stride + static_cast<long long>(hd.head0) * HD, hd.heads, a.qscale, buf, lane);
-        Pos16 P[R::kSub];
+        Pos16<kAligned> P[R::kSub];
         constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << kTile) - 1;
         uint32_t there = 0;  // positions attended to of the tile whose keys are requested
         // Step `tile` uses the keys requested in the step before, requests its
@@ -708,34 +762,46 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 }
             }
             if (tile + 1 < tile1) {
-                // lane i finds the row of the tile's position i (mod 16), the others read it from there
                 const int p0 = pbase + (tile + 1) * kTile;
-                const int last = min(p0 + kTile, len) - 1;
-                if (static_cast<int>(pa_div(last, a.page)) >= b0 + 32) {
-                    b0 = pa_div(max(p0, start), a.page);
-                    entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
-                }
-                const int p = p0 + (lane & (kTile - 1));
-                const bool in = p >= start && p <= last;
-                const int b = in ? pa_div(p, a.page) : b0;
-                const int page = __shfl_sync(0xffffffffu, entry, b - b0);
-                const bool ok = page >= 0 && page < a.n_pages;
-                bad |= in && !ok;
-                uint32_t r = (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p;
-                there = __ballot_sync(0xffffffffu, in && ok) & kAll;
-                if (there) {
-                    // a position that is left out reads a row that is not, with weight 0
-                    if (there != kAll) {
-                        const uint32_t other = __shfl_sync(0xffffffffu, r, __ffs(there) - 1);
-                        r = in && ok ? r : other;
-                    }
+                there = kAll;
+                if (p0 < start) there &= kAll << (start - p0);
+                if (p0 + kTile > len) there &= kAll >> (p0 + kTile - len);
+                // what is left out reads some row (row 0 in the place of an invalid page) and is masked later
+                if constexpr (kAligned) {
 #pragma unroll
                     for (int s = 0; s < R::kSub; ++s) {
-                        P[s].row[0] = __shfl_sync(0xffffffffu, r, 16 * s + g);
-                        P[s].row[1] = __shfl_sync(0xffffffffu, r, 16 * s + g + 8);
+                        if (block >= b0 + 32) refill();
+                        const int page = __shfl_sync(0xffffffffu, entry, block - b0);
+                        const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+                        P[s].first = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + offset : 0;
+                        if (!ok) {
+                            bad |= (there >> (16 * s) & 0xffff) != 0;
+                            there &= ~(0xffffu << (16 * s));
+                        }
+                        offset += 16;
+                        if (offset == a.page.d) offset = 0, ++block;
+                        R_.load_k(s, P[s]);
+                    }
+                } else {
+                    // lane i finds the row of the tile's position i (mod 16), the others get it from there
+                    const int p = p0 + (lane & (kTile - 1));
+                    const bool in = p >= start && p < len;
+                    const int b = pa_div(p, a.page);
+                    block = pa_div(max(p0, start), a.page);
+                    if (static_cast<int>(pa_div(min(p0 + kTile, len) - 1, a.page)) >= b0 + 32) refill();
+                    const int page = __shfl_sync(0xffffffffu, entry, in ? b - b0 : 0);
+                    const bool ok = in && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+                    bad |= in && !ok;
+                    const uint32_t r = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p : 0;
+                    there = __ballot_sync(0xffffffffu, ok) & kAll;
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            P[s].k[i] = static_cast<long long>(__shfl_sync(0xffffffffu, r, 16 * s + key_pos(lane, i))) - key_pos(lane, i);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            P[s].vrow[i] = __shfl_sync(0xffffffffu, r, 16 * s + 2 * t + (i & 1) + 4 * (i & 2));
+                            P[s].v[i] = static_cast<long long>(__shfl_sync(0xffffffffu, r, 16 * s + value_pos(lane, i))) - value_pos(lane, i);
                         R_.load_k(s, P[s]);
                     }
                 }
@@ -763,6 +829,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         for (int i = 0; i < 4; ++i) o[nb][j][i] *= f;
                 }
             }
+            if (now != kAll) R_.clear_values(now, lane);
             bool wide = false;
 #pragma unroll
             for (int s = 0; s < R::kSub; ++s) wide |= R_.value_range(s);
@@ -951,7 +1018,7 @@ constexpr int kMaxDevices = 64;
 
 // CTAs of a launch on the current device: all that are resident at once, at
 // most kMaxGrid (0: the kernel cannot run here).
-template <class R, int ACT>
+template <class R, int ACT, bool kAligned>
 cudaError_t pa_grid(int &grid) {
     static std::atomic<int> known[kMaxDevices];
     int dev = 0;
@@ -959,11 +1026,11 @@ cudaError_t pa_grid(int &grid) {
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices && (grid = known[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
     constexpr int smem = static_cast<int>(kFixedSmem<R::HD, R::kHeads> + 4 * kPagedMaxRows);
-    e = cudaFuncSetAttribute(paged_attn_kernel<R, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    e = cudaFuncSetAttribute(paged_attn_kernel<R, ACT, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     int sms = 0, per_sm = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R, ACT>, kPaThreads, smem)) !=
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R, ACT, kAligned>, kPaThreads, smem)) !=
         cudaSuccess)
         return e;
     grid = sms * per_sm < kMaxGrid ? sms * per_sm : kMaxGrid;
@@ -975,10 +1042,10 @@ cudaError_t pa_grid(int &grid) {
 template <class R>
 constexpr size_t kScratch = (4 * kMaxGrid + 255) / 256 * 256 + sizeof(float) * kMaxGrid * 2 * pa_piece_floats<R>;
 
-template <class R, int ACT>
+template <class R, int ACT, bool kAligned>
 cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cudaStream_t s) {
     int grid = 0;
-    const cudaError_t e = pa_grid<R, ACT>(grid);
+    const cudaError_t e = pa_grid<R, ACT, kAligned>(grid);
     if (e != cudaSuccess) return e;
     if (scratch_bytes < kScratch<R>) return cudaErrorInvalidValue;
     a.group = a.n_heads / a.n_kv_heads;
@@ -987,7 +1054,7 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     a.units = make_fast_div(a.n_kv_heads * chunks);
     a.cnt = static_cast<int *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
-    paged_attn_kernel<R, ACT><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
+    paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -1014,9 +1081,15 @@ cudaError_t launch_paged_attention(PagedAttnArgs a, int head_dim, int kv_type, i
                                    size_t scratch_bytes, cudaStream_t s) {
     return pa_variant(head_dim, kv_type, a.n_heads / a.n_kv_heads, [&](auto r) {
         using R = typename decltype(r)::Rows;
-        if (act == BMO_ACT_F32) return pa_launch<R, BMO_ACT_F32>(a, scratch, scratch_bytes, s);
-        if (act == BMO_ACT_F16) return pa_launch<R, BMO_ACT_F16>(a, scratch, scratch_bytes, s);
-        return pa_launch<R, BMO_ACT_BF16>(a, scratch, scratch_bytes, s);
+        const bool aligned = a.page.d % 16 == 0;
+        auto run = [&](auto type) {
+            constexpr int kAct = decltype(type)::value;
+            return aligned ? pa_launch<R, kAct, true>(a, scratch, scratch_bytes, s)
+                           : pa_launch<R, kAct, false>(a, scratch, scratch_bytes, s);
+        };
+        if (act == BMO_ACT_F32) return run(std::integral_constant<int, BMO_ACT_F32>{});
+        if (act == BMO_ACT_F16) return run(std::integral_constant<int, BMO_ACT_F16>{});
+        return run(std::integral_constant<int, BMO_ACT_BF16>{});
     });
 }
 
