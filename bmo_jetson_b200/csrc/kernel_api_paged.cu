@@ -29,7 +29,7 @@ bool cache_ok(const bmo_paged_kv *c) {
     if (c->n_layers <= 0 || c->n_kv_heads <= 0 || (c->head_dim != 64 && c->head_dim != 128)) return false;
     // the kernels number a layer's rows in 32 bits
     if (static_cast<long long>(c->book.n_pages) * c->book.page_size > 0xfffffffell / c->n_kv_heads) return false;
-    if (c->kv_type == kKvQ4_0) return c->k_scale && c->v_scale && aligned(c->k_scale, 2) && aligned(c->v_scale, 2);
+    if (c->kv_type == kKvQ4_0) return c->k_scale && c->v_scale && aligned(c->k_scale, 16) && aligned(c->v_scale, 16);
     return c->kv_type == kKvF16;
 }
 

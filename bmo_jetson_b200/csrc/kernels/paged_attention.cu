@@ -199,12 +199,17 @@ struct Pos16;
 template <>
 struct Pos16<true> {
     uint32_t first;
+    __device__ __forceinline__ long long row(int) const { return first; }
     __device__ __forceinline__ long long key(int) const { return first; }
     __device__ __forceinline__ long long value(int) const { return first; }
 };
 template <>
 struct Pos16<false> {
     long long k[2], v[4];
+    uint32_t mine;  // row of position lane % 16
+    __device__ __forceinline__ long long row(int i) const {  // every lane of the warp asks
+        return static_cast<long long>(__shfl_sync(0xffffffffu, mine, i)) - i;
+    }
     __device__ __forceinline__ long long key(int i) const { return k[i]; }
     __device__ __forceinline__ long long value(int i) const { return v[i]; }
 };
@@ -265,10 +270,18 @@ struct F16Rows {
             }
         }
     }
+    // Rows go straight into registers: the next tile's keys are requested as
+    // soon as a tile's scores are formed, its values at the start of its step.
+    static constexpr int kAhead = 1, kRing = 0;
     const char *kp, *vp;  // the lane's bytes of positions g and 2t, were they in rows g and 2t
-    __device__ __forceinline__ F16Rows(const PagedAttnArgs &a, int lane)
+    __device__ __forceinline__ F16Rows(const PagedAttnArgs &a, char *, int lane)
         : kp(static_cast<const char *>(a.k) + 2 * HD * (lane >> 2) + 16 * (lane & 3)),
           vp(static_cast<const char *>(a.v) + 4 * HD * (lane & 3) + 16 * (lane >> 2)) {}
+    template <class P>
+    __device__ __forceinline__ void request(int, const P (&p)[kSub], int) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) load_k(s, p[s]);
+    }
     template <class P>
     __device__ __forceinline__ void load_k(int s, const P &p) {
 #pragma unroll
@@ -295,7 +308,7 @@ struct F16Rows {
                     for (int c = 0; c < HD / 64; ++c) vr[s][i][c] = make_uint4(0, 0, 0, 0);
     }
     // sc[nb][i]: score (log2 units) of position g + 8 i for head (nb, t)
-    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2], int) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float c[4], d[4];  // two shorter chains
@@ -309,12 +322,15 @@ struct F16Rows {
             sc[nb][1] = ((c[2] + d[2]) + (c[3] + d[3])) * inv[nb];
         }
     }
+    __device__ __forceinline__ void commit() {}
+    __device__ __forceinline__ void wait() {}
+    __device__ __forceinline__ void next() {}
     __device__ __forceinline__ bool value_range(int) { return false; }
     __device__ __forceinline__ void raise_value_range(float (&)[NB][kO][4]) {}
     __device__ __forceinline__ void reset() {}
     // Adds the weighted values of the tile.  The tensor core's sum of a tile
     // starts from zero and is added in fp32: its own running sum is not rounded to nearest.
-    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4], int) {
         uint32_t b[kSub][NB][2];
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
@@ -358,6 +374,7 @@ template <int HD_>
 struct Q4Rows {
     static constexpr int HD = HD_, NB = 1;
     static constexpr int kMinCtas = 3;
+    static constexpr int kStages = 3;
     static constexpr int kHeadCost = 2;
     static constexpr int kHeads = 1;
     static constexpr int kSub = 2;
@@ -368,9 +385,7 @@ struct Q4Rows {
     uint32_t q[HD / 16][2];
     float inv, bias[2];
     float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
-    uint32_t kr[kSub][2][kKW], vr[kSub][4][kVW];
-    __half ks[kSub][2], vs[kSub][2];
-
+    __half vs[kSub][2];
     // B fragments of the query: a lane splits 4 elements, elements 16..31 of a
     // block divided by 16, and puts them where the lanes that hold their codes
     // find their fragments as 16-byte words: buf[block][hi, lo][16] (pairs of halves).
@@ -412,43 +427,59 @@ struct Q4Rows {
             q[2 * w][0] = u.x, q[2 * w][1] = u.y, q[2 * w + 1][0] = u.z, q[2 * w + 1][1] = u.w;
         }
     }
-    const char *kp, *vp;        // the lane's bytes of positions g and 2t, were they in rows g and 2t
-    const __half *ksp, *vsp;    // scales of its block of position g
-    __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, int lane)
-        : kp(static_cast<const char *>(a.k) + HD / 2 * (lane >> 2) + 4 * kKW * (lane & 3)),
-          vp(static_cast<const char *>(a.v) + HD * (lane & 3) + 4 * kVW * (lane >> 2)),
-          ksp(a.k_scale + kBlocks * (lane >> 2) + (lane & 3) % kBlocks),
-          vsp(a.v_scale + kBlocks * (lane >> 2) + (lane & 3) % kBlocks) {}
+    // Rows reach shared memory by asynchronous copies, kAhead tiles ahead (the
+    // arithmetic on codes leaves no registers to hold that much): a stage is
+    // the tile's key codes, value codes, key scales, value scales.  16-byte
+    // chunks of value rows 2, 3 (mod 4) are swapped so that a warp's reads spread over the banks.
+    static constexpr int kAhead = kStages - 1;
+    static constexpr int kTile = 16 * kSub, kRow = HD / 2, kScaleRow = 2 * kBlocks;
+    static constexpr int kOffV = kTile * kRow, kOffKs = 2 * kOffV, kOffVs = kOffKs + kTile * kScaleRow;
+    static constexpr int kStage = kOffVs + kTile * kScaleRow;
+    static constexpr int kRing = kStages * kStage;  // bytes of a warp
+    const char *k, *v, *ks, *vsp;  // the layer's planes
+    char *ring;
+    int stage;
+    __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, char *warp_ring, int)
+        : k(static_cast<const char *>(a.k)), v(static_cast<const char *>(a.v)),
+          ks(reinterpret_cast<const char *>(a.k_scale)), vsp(reinterpret_cast<const char *>(a.v_scale)), ring(warp_ring) {}
+    __device__ __forceinline__ static int swizzle(int row, int chunk) {  // byte of a 16-byte chunk of a value row
+        return row * kRow + 16 * (kRow == 64 ? chunk ^ (row & 2) : chunk);
+    }
+    // Requests tile rows; at_stage: stages from the one in use.
     template <class P>
-    __device__ __forceinline__ void load_k(int s, const P &p) {
+    __device__ __forceinline__ void request(int at_stage, const P (&p)[kSub], int lane) {
+        int st = stage + at_stage;
+        st = st >= kStages ? st - kStages : st;
+        char *dst = ring + st * kStage;
+        constexpr int kChunks = kRow / 16;  // of a row
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const char *src = kp + p.key(i) * (HD / 2) + 4 * HD * i;
-            if constexpr (HD == 128) {
-                const uint4 x = ldg_stream16(src);
-                kr[s][i][0] = x.x, kr[s][i][1] = x.y, kr[s][i][2] = x.z, kr[s][i][3] = x.w;
-            } else {
-                const uint2 x = ldg_stream8(src);
-                kr[s][i][0] = x.x, kr[s][i][1] = x.y;
+        for (int s = 0; s < kSub; ++s) {
+#pragma unroll
+            for (int i = 0; i < kChunks / 2; ++i) {
+                const int c = lane + 32 * i, row = c / kChunks;
+                const long long r = p[s].row(row) * kRow + c * 16;
+                cp_async16(dst + 16 * s * kRow + c * 16, k + r);
+                cp_async16(dst + kOffV + 16 * s * kRow + swizzle(row, c % kChunks), v + r);
             }
-            ks[s][i] = __ldg(ksp + p.key(i) * kBlocks + 8 * kBlocks * i);
+        }
+        // scales: a lane takes one position's of keys or of values
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) {
+            const int row = lane & 15;
+            const long long r = p[s].row(row) * kScaleRow + row * kScaleRow;
+            char *to = dst + (lane < 16 ? kOffKs : kOffVs) + (16 * s + row) * kScaleRow;
+            const char *from = (lane < 16 ? ks : vsp) + r;
+            if constexpr (kScaleRow == 8) cp_async8(to, from);
+            else cp_async4(to, from);
         }
     }
-    template <class P>
-    __device__ __forceinline__ void load_v(int s, const P &p) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const char *src = vp + p.value(i) * (HD / 2) + HD / 2 * value_pos(0, i);
-            if constexpr (HD == 128) {
-                const uint2 x = ldg_stream8(src);
-                vr[s][i][0] = x.x, vr[s][i][1] = x.y;
-            } else {
-                vr[s][i][0] = ldg_stream4(src);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) vs[s][i] = __ldg(vsp + p.key(i) * kBlocks + 8 * kBlocks * i);
+    __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    // The oldest requested tile has arrived, for all lanes.
+    __device__ __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        __syncwarp();
     }
+    __device__ __forceinline__ void next() { stage = stage + 1 == kStages ? 0 : stage + 1; }
     // Scales of positions that are left out must not meet their weight 0 as NaN (codes are always finite).
     __device__ __forceinline__ void clear_values(uint32_t there, int lane) {
 #pragma unroll
@@ -457,23 +488,46 @@ struct Q4Rows {
             for (int i = 0; i < 2; ++i)
                 if (!(there >> (16 * s + key_pos(lane, i)) & 1)) vs[s][i] = __ushort_as_half(0);
     }
+    __device__ __forceinline__ void load_v(int lane) {
+        const __half *src = reinterpret_cast<const __half *>(ring + stage * kStage + kOffVs) + (lane & 3) % kBlocks;
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) vs[s][i] = src[(16 * s + key_pos(lane, i)) * kBlocks];
+    }
     // A: codes n as subnormal halves, n 2^-24 (low nibbles) and 16 n 2^-24 (high
     // nibbles, whose q is divided by 16), so a code costs half a mask; the sums
     // start at -8 sum q, which makes them those of n - 8.  (Not done for the values: there the
     // offset would be summed over all positions and cost digits.)
-    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2], int lane) {
+        const char *base = ring + stage * kStage;
+        uint32_t kr[2][kKW];
+        __half sc16[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 16 * s + key_pos(lane, i);
+            const char *src = base + row * kRow + 4 * kKW * (lane & 3);
+            if constexpr (HD == 128) {
+                const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                kr[i][0] = x.x, kr[i][1] = x.y, kr[i][2] = x.z, kr[i][3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                kr[i][0] = x.x, kr[i][1] = x.y;
+            }
+            sc16[i] = *reinterpret_cast<const __half *>(base + kOffKs + row * kScaleRow + 2 * ((lane & 3) % kBlocks));
+        }
         float c[4], d[4];  // two shorter chains
         constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
-            const uint32_t x = kr[s][0][w], y = kr[s][1][w], x8 = x >> 8, y8 = y >> 8;
+            const uint32_t x = kr[0][w], y = kr[1][w], x8 = x >> 8, y8 = y >> 8;
             if (w == 0) mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[0][0], q[0][1], bias[0], bias[1]);
             else mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
             mma16816(d, w == 0, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
         }
         // lanes past the row's blocks hold zero sums
-        sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (__half2float(ks[s][0]) * 16777216.0f);
-        sc[0][1] = ((c[2] + d[2]) + (c[3] + d[3])) * (__half2float(ks[s][1]) * 16777216.0f);
+        sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (__half2float(sc16[0]) * 16777216.0f);
+        sc[0][1] = ((c[2] + d[2]) + (c[3] + d[3])) * (__half2float(sc16[1]) * 16777216.0f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 1);
@@ -481,7 +535,7 @@ struct Q4Rows {
             sc[0][i] *= inv;
         }
     }
-    __device__ __forceinline__ void reset() { vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
+    __device__ __forceinline__ void reset() { stage = 0, vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
     // Whether a value scale of part s passes the bound of what a weight may be multiplied by.
     __device__ __forceinline__ bool value_range(int s) {
         return fabsf(__half2float(vs[s][0])) > vlim || fabsf(__half2float(vs[s][1])) > vlim;
@@ -501,7 +555,21 @@ struct Q4Rows {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[0][j][i] *= f;
     }
-    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4], int lane) {
+        uint32_t vr[kSub][4][kVW];
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = 16 * s + value_pos(lane, i), byte = 4 * kVW * (lane >> 2);
+                const char *src = ring + stage * kStage + kOffV + swizzle(row, byte / 16) + byte % 16;
+                if constexpr (HD == 128) {
+                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    vr[s][i][0] = x.x, vr[s][i][1] = x.y;
+                } else {
+                    vr[s][i][0] = *reinterpret_cast<const uint32_t *>(src);
+                }
+            }
         uint32_t b[kSub][2];
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {  // w * scale / vlim <= 2^15; columns of no block are not used
@@ -605,7 +673,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     using Smem = PaSmem<HD, NH>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     Smem &S = *reinterpret_cast<Smem *>(smem_raw);
-    uint32_t *ends = reinterpret_cast<uint32_t *>(smem_raw + kFixedSmem<HD, NH>);  // of rows 0..r
+    char *ring = reinterpret_cast<char *>(smem_raw + kFixedSmem<HD, NH>);
+    uint32_t *ends = reinterpret_cast<uint32_t *>(ring + kPaWarps * R::kRing);  // of rows 0..r
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int group = a.group;        // query heads of a key head
     const uint32_t units = a.units.d;  // of a row: key heads x groups of NH query heads
@@ -674,7 +743,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
     }
 
-    R R_(a, lane);
+    R R_(a, ring + warp * R::kRing, lane);
     float *buf = S.buf[warp];
 #pragma unroll 1
     while (u < u_end) {
@@ -739,18 +808,25 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         R_.template load_q<ACT>(a.q, row * a.q_stride + static_cast<long long>(hd.head0) * HD, hd.heads, a.qscale, buf, lane);
         Pos16<kAligned> P[R::kSub];
         constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << kTile) - 1;
-        uint32_t there = 0;  // positions attended to of the tile whose keys are requested
-        // Step `tile` uses the keys requested in the step before, requests its
-        // own values and the next tile's keys; the first step only requests keys.
+        uint32_t there[R::kAhead] = {};  // positions attended to of the tiles requested
+        // Step `tile` uses the rows requested kAhead steps before and requests
+        // those of kAhead tiles later; the first kAhead steps only request.
 #pragma unroll 1
-        for (int tile = tile0 - 1; tile < tile1; ++tile) {
-            const uint32_t now = there;
+        for (int tile = tile0 - R::kAhead; tile < tile1; ++tile) {
+            const uint32_t now = there[0];
+#pragma unroll
+            for (int i = 0; i + 1 < R::kAhead; ++i) there[i] = there[i + 1];
             float sc[R::kSub][NB][2];
+            if (tile >= tile0) R_.wait();
             if (now) {
+                if constexpr (R::kRing == 0) {
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
+                    for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
+                } else {
+                    R_.load_v(lane);
+                }
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
+                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s], lane);
                 if (now != kAll) {
 #pragma unroll
                     for (int s = 0; s < R::kSub; ++s)
@@ -758,14 +834,15 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
-                                if (!(now >> (16 * s + 8 * i + g) & 1)) sc[s][nb][i] = -INFINITY;
+                                if (!(now >> (16 * s + key_pos(lane, i)) & 1)) sc[s][nb][i] = -INFINITY;
                 }
             }
-            if (tile + 1 < tile1) {
-                const int p0 = pbase + (tile + 1) * kTile;
-                there = kAll;
-                if (p0 < start) there &= kAll << (start - p0);
-                if (p0 + kTile > len) there &= kAll >> (p0 + kTile - len);
+            there[R::kAhead - 1] = 0;
+            if (tile + R::kAhead < tile1) {
+                const int p0 = pbase + (tile + R::kAhead) * kTile;
+                uint32_t mask = kAll;
+                if (p0 < start) mask &= kAll << (start - p0);
+                if (p0 + kTile > len) mask &= kAll >> (p0 + kTile - len);
                 // what is left out reads some row (row 0 in the place of an invalid page) and is masked later
                 if constexpr (kAligned) {
 #pragma unroll
@@ -775,12 +852,11 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
                         P[s].first = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + offset : 0;
                         if (!ok) {
-                            bad |= (there >> (16 * s) & 0xffff) != 0;
-                            there &= ~(0xffffu << (16 * s));
+                            bad |= (mask >> (16 * s) & 0xffff) != 0;
+                            mask &= ~(0xffffu << (16 * s));
                         }
                         offset += 16;
                         if (offset == a.page.d) offset = 0, ++block;
-                        R_.load_k(s, P[s]);
                     }
                 } else {
                     // lane i finds the row of the tile's position i (mod 16), the others get it from there
@@ -793,20 +869,24 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                     const bool ok = in && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
                     bad |= in && !ok;
                     const uint32_t r = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p : 0;
-                    there = __ballot_sync(0xffffffffu, ok) & kAll;
+                    mask = __ballot_sync(0xffffffffu, ok) & kAll;
 #pragma unroll
                     for (int s = 0; s < R::kSub; ++s) {
+                        P[s].mine = __shfl_sync(0xffffffffu, r, 16 * s + (lane & 15));
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            P[s].k[i] = static_cast<long long>(__shfl_sync(0xffffffffu, r, 16 * s + key_pos(lane, i))) - key_pos(lane, i);
+                        for (int i = 0; i < 2; ++i) P[s].k[i] = P[s].row(key_pos(lane, i));
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            P[s].v[i] = static_cast<long long>(__shfl_sync(0xffffffffu, r, 16 * s + value_pos(lane, i))) - value_pos(lane, i);
-                        R_.load_k(s, P[s]);
+                        for (int i = 0; i < 4; ++i) P[s].v[i] = P[s].row(value_pos(lane, i));
                     }
                 }
+                there[R::kAhead - 1] = mask;
+                R_.request(R::kAhead, P, lane);
             }
-            if (!now) continue;
+            R_.commit();
+            if (!now) {
+                R_.next();
+                continue;
+            }
             bool rise = false;
 #pragma unroll
             for (int s = 0; s < R::kSub; ++s)
@@ -844,7 +924,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                     l[nb] += sc[s][nb][0] + sc[s][nb][1];
                 }
             }
-            R_.values(sc, o);
+            R_.values(sc, o, lane);
+            R_.next();
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -1025,12 +1106,13 @@ cudaError_t pa_grid(int &grid) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices && (grid = known[dev].load(std::memory_order_acquire)) > 0) return cudaSuccess;
-    constexpr int smem = static_cast<int>(kFixedSmem<R::HD, R::kHeads> + 4 * kPagedMaxRows);
+    constexpr int smem = static_cast<int>(kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * kPagedMaxRows);
     e = cudaFuncSetAttribute(paged_attn_kernel<R, ACT, kAligned>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     int sms = 0, per_sm = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R, ACT, kAligned>, kPaThreads, smem)) !=
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_attn_kernel<R, ACT, kAligned>, kPaThreads,
+                                                           smem - 4 * kPagedMaxRows + 4 * 512)) !=
         cudaSuccess)
         return e;
     grid = sms * per_sm < kMaxGrid ? sms * per_sm : kMaxGrid;
@@ -1054,7 +1136,7 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     a.units = make_fast_div(a.n_kv_heads * chunks);
     a.cnt = static_cast<int *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
-    paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + 4 * a.n_rows, s>>>(a);
+    paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * a.n_rows, s>>>(a);
     return cudaGetLastError();
 }
 

@@ -196,7 +196,7 @@ typedef struct bmo_page_book {
 
 typedef struct bmo_paged_kv {
     bmo_page_book book;
-    void *k, *v;             /* device, 16-byte aligned */
+    void *k, *v;             /* device, 16-byte aligned (the scales too) */
     void *k_scale, *v_scale; /* kv_type 1 only */
     int32_t n_layers, n_kv_heads, head_dim, kv_type;
 } bmo_paged_kv;
