@@ -21,7 +21,7 @@ bool book_ok(const bmo_page_book &b) {
 
 bool table_ok(const bmo_page_book &b) {
     return b.table && b.lens && b.n_req > 0 && b.max_blocks > 0 &&
-           static_cast<long long>(b.max_blocks) * b.page_size <= INT_MAX;
+           static_cast<long long>(b.max_blocks) * b.page_size <= INT_MAX - 65535;  // room to step past the end
 }
 
 bool cache_ok(const bmo_paged_kv *c) {

@@ -80,6 +80,33 @@ __device__ __forceinline__ uint32_t ldg_stream4(const void *p) {
 }
 
 // c += A B, and c = A B + start.
+// Shared memory by 32-bit address.
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t p) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t lds4(uint32_t p) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_half(uint32_t p) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(p) : "memory");
+    return __half2float(__ushort_as_half(v));
+}
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void *src) {
+    if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -272,16 +299,11 @@ struct F16Rows {
     }
     // Rows go straight into registers: the next tile's keys are requested as
     // soon as a tile's scores are formed, its values at the start of its step.
-    static constexpr int kAhead = 1, kRing = 0;
+    static constexpr int kRing = 0;
     const char *kp, *vp;  // the lane's bytes of positions g and 2t, were they in rows g and 2t
     __device__ __forceinline__ F16Rows(const PagedAttnArgs &a, char *, int lane)
         : kp(static_cast<const char *>(a.k) + 2 * HD * (lane >> 2) + 16 * (lane & 3)),
           vp(static_cast<const char *>(a.v) + 4 * HD * (lane & 3) + 16 * (lane >> 2)) {}
-    template <class P>
-    __device__ __forceinline__ void request(int, const P (&p)[kSub], int) {
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) load_k(s, p[s]);
-    }
     template <class P>
     __device__ __forceinline__ void load_k(int s, const P &p) {
 #pragma unroll
@@ -308,7 +330,7 @@ struct F16Rows {
                     for (int c = 0; c < HD / 64; ++c) vr[s][i][c] = make_uint4(0, 0, 0, 0);
     }
     // sc[nb][i]: score (log2 units) of position g + 8 i for head (nb, t)
-    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2], int) {
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             float c[4], d[4];  // two shorter chains
@@ -322,15 +344,10 @@ struct F16Rows {
             sc[nb][1] = ((c[2] + d[2]) + (c[3] + d[3])) * inv[nb];
         }
     }
-    __device__ __forceinline__ void commit() {}
-    __device__ __forceinline__ void wait() {}
-    __device__ __forceinline__ void next() {}
-    __device__ __forceinline__ bool value_range(int) { return false; }
-    __device__ __forceinline__ void raise_value_range(float (&)[NB][kO][4]) {}
     __device__ __forceinline__ void reset() {}
     // Adds the weighted values of the tile.  The tensor core's sum of a tile
     // starts from zero and is added in fp32: its own running sum is not rounded to nearest.
-    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4], int) {
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
         uint32_t b[kSub][NB][2];
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
@@ -374,7 +391,6 @@ template <int HD_>
 struct Q4Rows {
     static constexpr int HD = HD_, NB = 1;
     static constexpr int kMinCtas = 3;
-    static constexpr int kStages = 3;
     static constexpr int kHeadCost = 2;
     static constexpr int kHeads = 1;
     static constexpr int kSub = 2;
@@ -385,7 +401,7 @@ struct Q4Rows {
     uint32_t q[HD / 16][2];
     float inv, bias[2];
     float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
-    __half vs[kSub][2];
+    float vs[kSub][2];
     // B fragments of the query: a lane splits 4 elements, elements 16..31 of a
     // block divided by 16, and puts them where the lanes that hold their codes
     // find their fragments as 16-byte words: buf[block][hi, lo][16] (pairs of halves).
@@ -427,94 +443,89 @@ struct Q4Rows {
             q[2 * w][0] = u.x, q[2 * w][1] = u.y, q[2 * w + 1][0] = u.z, q[2 * w + 1][1] = u.w;
         }
     }
-    // Rows reach shared memory by asynchronous copies, kAhead tiles ahead (the
+    // Rows reach shared memory by asynchronous copies, two tiles ahead (the
     // arithmetic on codes leaves no registers to hold that much): a stage is
     // the tile's key codes, value codes, key scales, value scales.  16-byte
     // chunks of value rows 2, 3 (mod 4) are swapped so that a warp's reads spread over the banks.
-    static constexpr int kAhead = kStages - 1;
     static constexpr int kTile = 16 * kSub, kRow = HD / 2, kScaleRow = 2 * kBlocks;
     static constexpr int kOffV = kTile * kRow, kOffKs = 2 * kOffV, kOffVs = kOffKs + kTile * kScaleRow;
     static constexpr int kStage = kOffVs + kTile * kScaleRow;
-    static constexpr int kRing = kStages * kStage;  // bytes of a warp
-    const char *k, *v, *ks, *vsp;  // the layer's planes
-    char *ring;
-    int stage;
-    __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, char *warp_ring, int)
-        : k(static_cast<const char *>(a.k)), v(static_cast<const char *>(a.v)),
-          ks(reinterpret_cast<const char *>(a.k_scale)), vsp(reinterpret_cast<const char *>(a.v_scale)), ring(warp_ring) {}
-    __device__ __forceinline__ static int swizzle(int row, int chunk) {  // byte of a 16-byte chunk of a value row
-        return row * kRow + 16 * (kRow == 64 ? chunk ^ (row & 2) : chunk);
+    static constexpr int kRing = 3 * kStage;  // bytes of a warp
+    const char *kp, *vp, *sp;       // the lane's bytes of rows 0..15: codes of keys and values, scales of either
+    uint32_t ring, to_k, to_v, to_s;  // where they go in a stage
+    uint32_t at_k, at_ks, at_v, at_vs;  // what the lane reads of a stage
+    uint32_t stage;  // that of the tile whose values are added; the next one's is kStage further
+    __device__ __forceinline__ Q4Rows(const PagedAttnArgs &a, char *warp_ring, int lane) : ring(smem_addr(warp_ring)) {
+        constexpr int kChunks = kRow / 16;  // of a row: a lane copies chunks lane, lane + 32, .. of 16 rows
+        const int g = lane >> 2, t = lane & 3, row = lane / kChunks;
+        kp = static_cast<const char *>(a.k) + 16 * lane;
+        vp = static_cast<const char *>(a.v) + 16 * lane;
+        sp = static_cast<const char *>(lane < 16 ? static_cast<const void *>(a.k_scale) : a.v_scale) + (lane & 15) * kScaleRow;
+        to_k = 16 * lane;
+        to_v = kOffV + swizzle(row, lane % kChunks);
+        to_s = (lane < 16 ? kOffKs : kOffVs) + (lane & 15) * kScaleRow;
+        at_k = g * kRow + 4 * kKW * t;
+        at_ks = kOffKs + g * kScaleRow + 2 * (t % kBlocks);
+        at_v = kOffV + swizzle(2 * t, 4 * kVW * g / 16) + 4 * kVW * g % 16;
+        at_vs = kOffVs + g * kScaleRow + 2 * (t % kBlocks);
     }
-    // Requests tile rows; at_stage: stages from the one in use.
+    // Byte of a 16-byte chunk of a value row; rows 1 and 8 on have the same swizzle.
+    __device__ __forceinline__ static int swizzle(int row, int chunk) { return row * kRow + 16 * (kRow == 64 ? chunk ^ (row & 2) : chunk); }
+    // Requests a tile, into the stage two after the one in use.
     template <class P>
-    __device__ __forceinline__ void request(int at_stage, const P (&p)[kSub], int lane) {
-        int st = stage + at_stage;
-        st = st >= kStages ? st - kStages : st;
-        char *dst = ring + st * kStage;
-        constexpr int kChunks = kRow / 16;  // of a row
+    __device__ __forceinline__ void request(const P (&p)[kSub], int lane) {
+        const uint32_t dst = stage == ring ? ring + 2 * kStage : stage - kStage;
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {
 #pragma unroll
-            for (int i = 0; i < kChunks / 2; ++i) {
-                const int c = lane + 32 * i, row = c / kChunks;
-                const long long r = p[s].row(row) * kRow + c * 16;
-                cp_async16(dst + 16 * s * kRow + c * 16, k + r);
-                cp_async16(dst + kOffV + 16 * s * kRow + swizzle(row, c % kChunks), v + r);
+            for (int i = 0; i < kRow / 32; ++i) {  // 512 bytes of the 16 rows each
+                const long long r = p[s].row((lane + 32 * i) / (kRow / 16)) * kRow + 512 * i;
+                copy_async<16>(dst + to_k + 16 * s * kRow + 512 * i, kp + r);
+                copy_async<16>(dst + to_v + 16 * s * kRow + 512 * i, vp + r);
             }
-        }
-        // scales: a lane takes one position's of keys or of values
-#pragma unroll
-        for (int s = 0; s < kSub; ++s) {
-            const int row = lane & 15;
-            const long long r = p[s].row(row) * kScaleRow + row * kScaleRow;
-            char *to = dst + (lane < 16 ? kOffKs : kOffVs) + (16 * s + row) * kScaleRow;
-            const char *from = (lane < 16 ? ks : vsp) + r;
-            if constexpr (kScaleRow == 8) cp_async8(to, from);
-            else cp_async4(to, from);
+            copy_async<kScaleRow>(dst + to_s + 16 * s * kScaleRow, sp + p[s].row(lane & 15) * kScaleRow);
         }
     }
     __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-    // The oldest requested tile has arrived, for all lanes.
+    // All requests but the last have arrived, for all lanes.
     __device__ __forceinline__ void wait() {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
     }
-    __device__ __forceinline__ void next() { stage = stage + 1 == kStages ? 0 : stage + 1; }
-    // Scales of positions that are left out must not meet their weight 0 as NaN (codes are always finite).
-    __device__ __forceinline__ void clear_values(uint32_t there, int lane) {
+    __device__ __forceinline__ void next() { stage = stage == ring + 2 * kStage ? ring : stage + kStage; }
+    // The value scales of the tile in use; those of positions that are left out
+    // must not meet their weight 0 as NaN (codes are always finite).
+    __device__ __forceinline__ void load_scales(uint32_t there, int lane) {
+#pragma unroll
+        for (int s = 0; s < kSub; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) vs[s][i] = lds_half(stage + at_vs + (16 * s + 8 * i) * kScaleRow);
+        if (there == (kTile == 32 ? 0xffffffffu : 0xffffu)) return;
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (!(there >> (16 * s + key_pos(lane, i)) & 1)) vs[s][i] = __ushort_as_half(0);
-    }
-    __device__ __forceinline__ void load_v(int lane) {
-        const __half *src = reinterpret_cast<const __half *>(ring + stage * kStage + kOffVs) + (lane & 3) % kBlocks;
-#pragma unroll
-        for (int s = 0; s < kSub; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) vs[s][i] = src[(16 * s + key_pos(lane, i)) * kBlocks];
+                if (!(there >> (16 * s + key_pos(lane, i)) & 1)) vs[s][i] = 0.0f;
     }
     // A: codes n as subnormal halves, n 2^-24 (low nibbles) and 16 n 2^-24 (high
     // nibbles, whose q is divided by 16), so a code costs half a mask; the sums
     // start at -8 sum q, which makes them those of n - 8.  (Not done for the values: there the
     // offset would be summed over all positions and cost digits.)
-    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2], int lane) {
-        const char *base = ring + stage * kStage;
+    __device__ __forceinline__ void scores(int s, float (&sc)[NB][2]) {
+        const uint32_t base = stage == ring + 2 * kStage ? ring : stage + kStage;  // of the next tile
         uint32_t kr[2][kKW];
-        __half sc16[2];
+        float ks[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int row = 16 * s + key_pos(lane, i);
-            const char *src = base + row * kRow + 4 * kKW * (lane & 3);
+            const uint32_t src = base + at_k + (16 * s + 8 * i) * kRow;
             if constexpr (HD == 128) {
-                const uint4 x = *reinterpret_cast<const uint4 *>(src);
+                const uint4 x = lds16(src);
                 kr[i][0] = x.x, kr[i][1] = x.y, kr[i][2] = x.z, kr[i][3] = x.w;
             } else {
-                const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                const uint2 x = lds8(src);
                 kr[i][0] = x.x, kr[i][1] = x.y;
             }
-            sc16[i] = *reinterpret_cast<const __half *>(base + kOffKs + row * kScaleRow + 2 * ((lane & 3) % kBlocks));
+            ks[i] = lds_half(base + at_ks + (16 * s + 8 * i) * kScaleRow);
         }
         float c[4], d[4];  // two shorter chains
         constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
@@ -526,8 +537,8 @@ struct Q4Rows {
             mma16816(d, w == 0, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
         }
         // lanes past the row's blocks hold zero sums
-        sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (__half2float(sc16[0]) * 16777216.0f);
-        sc[0][1] = ((c[2] + d[2]) + (c[3] + d[3])) * (__half2float(sc16[1]) * 16777216.0f);
+        sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (ks[0] * 16777216.0f);
+        sc[0][1] = ((c[2] + d[2]) + (c[3] + d[3])) * (ks[1] * 16777216.0f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 1);
@@ -535,17 +546,18 @@ struct Q4Rows {
             sc[0][i] *= inv;
         }
     }
-    __device__ __forceinline__ void reset() { stage = 0, vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
+    __device__ __forceinline__ void reset() { stage = ring, vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
     // Whether a value scale of part s passes the bound of what a weight may be multiplied by.
     __device__ __forceinline__ bool value_range(int s) {
-        return fabsf(__half2float(vs[s][0])) > vlim || fabsf(__half2float(vs[s][1])) > vlim;
+        return fmaxf(fabsf(vs[s][0]), fabsf(vs[s][1])) > vlim;
     }
     __device__ __forceinline__ void raise_value_range(float (&o)[NB][kO][4]) {
         float m = vlim;
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
-            m = fmaxf(m, fmaxf(fabsf(__half2float(vs[s][0])), fabsf(__half2float(vs[s][1]))));
+            m = fmaxf(m, fmaxf(fabsf(vs[s][0]), fabsf(vs[s][1])));
         m = warp_max(m);
+        if (!(m > vlim)) return;
         const int ex = min(((__float_as_int(m) >> 23) & 255) + 2, 127 + 18);  // a power of two above 2 m
         const float lim = __int_as_float(ex << 23);
         const float f = vlim * __int_as_float((254 - ex) << 23);
@@ -555,25 +567,24 @@ struct Q4Rows {
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[0][j][i] *= f;
     }
-    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4], int lane) {
+    __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
         uint32_t vr[kSub][4][kVW];
 #pragma unroll
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = 16 * s + value_pos(lane, i), byte = 4 * kVW * (lane >> 2);
-                const char *src = ring + stage * kStage + kOffV + swizzle(row, byte / 16) + byte % 16;
+                const uint32_t src = stage + at_v + (16 * s + value_pos(0, i)) * kRow;
                 if constexpr (HD == 128) {
-                    const uint2 x = *reinterpret_cast<const uint2 *>(src);
+                    const uint2 x = lds8(src);
                     vr[s][i][0] = x.x, vr[s][i][1] = x.y;
                 } else {
-                    vr[s][i][0] = *reinterpret_cast<const uint32_t *>(src);
+                    vr[s][i][0] = lds4(src);
                 }
             }
         uint32_t b[kSub][2];
 #pragma unroll
         for (int s = 0; s < kSub; ++s) {  // w * scale / vlim <= 2^15; columns of no block are not used
-            split_half2(w[s][0][0] * (__half2float(vs[s][0]) * vinv), w[s][0][1] * (__half2float(vs[s][1]) * vinv), b[s][0], b[s][1]);
+            split_half2(w[s][0][0] * (vs[s][0] * vinv), w[s][0][1] * (vs[s][1] * vinv), b[s][0], b[s][1]);
             b[s][0] = transpose8(b[s][0]);
             b[s][1] = transpose8(b[s][1]);
         }
@@ -783,17 +794,26 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const int start = a.window > 0 ? max(0, len - a.window) : 0;
         const int pbase = start / kTile * kTile;
 
-        // entries [b0, b0 + 32) of the row of the block table, one a lane
+        constexpr uint32_t kNoPage = 0xffffffffu;  // an entry that is not a page of the cache
         const int *table = a.table + static_cast<long long>(req) * a.max_blocks;
-        const int from_pos = kAligned ? pbase + tile0 * kTile : max(start, pbase + tile0 * kTile);
-        int block = pa_div(from_pos, a.page);         // of the next 16 positions
-        uint32_t offset = from_pos - block * a.page.d;  // of these in their page
-        int b0, entry;
-        auto refill = [&] {
-            b0 = block;
-            entry = b0 + lane < a.max_blocks ? table[b0 + lane] : -1;
+        auto first_row = [&](int b) {  // of block b
+            const uint32_t page = static_cast<uint32_t>(b) < static_cast<uint32_t>(a.max_blocks) ? table[b] : -1;
+            return page < static_cast<uint32_t>(a.n_pages) ? (page * a.n_kv_heads + kh) * a.page.d : kNoPage;
         };
-        refill();
+        // Ring, aligned: rows of position `walk` + 16 i, in lane i; else of blocks walk + i.
+        int walk;
+        uint32_t entry;
+        auto refill = [&](int at) {
+            walk = at;
+            if constexpr (kAligned) {
+                const int p = at + 16 * lane, b = pa_div(p, a.page);
+                const uint32_t r = first_row(b);
+                entry = r == kNoPage ? r : r + (p - b * a.page.d);
+            } else {
+                entry = first_row(at + lane);
+            }
+        };
+        if (R::kRing > 0 || !kAligned) refill(kAligned ? pbase + tile0 * kTile : pa_div(max(start, pbase + tile0 * kTile), a.page));
         float o[NB][kO][4], m[NB], l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -808,25 +828,128 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         R_.template load_q<ACT>(a.q, row * a.q_stride + static_cast<long long>(hd.head0) * HD, hd.heads, a.qscale, buf, lane);
         Pos16<kAligned> P[R::kSub];
         constexpr uint32_t kAll = kTile == 32 ? 0xffffffffu : (1u << kTile) - 1;
-        uint32_t there[R::kAhead] = {};  // positions attended to of the tiles requested
+        // Rows of the next tile, and which of its positions are attended to.
+        // What is left out reads some row (row 0 in the place of an invalid page) and is masked later.
+        auto locate = [&](int tile) {
+            const int p0 = pbase + tile * kTile;
+            uint32_t mask = kAll;
+            if (p0 < start || p0 + kTile > len) {
+                if (p0 < start) mask &= kAll << (start - p0);
+                if (p0 + kTile > len) mask &= kAll >> (p0 + kTile - len);
+            }
+            if constexpr (kAligned) {
+                if (p0 >= walk + 16 * 32) refill(p0);
+                uint32_t top = 0;
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) {
+                    P[s].first = __shfl_sync(0xffffffffu, entry, (p0 - walk) / 16 + s);
+                    top = max(top, P[s].first);
+                }
+                if (top == kNoPage) {
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) {
+                        if (P[s].first != kNoPage) continue;
+                        P[s].first = 0;
+                        bad |= (mask >> (16 * s) & 0xffff) != 0;
+                        mask &= ~(0xffffu << (16 * s));
+                    }
+                }
+            } else {
+                // lane i finds the row of the tile's position i (mod 16), the others get it from there
+                const int p = p0 + (lane & (kTile - 1));
+                const bool in = p >= start && p < len;
+                const int b = pa_div(p, a.page);
+                if (static_cast<int>(pa_div(min(p0 + kTile, len) - 1, a.page)) >= walk + 32) refill(pa_div(max(p0, start), a.page));
+                const uint32_t base = __shfl_sync(0xffffffffu, entry, in ? b - walk : 0);
+                const bool ok = in && base != kNoPage;
+                bad |= in && !ok;
+                const uint32_t r = ok ? base + (p - b * a.page.d) : 0;
+                mask = __ballot_sync(0xffffffffu, ok) & kAll;
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) {
+                    P[s].mine = __shfl_sync(0xffffffffu, r, 16 * s + (lane & 15));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) P[s].k[i] = P[s].row(key_pos(lane, i));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) P[s].v[i] = P[s].row(value_pos(lane, i));
+                }
+            }
+            return mask;
+        };
+        float sc[R::kSub][NB][2] = {};  // scores, then weights
+        auto mask_scores = [&](uint32_t mask) {
+            if (mask == kAll) return;
+#pragma unroll
+            for (int s = 0; s < R::kSub; ++s)
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (!(mask >> (16 * s + key_pos(lane, i)) & 1)) sc[s][nb][i] = -INFINITY;
+        };
+        // Scores to weights; raises the maximum, and with it rescales the sums, where a score passes it by too much.
+        auto weigh = [&] {
+            bool rise = false;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float top = fmaxf(sc[0][nb][0], sc[0][nb][1]);
+#pragma unroll
+                for (int s = 1; s < R::kSub; ++s) top = fmaxf(top, fmaxf(sc[s][nb][0], sc[s][nb][1]));
+                rise |= top > m[nb] + kSlack;
+            }
+            if constexpr (R::kRing > 0) {
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) rise |= R_.value_range(s);
+            }
+            if (__any_sync(0xffffffffu, rise)) {
+                if constexpr (R::kRing > 0) R_.raise_value_range(o);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float x = m[nb];
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) x = fmaxf(x, fmaxf(sc[s][nb][0], sc[s][nb][1]));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float f = x == -INFINITY ? 1.0f : ex2(m[nb] - x);
+                    m[nb] = x;
+                    l[nb] *= f;
+#pragma unroll
+                    for (int j = 0; j < kO; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[nb][j][i] *= f;
+                }
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) {
+                    sc[s][nb][0] = ex2(sc[s][nb][0] - ref);
+                    sc[s][nb][1] = ex2(sc[s][nb][1] - ref);
+                    l[nb] += sc[s][nb][0] + sc[s][nb][1];
+                }
+            }
+        };
+        uint32_t there = 0;  // positions attended to of the tile requested last
+        if constexpr (R::kRing == 0) {
+            // Entries [b0, b0 + 32) of the block table, one a lane, and the next tile's
+            // block and place in it.  (Rows found as for the other loop measured 270 us against 259.)
+            int block = pa_div(pbase + tile0 * kTile, a.page), b0 = block;
+            uint32_t offset = pbase + tile0 * kTile - block * a.page.d;
+            auto entries = [&] { return b0 + lane < a.max_blocks ? table[b0 + lane] : -1; };
+            int entry = kAligned ? entries() : 0;
+        uint32_t there[1] = {};  // positions attended to of the tiles requested
         // Step `tile` uses the rows requested kAhead steps before and requests
         // those of kAhead tiles later; the first kAhead steps only request.
 #pragma unroll 1
-        for (int tile = tile0 - R::kAhead; tile < tile1; ++tile) {
+        for (int tile = tile0 - 1; tile < tile1; ++tile) {
             const uint32_t now = there[0];
-#pragma unroll
-            for (int i = 0; i + 1 < R::kAhead; ++i) there[i] = there[i + 1];
             float sc[R::kSub][NB][2];
-            if (tile >= tile0) R_.wait();
             if (now) {
-                if constexpr (R::kRing == 0) {
 #pragma unroll
-                    for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
-                } else {
-                    R_.load_v(lane);
-                }
+                for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s], lane);
+                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
                 if (now != kAll) {
 #pragma unroll
                     for (int s = 0; s < R::kSub; ++s)
@@ -837,17 +960,17 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                                 if (!(now >> (16 * s + key_pos(lane, i)) & 1)) sc[s][nb][i] = -INFINITY;
                 }
             }
-            there[R::kAhead - 1] = 0;
-            if (tile + R::kAhead < tile1) {
-                const int p0 = pbase + (tile + R::kAhead) * kTile;
-                uint32_t mask = kAll;
-                if (p0 < start) mask &= kAll << (start - p0);
-                if (p0 + kTile > len) mask &= kAll >> (p0 + kTile - len);
-                // what is left out reads some row (row 0 in the place of an invalid page) and is masked later
+            there[0] = 0;
+            if (tile + 1 < tile1) {
+                uint32_t mask;
                 if constexpr (kAligned) {
+                    const int p0 = pbase + (tile + 1) * kTile;
+                    mask = kAll;
+                    if (p0 < start) mask &= kAll << (start - p0);
+                    if (p0 + kTile > len) mask &= kAll >> (p0 + kTile - len);
 #pragma unroll
                     for (int s = 0; s < R::kSub; ++s) {
-                        if (block >= b0 + 32) refill();
+                        if (block >= b0 + 32) b0 = block, entry = entries();
                         const int page = __shfl_sync(0xffffffffu, entry, block - b0);
                         const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
                         P[s].first = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + offset : 0;
@@ -859,32 +982,13 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         if (offset == a.page.d) offset = 0, ++block;
                     }
                 } else {
-                    // lane i finds the row of the tile's position i (mod 16), the others get it from there
-                    const int p = p0 + (lane & (kTile - 1));
-                    const bool in = p >= start && p < len;
-                    const int b = pa_div(p, a.page);
-                    block = pa_div(max(p0, start), a.page);
-                    if (static_cast<int>(pa_div(min(p0 + kTile, len) - 1, a.page)) >= b0 + 32) refill();
-                    const int page = __shfl_sync(0xffffffffu, entry, in ? b - b0 : 0);
-                    const bool ok = in && static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
-                    bad |= in && !ok;
-                    const uint32_t r = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh - b) * a.page.d + p : 0;
-                    mask = __ballot_sync(0xffffffffu, ok) & kAll;
-#pragma unroll
-                    for (int s = 0; s < R::kSub; ++s) {
-                        P[s].mine = __shfl_sync(0xffffffffu, r, 16 * s + (lane & 15));
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) P[s].k[i] = P[s].row(key_pos(lane, i));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) P[s].v[i] = P[s].row(value_pos(lane, i));
-                    }
+                    mask = locate(tile + 1);
                 }
-                there[R::kAhead - 1] = mask;
-                R_.request(R::kAhead, P, lane);
+                there[0] = mask;
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) R_.load_k(s, P[s]);
             }
-            R_.commit();
             if (!now) {
-                R_.next();
                 continue;
             }
             bool rise = false;
@@ -910,10 +1014,6 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 }
             }
             if (now != kAll) R_.clear_values(now, lane);
-            bool wide = false;
-#pragma unroll
-            for (int s = 0; s < R::kSub; ++s) wide |= R_.value_range(s);
-            if (__any_sync(0xffffffffu, wide)) R_.raise_value_range(o);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
@@ -924,8 +1024,37 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                     l[nb] += sc[s][nb][0] + sc[s][nb][1];
                 }
             }
-            R_.values(sc, o, lane);
-            R_.next();
+            R_.values(sc, o);
+        }
+        } else {
+            // Step `tile` requests the rows of two tiles later, forms the next
+            // tile's scores and adds its own values: two independent streams of arithmetic.
+#pragma unroll 1
+            for (int tile = tile0 - 2; tile < tile1; ++tile) {
+                const uint32_t next = there;
+                __syncwarp();  // the stage that is filled now was read in the last step
+                if (tile + 2 < tile1) {
+                    there = locate(tile + 2);
+                    R_.request(P, lane);
+                }
+                R_.commit();
+                const bool more = tile + 1 >= tile0 && tile + 1 < tile1;
+                float w[R::kSub][NB][2];
+#pragma unroll
+                for (int s = 0; s < R::kSub; ++s) w[s][0][0] = sc[s][0][0], w[s][0][1] = sc[s][0][1];
+                R_.wait();
+                if (more) {
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
+                }
+                if (tile >= tile0) R_.values(w, o);
+                R_.next();
+                if (more) {
+                    mask_scores(next);
+                    R_.load_scales(next, lane);
+                    weigh();
+                }
+            }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
