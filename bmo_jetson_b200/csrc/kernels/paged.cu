@@ -8,6 +8,7 @@
 #include <cuda_bf16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "../paged.h"
 #include "common.cuh"
@@ -248,88 +249,93 @@ __global__ void plan_list_kernel(PagedPlanArgs a) {
 }
 
 // ---- activations of the three types, 4 elements at a time ----
+//
+// Raw: the 4 elements as loaded, so that many loads can be requested before
+// the first is converted.  kVec: rows start on 4 elements' alignment.
 
-template <int ACT>
-struct Act;
-template <>
-struct Act<BMO_ACT_F32> {
+struct Act32 {
     using T = float;
-    static __device__ __forceinline__ float4 load4(const T *p, bool vec) {
-        return vec ? __ldcs(reinterpret_cast<const float4 *>(p)) : make_float4(p[0], p[1], p[2], p[3]);
+    using Raw = float4;
+    template <bool kVec>
+    static __device__ __forceinline__ Raw load(const T *p) {
+        if constexpr (kVec) return __ldcs(reinterpret_cast<const float4 *>(p));
+        else return make_float4(p[0], p[1], p[2], p[3]);
     }
-    static __device__ __forceinline__ void store4(T *p, float4 x, bool vec) {
-        if (vec) {
-            *reinterpret_cast<float4 *>(p) = x;
-        } else {
-            p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
-        }
+    static __device__ __forceinline__ float4 value(Raw r) { return r; }
+    template <bool kVec>
+    static __device__ __forceinline__ void store(T *p, float4 x) {
+        if constexpr (kVec) *reinterpret_cast<float4 *>(p) = x;
+        else p[0] = x.x, p[1] = x.y, p[2] = x.z, p[3] = x.w;
     }
 };
+template <class Half>
+struct IsBf16 {
+    static constexpr bool value = false;
+};
 template <>
-struct Act<BMO_ACT_F16> {
-    using T = __half;
-    static __device__ __forceinline__ float4 load4(const T *p, bool vec) {
-        __half2 a, b;
-        if (vec) {
-            const uint2 u = __ldcs(reinterpret_cast<const uint2 *>(p));
-            a = *reinterpret_cast<const __half2 *>(&u.x), b = *reinterpret_cast<const __half2 *>(&u.y);
-        } else {
-            a = __halves2half2(p[0], p[1]), b = __halves2half2(p[2], p[3]);
-        }
-        const float2 x = __half22float2(a), y = __half22float2(b);
+struct IsBf16<__nv_bfloat16> {
+    static constexpr bool value = true;
+};
+template <class Half>
+struct Act16 {
+    using T = Half;
+    using Raw = uint2;
+    template <bool kVec>
+    static __device__ __forceinline__ Raw load(const T *p) {
+        if constexpr (kVec) return __ldcs(reinterpret_cast<const uint2 *>(p));
+        const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
+        return make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+    }
+    static __device__ __forceinline__ float4 value(Raw r) {
+        if constexpr (IsBf16<T>::value)
+            return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                               __uint_as_float(r.y & 0xffff0000u));
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&r.x)),
+                     y = __half22float2(*reinterpret_cast<const __half2 *>(&r.y));
         return make_float4(x.x, x.y, y.x, y.y);
     }
-    static __device__ __forceinline__ void store4(T *p, float4 x, bool vec) {
-        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
-        if (vec) {
-            *reinterpret_cast<uint2 *>(p) =
-                make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    template <bool kVec>
+    static __device__ __forceinline__ void store(T *p, float4 x) {
+        Raw r;
+        if constexpr (IsBf16<T>::value) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+            r = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
         } else {
-            p[0] = __low2half(a), p[1] = __high2half(a), p[2] = __low2half(b), p[3] = __high2half(b);
+            const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+            r = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
         }
+        uint16_t *h = reinterpret_cast<uint16_t *>(p);
+        if constexpr (kVec) *reinterpret_cast<uint2 *>(p) = r;
+        else h[0] = r.x & 0xffff, h[1] = r.x >> 16, h[2] = r.y & 0xffff, h[3] = r.y >> 16;
     }
+};
+template <int ACT>
+struct ActOf {
+    using type = Act32;
 };
 template <>
-struct Act<BMO_ACT_BF16> {
-    using T = __nv_bfloat16;
-    static __device__ __forceinline__ float4 load4(const T *p, bool vec) {
-        uint2 u;
-        if (vec) {
-            u = __ldcs(reinterpret_cast<const uint2 *>(p));
-        } else {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(p);
-            u = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
-        }
-        return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
-                           __uint_as_float(u.y & 0xffff0000u));
-    }
-    static __device__ __forceinline__ void store4(T *p, float4 x, bool vec) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
-        if (vec) {
-            *reinterpret_cast<uint2 *>(p) =
-                make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
-        } else {
-            p[0] = __low2bfloat16(a), p[1] = __high2bfloat16(a), p[2] = __low2bfloat16(b), p[3] = __high2bfloat16(b);
-        }
-    }
+struct ActOf<BMO_ACT_F16> {
+    using type = Act16<__half>;
 };
-
-template <typename T>
-__device__ __forceinline__ bool can_vec4(const T *p, long long stride) {
-    return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && stride % 4 == 0;
-}
+template <>
+struct ActOf<BMO_ACT_BF16> {
+    using type = Act16<__nv_bfloat16>;
+};
+template <int ACT>
+using Act = typename ActOf<ACT>::type;
 
 // ---- append ----
 //
 // Bound by its bytes when there are many rows, by latency for a frame of one
-// position a session.  One thread holds 4 elements of a row, so a row of 128
-// is one warp's 512 (fp32) contiguous bytes and a rotated pair stays in one
-// thread.  A CTA takes kAppendRows rows of one token, all loads requested
-// before the angles are computed: cos and sin in double (rounded to fp32, as
-// the exact-order step's table) cost about as long as the loads take, and
-// are shared by the CTA's rows.
-constexpr int kAppendThreads = 256;
-constexpr int kAppendIter = 4;
+// position a session.  A lane holds 4 elements of a row, two rotated pairs, and
+// the same 4 of every row it meets, so a warp that takes rows of one
+// token needs each of the token's angles once, two a lane, in registers: cos
+// and sin in double, rounded to fp32 as the exact-order step's table.  The rows' loads are
+// requested kAppendRows at a time, the first ones before the angles are computed.
+// Warps take few rows each when there are few tokens (launch_paged_append), all of
+// a token's when there are many.
+constexpr int kAppendThreads = 128;
+constexpr int kAppendRows = 8;  // row slots of a lane in flight
 
 // One Q4_0 block per 8 lanes, 4 consecutive values each: the same codes and
 // scale as warp_store_q4_0.
@@ -361,72 +367,82 @@ __device__ __forceinline__ void group_store_q4_0(float4 x, uint8_t *qs_dst, __ha
     if (live && l == 0) *d_dst = __float2half_rn(d);
 }
 
-template <int HD, bool Q4, int ACT>
+template <int HD, bool Q4, int ACT, bool kVec>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ PagedAppendArgs a) {
     using A = Act<ACT>;
     using T = typename A::T;
-    constexpr int kLanes = HD / 4, kRows = kAppendThreads / kLanes;
-    __shared__ float2 cs[HD / 2];
-    const int tid = threadIdx.x, token = blockIdx.x;
-    const int d = tid % kLanes * 4;
-    const int row0 = blockIdx.y * (kRows * kAppendIter) + tid / kLanes;
+    constexpr int kLanes = HD / 4, kWide = 32 / kLanes;  // lanes of a row, rows of a warp's access
+    const int lane = threadIdx.x & 31;
+    const long long item = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+    const int token = static_cast<int>(item / a.parts), part = static_cast<int>(item - static_cast<long long>(token) * a.parts);
+    if (token >= a.n) return;
+    const int d = lane % kLanes * 4;
     const int n_rows = a.n_heads + 2 * a.n_kv_heads;
-    const T *q = static_cast<const T *>(a.q) + token * a.q_stride;
-    const T *k = static_cast<const T *>(a.k) + token * a.k_stride;
-    const T *v = static_cast<const T *>(a.v) + token * a.v_stride;
-    T *qo = static_cast<T *>(a.q_out) + token * a.q_out_stride;
+    const int end = min(n_rows, (part + 1) * a.part_rows);
+    const T *q = static_cast<const T *>(a.q) + token * a.q_stride + d;
+    const T *k = static_cast<const T *>(a.k) + token * a.k_stride + d;
+    const T *v = static_cast<const T *>(a.v) + token * a.v_stride + d;
+    T *qo = static_cast<T *>(a.q_out) + token * a.q_out_stride + d;
 
-    float4 x[kAppendIter];
+    int row0 = part * a.part_rows + lane / kLanes;
+    typename A::Raw raw[kAppendRows];
+    auto load = [&] {
 #pragma unroll
-    for (int i = 0; i < kAppendIter; ++i) {
-        const int row = row0 + i * kRows;
-        x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (row >= n_rows) continue;
-        if (row < a.n_heads) x[i] = A::load4(q + row * HD + d, can_vec4(q, 0));
-        else if (row < a.n_heads + a.n_kv_heads) x[i] = A::load4(k + (row - a.n_heads) * HD + d, can_vec4(k, 0));
-        else x[i] = A::load4(v + (row - a.n_heads - a.n_kv_heads) * HD + d, can_vec4(v, 0));
-    }
-    const int slot = a.slot[token];
-    if (a.rotate) {
-        if (tid < HD / 2) {
-            const float angle = __fmul_rn(static_cast<float>(a.pos[token]), a.inv_freq[tid]);
-            double sn, cn;
-            sincos(static_cast<double>(angle), &sn, &cn);
-            cs[tid] = make_float2(__double2float_rn(cn), __double2float_rn(sn));
+        for (int i = 0; i < kAppendRows; ++i) {
+            const int row = min(row0 + i * kWide, end - 1);
+            const T *src = row < a.n_heads ? q + row * HD
+                                           : row < a.n_heads + a.n_kv_heads ? k + (row - a.n_heads) * HD
+                                                                            : v + (row - a.n_heads - a.n_kv_heads) * HD;
+            raw[i] = A::template load<kVec>(src);
         }
-        __syncthreads();
+    };
+    load();
+    const int slot = a.slot[token];
+    float2 c0 = make_float2(1.0f, 0.0f), c1 = c0;
+    if (a.rotate) {
+        const float pos = static_cast<float>(a.pos[token]);
+        double sn, cn;
+        sincos(static_cast<double>(__fmul_rn(pos, a.inv_freq[d / 2])), &sn, &cn);
+        c0 = make_float2(__double2float_rn(cn), __double2float_rn(sn));
+        sincos(static_cast<double>(__fmul_rn(pos, a.inv_freq[d / 2 + 1])), &sn, &cn);
+        c1 = make_float2(__double2float_rn(cn), __double2float_rn(sn));
     }
     const bool stored = slot >= 0 && slot < a.n_slots;
-    if (tid == 0 && !stored && slot != -1) raise_error(a.status, kErrBadIndex);
+    if (part == 0 && lane == 0 && !stored && slot != -1) raise_error(a.status, kErrBadIndex);
     const uint32_t page = stored ? fast_div(slot, a.page) : 0;
     const uint32_t at = stored ? slot - page * a.page.d : 0;
+    const long long row_of_page = static_cast<long long>(page) * a.n_kv_heads * a.page.d + at;
+    for (;;) {
 #pragma unroll
-    for (int i = 0; i < kAppendIter; ++i) {
-        const int row = row0 + i * kRows;
-        const bool is_q = row < a.n_heads, is_v = row >= a.n_heads + a.n_kv_heads;
-        float4 y = x[i];
-        if (a.rotate && !is_v) {
-            const float2 c0 = cs[d / 2], c1 = cs[d / 2 + 1];
-            y.x = __fsub_rn(__fmul_rn(x[i].x, c0.x), __fmul_rn(x[i].y, c0.y));
-            y.y = __fadd_rn(__fmul_rn(x[i].x, c0.y), __fmul_rn(x[i].y, c0.x));
-            y.z = __fsub_rn(__fmul_rn(x[i].z, c1.x), __fmul_rn(x[i].w, c1.y));
-            y.w = __fadd_rn(__fmul_rn(x[i].z, c1.y), __fmul_rn(x[i].w, c1.x));
+        for (int i = 0; i < kAppendRows; ++i) {
+            const int row = row0 + i * kWide;
+            const bool is_q = row < a.n_heads, is_v = row >= a.n_heads + a.n_kv_heads;
+            const float4 x = A::value(raw[i]);
+            float4 y = x;
+            if (a.rotate && !is_v) {
+                y.x = __fsub_rn(__fmul_rn(x.x, c0.x), __fmul_rn(x.y, c0.y));
+                y.y = __fadd_rn(__fmul_rn(x.x, c0.y), __fmul_rn(x.y, c0.x));
+                y.z = __fsub_rn(__fmul_rn(x.z, c1.x), __fmul_rn(x.w, c1.y));
+                y.w = __fadd_rn(__fmul_rn(x.z, c1.y), __fmul_rn(x.w, c1.x));
+            }
+            if (is_q && row < end) A::template store<kVec>(qo + row * HD, y);
+            const bool live = stored && !is_q && row < end;
+            if constexpr (!Q4) {
+                if (!live) continue;
+            }
+            const int h = row - a.n_heads - (is_v ? a.n_kv_heads : 0);
+            const long long e = live ? (row_of_page + static_cast<long long>(h) * a.page.d) * HD + d : 0;
+            void *cache = is_v ? a.v_cache : a.k_cache;
+            if constexpr (Q4) {
+                __half *scale = is_v ? a.v_scale : a.k_scale;
+                group_store_q4_0(y, static_cast<uint8_t *>(cache) + (e & ~31ll) / 2, scale + e / 32, live);
+            } else {
+                Act<BMO_ACT_F16>::store<true>(static_cast<__half *>(cache) + e, y);
+            }
         }
-        if (is_q) A::store4(qo + row * HD + d, y, can_vec4(qo, 0));
-        const bool live = stored && !is_q && row < n_rows;
-        if constexpr (!Q4) {
-            if (!live) continue;
-        }
-        const int h = row - a.n_heads - (is_v ? a.n_kv_heads : 0);
-        const long long e =
-            live ? ((static_cast<long long>(page) * a.n_kv_heads + h) * a.page.d + at) * HD + d : 0;
-        void *cache = is_v ? a.v_cache : a.k_cache;
-        if constexpr (Q4) {
-            __half *scale = is_v ? a.v_scale : a.k_scale;
-            group_store_q4_0(y, static_cast<uint8_t *>(cache) + (e & ~31ll) / 2, scale + e / 32, live);
-        } else {
-            Act<BMO_ACT_F16>::store4(static_cast<__half *>(cache) + e, y, true);
-        }
+        row0 += kAppendRows * kWide;
+        if (row0 - lane / kLanes >= end) break;
+        load();
     }
 }
 
@@ -471,8 +487,8 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
                 hi = make_float4(n[4], n[5], n[6], n[7]);
             }
             T *o = out + c / 4 * 32 + c % 4 * 4;
-            A::store4(o, lo, true);
-            A::store4(o + 16, hi, true);
+            A::template store<true>(o, lo);
+            A::template store<true>(o + 16, hi);
         } else {
             if (stored) {
                 const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(cache) + row * HD) + c);
@@ -482,19 +498,41 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
                 lo = make_float4(f0.x, f0.y, f1.x, f1.y);
                 hi = make_float4(f2.x, f2.y, f3.x, f3.y);
             }
-            A::store4(out + 8 * c, lo, true);
-            A::store4(out + 8 * c + 4, hi, true);
+            A::template store<true>(out + 8 * c, lo);
+            A::template store<true>(out + 8 * c + 4, hi);
         }
     }
 }
 
 template <int HD, bool Q4>
-cudaError_t append_act(const PagedAppendArgs &a, int act, cudaStream_t s) {
-    constexpr int kRows = kAppendThreads / (HD / 4) * kAppendIter;
-    const dim3 grid(a.n, (a.n_heads + 2 * a.n_kv_heads + kRows - 1) / kRows);
-    if (act == BMO_ACT_F32) append_kernel<HD, Q4, BMO_ACT_F32><<<grid, kAppendThreads, 0, s>>>(a);
-    else if (act == BMO_ACT_F16) append_kernel<HD, Q4, BMO_ACT_F16><<<grid, kAppendThreads, 0, s>>>(a);
-    else append_kernel<HD, Q4, BMO_ACT_BF16><<<grid, kAppendThreads, 0, s>>>(a);
+cudaError_t append_act(PagedAppendArgs a, int act, cudaStream_t s) {
+    // Rows of a warp: one round of loads, or more rounds (fewer angles computed
+    // twice) once the warps are many: 32 an SM keep its loads in flight.
+    constexpr int kRound = kAppendRows * (128 / HD), kManyWarps = 148 * 32;
+    const int rows = a.n_heads + 2 * a.n_kv_heads;
+    const long long rounds = static_cast<long long>(a.n) * ((rows + kRound - 1) / kRound);
+    const int per = static_cast<int>(rounds / kManyWarps < 1 ? 1 : rounds / kManyWarps);
+    a.part_rows = per * kRound < rows ? per * kRound : rows;
+    a.parts = (rows + a.part_rows - 1) / a.part_rows;
+    const long long warps = static_cast<long long>(a.n) * a.parts;
+    const long long grid = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
+    const unsigned g = static_cast<unsigned>(grid);
+    auto run = [&](auto type) {
+        constexpr int kAct = decltype(type)::value;
+        using T = typename Act<kAct>::T;
+        auto vec = [&](const void *p, long long stride) {
+            return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && (a.n == 1 || stride % 4 == 0);
+        };
+        if (vec(a.k, a.k_stride) && vec(a.v, a.v_stride) &&
+            (!a.n_heads || (vec(a.q, a.q_stride) && vec(a.q_out, a.q_out_stride))))
+            append_kernel<HD, Q4, kAct, true><<<g, kAppendThreads, 0, s>>>(a);
+        else
+            append_kernel<HD, Q4, kAct, false><<<g, kAppendThreads, 0, s>>>(a);
+    };
+    if (act == BMO_ACT_F32) run(std::integral_constant<int, BMO_ACT_F32>{});
+    else if (act == BMO_ACT_F16) run(std::integral_constant<int, BMO_ACT_F16>{});
+    else run(std::integral_constant<int, BMO_ACT_BF16>{});
     return cudaGetLastError();
 }
 

@@ -38,6 +38,7 @@ struct PagedAppendArgs {
     void *k_cache, *v_cache;      // of the layer
     __half *k_scale, *v_scale;
     int n, n_heads, n_kv_heads;   // n_heads 0: no q
+    int parts, part_rows;         // warps of a token and rows of each (set by the launcher)
     long long n_slots;
     FastDiv page;
     int *status;
