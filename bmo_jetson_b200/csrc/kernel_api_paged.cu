@@ -10,13 +10,14 @@
 namespace bmo {
 namespace {
 
+constexpr int kPlanRoom = 65536;  // the plan's counters step past max_tokens by no more
 constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
 
 bool aligned(const void *p, size_t n) { return !(reinterpret_cast<uintptr_t>(p) & (n - 1)); }
 
 bool book_ok(const bmo_page_book &b) {
     return b.n_pages > 0 && b.page_size > 0 && b.page_size <= kPagedMaxPageSize && b.window >= 0 &&
-           static_cast<long long>(b.n_pages) * b.page_size <= INT_MAX;
+           static_cast<long long>(b.n_pages) * b.page_size <= INT_MAX - 65535;
 }
 
 bool table_ok(const bmo_page_book &b) {
@@ -91,7 +92,7 @@ int bmo_k_paged_plan(const bmo_page_book *book, const int32_t *n_new_dev, int ma
                      int32_t *pos_dev, int32_t *req_dev, int32_t *offsets_dev, int32_t *lens_out_dev,
                      int32_t *state_out_dev, void *stream) {
     if (!book || !book_ok(*book) || !table_ok(*book) || !book->free_pages || !book->state || !n_new_dev ||
-        max_tokens < 0 || (max_tokens && (!slot_dev || !pos_dev || !req_dev)) || !offsets_dev || !lens_out_dev ||
+        max_tokens < 0 || max_tokens >= INT_MAX - kPlanRoom || (max_tokens && (!slot_dev || !pos_dev || !req_dev)) || !offsets_dev || !lens_out_dev ||
         !state_out_dev || book->n_req > kPagedMaxReq)
         return kInvalid;
     PagedPlanArgs a{*book,       n_new_dev,    max_tokens,   slot_dev,     pos_dev,

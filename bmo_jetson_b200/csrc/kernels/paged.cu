@@ -40,21 +40,20 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f) {
 // What bounds it is latency: a few dependent loads and block barriers over a
 // few KB, so one CTA does all of it and no second launch follows, unless
 // there are so many new positions that one SM would take longer than the
-// launch (kPlanOneCta).  Every prefix sum is searched by the thread that
-// writes an entry, so entries are written side by side whatever the requests'
-// lengths are.
+// launch (kPlanOneCta).  Where no request has more than kFew of anything, the usual
+// step, each thread writes what its request has.  Otherwise the thread that writes
+// an entry searches the prefix sums for its request, so entries are written
+// side by side whatever the requests' lengths are, kPlanBatch of a thread's in flight.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanOneCta = 8192;
+constexpr int kFew = 2;
+constexpr int kPlanBatch = 4;
 
 struct PlanItem {
-    int len, add, take, give, first;  // first: first block given back
-    int after;
-    bool ends;
-};
-
-struct PlanSums {
-    long long take, give, add;
-    int bad;
+    int len, have;          // positions and pages before the step
+    uint32_t add, take, give;
+    int first;              // first block given back
+    int after;              // positions after the step
 };
 
 __device__ __forceinline__ PlanItem plan_item(const PagedPlanArgs &a, int r, int &bad) {
@@ -63,47 +62,61 @@ __device__ __forceinline__ PlanItem plan_item(const PagedPlanArgs &a, int r, int
     const long long cap = static_cast<long long>(b.max_blocks) * ps;  // < 2^31
     PlanItem it{};
     it.len = b.lens[r];
+    const int n = a.n_new[r];
     if (it.len < 0 || it.len > cap) {
         bad |= 1 << kErrBadIndex;
         it.len = 0;
         return it;
     }
-    const int n = a.n_new[r];
-    it.ends = n < 0;
     it.add = max(n, 0);
     if (it.add > cap - it.len) {
         bad |= 1 << kErrTableFull;
         it.add = 0;
     }
-    it.after = it.ends ? 0 : it.len + it.add;
-    const int have = (it.len + ps - 1) / ps;
-    it.take = it.ends ? 0 : (it.after + ps - 1) / ps - have;
+    it.after = n < 0 ? 0 : it.len + it.add;
+    it.have = (it.len + ps - 1) / ps;
+    it.take = n < 0 ? 0 : (it.after + ps - 1) / ps - it.have;
     it.first = b.window > 0 ? max(0, it.len - b.window) / ps : 0;
-    const int last = it.ends ? have : (b.window > 0 ? max(0, it.after - b.window) / ps : 0);
-    it.give = last - it.first;
+    it.give = (n < 0 ? it.have : b.window > 0 ? max(0, it.after - b.window) / ps : 0) - it.first;
     return it;
 }
 
-// Inclusive prefix sum over the CTA; `total` receives the whole sum.
-__device__ __forceinline__ int block_scan(int v, int *warp_sums, int &total) {
+// Sums below 2^31 exactly, larger ones as 2^31 - 1 (no step is that large).
+__device__ __forceinline__ uint32_t add_sat(uint32_t x, uint32_t y) { return min(x + y, 0x7fffffffu); }
+
+struct PlanSums {
+    uint32_t take, give, add;
+};
+__device__ __forceinline__ PlanSums operator+(PlanSums x, PlanSums y) {
+    return {add_sat(x.take, y.take), add_sat(x.give, y.give), add_sat(x.add, y.add)};
+}
+__device__ __forceinline__ PlanSums shfl_up(PlanSums x, int d) {
+    return {__shfl_up_sync(0xffffffffu, x.take, d), __shfl_up_sync(0xffffffffu, x.give, d), __shfl_up_sync(0xffffffffu, x.add, d)};
+}
+
+// Inclusive prefix sums over the CTA; `total` receives the whole sums.
+__device__ __forceinline__ PlanSums block_scan(PlanSums v, PlanSums *warp_sums, PlanSums &total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+        const PlanSums u = shfl_up(v, o);
+        if (lane >= o) v = v + u;
     }
     __syncthreads();
     if (lane == 31) warp_sums[warp] = v;
     __syncthreads();
-    int w = warp_sums[lane];
+    PlanSums w = warp_sums[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane >= o) w += u;
+        const PlanSums u = shfl_up(w, o);
+        if (lane >= o) w = w + u;
     }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-    return v + (warp ? before : 0);
+    auto from = [&](int l) {
+        return PlanSums{__shfl_sync(0xffffffffu, w.take, l), __shfl_sync(0xffffffffu, w.give, l), __shfl_sync(0xffffffffu, w.add, l)};
+    };
+    total = from(31);
+    const PlanSums before = from(max(warp - 1, 0));
+    return warp ? v + before : v;
 }
 
 // First index whose inclusive prefix sum exceeds i (ends[n - 1] > i).
@@ -117,36 +130,76 @@ __device__ __forceinline__ int owner(const int *ends, int n, int i) {
     return lo;
 }
 
+// For entries i < n of this CTA: read(i, request, number within the request)
+// of up to kPlanBatch of a thread's entries, then write(i, what was read).
+template <class T, class Read, class Write>
+__device__ __forceinline__ void plan_fill(const int *ends, int n_req, int n, Read read, Write write) {
+    for (int i0 = threadIdx.x; i0 < n; i0 += kPlanBatch * kPlanThreads) {
+        T got[kPlanBatch];
+#pragma unroll
+        for (int k = 0; k < kPlanBatch; ++k) {
+            const int i = i0 + k * kPlanThreads;
+            if (i >= n) continue;
+            const int w = owner(ends, n_req, i);
+            got[k] = read(i, w, i - (w ? ends[w - 1] : 0));
+        }
+#pragma unroll
+        for (int k = 0; k < kPlanBatch; ++k)
+            if (i0 + k * kPlanThreads < n) write(i0 + k * kPlanThreads, got[k]);
+    }
+}
+
+struct PlanCell {
+    long long at;
+    int page;
+};
+struct PlanToken {
+    int slot, pos, req;
+};
+
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int list_here) {
-    __shared__ int warp_sums[32];
+    __shared__ PlanSums warp_sums[32];
     __shared__ int s_end[kPlanThreads], s_len[kPlanThreads], s_first[kPlanThreads];
     __shared__ unsigned long long s_tot[3];
     __shared__ int s_bad;
     const bmo_page_book &b = a.book;
     const int tid = threadIdx.x, ps = b.page_size, n_pages = b.n_pages;
     const int head = b.state[0], count = b.state[1];
+    const bool one = b.n_req <= kPlanThreads;  // each thread has one request at most
 
-    // totals, and whether the step can be served
-    if (tid < 3) s_tot[tid] = 0;
-    if (tid == 0) s_bad = 0;
-    __syncthreads();
-    {
-        PlanSums t{};
-        for (int r = tid; r < b.n_req; r += kPlanThreads) {
-            const PlanItem it = plan_item(a, r, t.bad);
-            t.take += it.take;
-            t.give += it.give;
-            t.add += it.add;
+    // ---- totals, and whether the step can be served ----
+    PlanItem it{};
+    PlanSums end{}, total{};
+    int bad = 0, old_page = -1;
+    long long all_take, all_give, all_add;
+    if (one) {
+        if (tid < b.n_req) {
+            it = plan_item(a, tid, bad);
+            // the page that the request's next position lies in, unless that begins a page
+            if (it.add && it.len % ps) old_page = b.table[static_cast<long long>(tid) * b.max_blocks + it.len / ps];
         }
-        if (t.take) atomicAdd(&s_tot[0], static_cast<unsigned long long>(t.take));
-        if (t.give) atomicAdd(&s_tot[1], static_cast<unsigned long long>(t.give));
-        if (t.add) atomicAdd(&s_tot[2], static_cast<unsigned long long>(t.add));
-        if (t.bad) atomicOr(&s_bad, t.bad);
+        end = block_scan({it.take, it.give, it.add}, warp_sums, total);
+        all_take = total.take, all_give = total.give, all_add = total.add;
+        if (tid == 0) s_bad = 0;
+        __syncthreads();
+        if (bad) atomicOr(&s_bad, bad);
+    } else {
+        if (tid < 3) s_tot[tid] = 0;
+        if (tid == 0) s_bad = 0;
+        __syncthreads();
+        unsigned long long t[3] = {};
+        for (int r = tid; r < b.n_req; r += kPlanThreads) {
+            const PlanItem x = plan_item(a, r, bad);
+            t[0] += x.take, t[1] += x.give, t[2] += x.add;
+        }
+        for (int i = 0; i < 3; ++i)
+            if (t[i]) atomicAdd(&s_tot[i], t[i]);
+        if (bad) atomicOr(&s_bad, bad);
+        __syncthreads();
+        all_take = s_tot[0], all_give = s_tot[1], all_add = s_tot[2];
     }
-    __syncthreads();
-    const long long all_take = static_cast<long long>(s_tot[0]), all_give = static_cast<long long>(s_tot[1]),
-                    all_add = static_cast<long long>(s_tot[2]);
-    int bad = s_bad;
+    const bool few = __syncthreads_and(one && it.take <= kFew && it.give <= kFew && it.add <= kFew);
+    bad = s_bad;
     if (!bad) {
         if (head < 0 || head >= n_pages || count < 0 || count > n_pages) bad |= 1 << kErrBadIndex;
         else if (all_take > count) bad |= 1 << kErrNoPages;
@@ -156,75 +209,104 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
     }
     const bool ok = bad == 0;
     const int n_add = ok ? static_cast<int>(all_add) : 0;
+    auto ring_at = [&](long long i) { return (static_cast<long long>(head) + i) % n_pages; };
+    auto cell = [&](int r, int block) { return static_cast<long long>(r) * b.max_blocks + block; };
 
-    // new pages and the list of new positions, kPlanThreads requests at a time
-    if (ok) {
-        int take0 = 0, add0 = 0;
-        for (int r0 = 0; r0 < b.n_req; r0 += kPlanThreads) {
+    if (few && ok) {
+        const int r = tid;
+        int taken[kFew] = {-1, -1};
+#pragma unroll
+        for (int j = 0; j < kFew; ++j)
+            if (j < it.take) {
+                taken[j] = b.free_pages[ring_at(end.take - it.take + j)];
+                b.table[cell(r, it.have + j)] = taken[j];
+            }
+        int given[kFew];
+#pragma unroll
+        for (int j = 0; j < kFew; ++j)
+            if (j < it.give) {
+                const int block = it.first + j;
+                given[j] = block >= it.have ? taken[block - it.have ? 1 : 0] : b.table[cell(r, block)];
+            }
+#pragma unroll
+        for (int j = 0; j < kFew; ++j)
+            if (j < it.add) {
+                const int p = it.len + j, i = end.add - it.add + j, block = p / ps;
+                const int page = block < it.have ? old_page : taken[block - it.have ? 1 : 0];
+                if (list_here) a.slot[i] = page * ps + (p - block * ps), a.pos[i] = p, a.req[i] = r;
+            }
+        if (r < b.n_req) a.offsets[r] = end.add - it.add;
+        __syncthreads();  // every page is taken before one is given back into the ring
+#pragma unroll
+        for (int j = 0; j < kFew; ++j)
+            if (j < it.give) b.free_pages[ring_at(count + static_cast<long long>(end.give - it.give) + j)] = given[j];
+        if (r < b.n_req) a.lens_out[r] = it.after;
+    } else {
+        // new pages and the list of new positions, kPlanThreads requests at a time
+        long long take0 = 0;
+        int add0 = 0;
+        for (int r0 = 0; ok && r0 < b.n_req; r0 += kPlanThreads) {
             const int r = r0 + tid, nr = min(kPlanThreads, b.n_req - r0);
-            int ignore = 0, takes, adds;
-            PlanItem it{};
-            if (r < b.n_req) it = plan_item(a, r, ignore);
-            const int take_end = block_scan(it.take, warp_sums, takes);
-            const int add_end = block_scan(it.add, warp_sums, adds);
-            s_end[tid] = take_end;
+            if (!one) {
+                int ignore = 0;
+                it = r < b.n_req ? plan_item(a, r, ignore) : PlanItem{};
+                end = block_scan({it.take, it.give, it.add}, warp_sums, total);
+            }
+            s_end[tid] = end.take;
             s_len[tid] = it.len;
             __syncthreads();
-            for (int i = tid; i < takes; i += kPlanThreads) {
-                const int w = owner(s_end, nr, i);
-                const int block = (s_len[w] + ps - 1) / ps + i - (w ? s_end[w - 1] : 0);
-                const long long at = (static_cast<long long>(head) + take0 + i) % n_pages;
-                b.table[static_cast<long long>(r0 + w) * b.max_blocks + block] = b.free_pages[at];
-            }
+            plan_fill<PlanCell>(
+                s_end, nr, total.take,
+                [&](int i, int w, int j) {
+                    return PlanCell{cell(r0 + w, (s_len[w] + ps - 1) / ps + j), b.free_pages[ring_at(take0 + i)]};
+                },
+                [&](int, PlanCell c) { b.table[c.at] = c.page; });
             __syncthreads();
-            if (r < b.n_req) a.offsets[r] = add0 + add_end - it.add;
+            if (r < b.n_req) a.offsets[r] = add0 + static_cast<int>(end.add - it.add);
             if (list_here) {
-                s_end[tid] = add_end;
+                s_end[tid] = end.add;
                 __syncthreads();
-                for (int i = tid; i < adds; i += kPlanThreads) {
-                    const int w = owner(s_end, nr, i);
-                    const int p = s_len[w] + i - (w ? s_end[w - 1] : 0);
-                    const int page = b.table[static_cast<long long>(r0 + w) * b.max_blocks + p / ps];
-                    a.slot[add0 + i] = page * ps + p % ps;
-                    a.pos[add0 + i] = p;
-                    a.req[add0 + i] = r0 + w;
-                }
+                plan_fill<PlanToken>(
+                    s_end, nr, total.add,
+                    [&](int, int w, int j) {
+                        const int p = s_len[w] + j;
+                        return PlanToken{b.table[cell(r0 + w, p / ps)] * ps + p % ps, p, r0 + w};
+                    },
+                    [&](int i, PlanToken t) { a.slot[add0 + i] = t.slot, a.pos[add0 + i] = t.pos, a.req[add0 + i] = t.req; });
                 __syncthreads();
             }
-            take0 += takes;
-            add0 += adds;
+            take0 += total.take;
+            add0 += total.add;
         }
-    } else {
-        for (int r = tid; r < b.n_req; r += kPlanThreads) a.offsets[r] = 0;
+        if (!ok)
+            for (int r = tid; r < b.n_req; r += kPlanThreads) a.offsets[r] = 0;
+        __syncthreads();  // every page is taken before one is given back into the ring
+        long long give0 = 0;
+        for (int r0 = 0; r0 < b.n_req; r0 += kPlanThreads) {
+            const int r = r0 + tid, nr = min(kPlanThreads, b.n_req - r0);
+            if (!one && ok) {
+                int ignore = 0;
+                it = r < b.n_req ? plan_item(a, r, ignore) : PlanItem{};
+                end = block_scan({it.take, it.give, it.add}, warp_sums, total);
+            }
+            if (ok && all_give) {
+                s_end[tid] = end.give;
+                s_first[tid] = it.first;
+                __syncthreads();
+                plan_fill<int>(
+                    s_end, nr, total.give, [&](int, int w, int j) { return b.table[cell(r0 + w, s_first[w] + j)]; },
+                    [&](int i, int page) { b.free_pages[ring_at(count + give0 + i)] = page; });
+                __syncthreads();
+                give0 += total.give;
+            }
+            if (r < b.n_req) a.lens_out[r] = ok ? it.after : b.lens[r];
+        }
     }
     if (tid == 0) a.offsets[b.n_req] = n_add;
     if (list_here)
         for (int i = n_add + tid; i < a.max_tokens; i += kPlanThreads) a.slot[i] = a.pos[i] = a.req[i] = -1;
-    __syncthreads();  // every page is taken before one is given back into the ring
-
-    int give0 = 0;
-    for (int r0 = 0; r0 < b.n_req; r0 += kPlanThreads) {
-        const int r = r0 + tid, nr = min(kPlanThreads, b.n_req - r0);
-        int ignore = 0, gives = 0;
-        PlanItem it{};
-        if (r < b.n_req) it = plan_item(a, r, ignore);
-        if (ok && all_give) {
-            s_end[tid] = block_scan(it.give, warp_sums, gives);
-            s_first[tid] = it.first;
-            __syncthreads();
-            for (int i = tid; i < gives; i += kPlanThreads) {
-                const int w = owner(s_end, nr, i);
-                const int block = s_first[w] + i - (w ? s_end[w - 1] : 0);
-                const long long at = (static_cast<long long>(head) + count + give0 + i) % n_pages;
-                b.free_pages[at] = b.table[static_cast<long long>(r0 + w) * b.max_blocks + block];
-            }
-            __syncthreads();
-            give0 += gives;
-        }
-        if (r < b.n_req) a.lens_out[r] = ok ? it.after : b.lens[r];
-    }
     if (tid == 0) {
-        a.state_out[0] = ok ? static_cast<int>((head + all_take) % n_pages) : head;
+        a.state_out[0] = ok ? static_cast<int>(ring_at(all_take)) : head;
         a.state_out[1] = ok ? static_cast<int>(count - all_take + all_give) : count;
         a.state_out[2] = bad;
         a.state_out[3] = n_add;
@@ -232,16 +314,27 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
 }
 
 // The list of new positions alone, over all SMs, from the plan's offsets.
-__global__ void plan_list_kernel(PagedPlanArgs a) {
+constexpr int kListThreads = 256;
+constexpr int kListStaged = 2048;  // offsets kept in shared memory
+
+__global__ void __launch_bounds__(kListThreads) plan_list_kernel(PagedPlanArgs a) {
+    __shared__ int s_ends[kListStaged];
     const bmo_page_book &b = a.book;
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    pdl_wait();
+    const bool staged = b.n_req <= kListStaged;
+    if (staged) {
+        for (int r = threadIdx.x; r < b.n_req; r += kListThreads) s_ends[r] = a.offsets[r + 1];
+        __syncthreads();
+    }
+    const int *ends = staged ? s_ends : a.offsets + 1;
+    const int i = blockIdx.x * kListThreads + threadIdx.x;
     if (i >= a.max_tokens) return;
-    if (i >= a.offsets[b.n_req]) {
+    if (i >= ends[b.n_req - 1]) {
         a.slot[i] = a.pos[i] = a.req[i] = -1;
         return;
     }
-    const int r = owner(a.offsets + 1, b.n_req, i);
-    const int p = a.lens_out[r] - (a.offsets[r + 1] - i);
+    const int r = owner(ends, b.n_req, i);
+    const int p = a.lens_out[r] - (ends[r] - i);
     const int page = b.table[static_cast<long long>(r) * b.max_blocks + p / b.page_size];
     a.slot[i] = page * b.page_size + p % b.page_size;
     a.pos[i] = p;
@@ -448,76 +541,92 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 // ---- read ----
 //
-// Bound by its bytes.  One CTA per row number; a thread turns 16 bytes of
-// fp16 or 4 bytes of nibbles into 8 elements.
-constexpr int kReadThreads = 256;
+// Bound by its bytes, most of them written when codes become floats.  A lane
+// makes 4 consecutive elements, so a warp writes whole lines; two lanes read the
+// same 4 bytes of codes, one for the low nibbles and one for the high ones.  Rows are shared out over
+// warps as for the append.
+constexpr int kReadThreads = 128;
+constexpr int kReadRows = 8;  // row slots of a lane in flight
 
 template <int HD, bool Q4, int ACT>
 __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constant__ PagedReadArgs a) {
     using A = Act<ACT>;
     using T = typename A::T;
-    constexpr int kPer = HD / 8;
-    const int slot = a.slot[blockIdx.x];
+    constexpr int kLanes = HD / 4, kWide = 32 / kLanes;  // lanes of a row, rows of a warp's access
+    const int lane = threadIdx.x & 31, c = lane % kLanes;
+    const long long item = static_cast<long long>(blockIdx.x) * (kReadThreads / 32) + (threadIdx.x >> 5);
+    const int token = static_cast<int>(item / a.parts), part = static_cast<int>(item - static_cast<long long>(token) * a.parts);
+    if (token >= a.n) return;
+    const int slot = a.slot[token];
     const bool stored = slot >= 0 && slot < a.n_slots;
-    if (threadIdx.x == 0 && !stored && slot != -1) raise_error(a.status, kErrBadIndex);
+    if (part == 0 && lane == 0 && !stored && slot != -1) raise_error(a.status, kErrBadIndex);
     const uint32_t page = stored ? fast_div(slot, a.page) : 0;
     const uint32_t at = stored ? slot - page * a.page.d : 0;
-    const int items = a.n_kv_heads * kPer;
-    const long long out0 = static_cast<long long>(blockIdx.x) * a.n_kv_heads * HD;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 2 * items; i += blockDim.x) {
-        const bool is_v = i >= items;
-        const int j = is_v ? i - items : i;
-        const int h = j / kPer, c = j % kPer;
-        const long long row = (static_cast<long long>(page) * a.n_kv_heads + h) * a.page.d + at;
-        const void *cache = is_v ? a.v_cache : a.k_cache;
-        T *out = static_cast<T *>(is_v ? a.v_out : a.k_out) + out0 + h * HD;
-        float4 lo = make_float4(0.0f, 0.0f, 0.0f, 0.0f), hi = lo;
-        if constexpr (Q4) {
-            if (stored) {
-                const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(cache) + row * (HD / 2)) + c);
-                const float s = __half2float(__ldg((is_v ? a.v_scale : a.k_scale) + row * (HD / 32) + c / 4));
-                float n[8];
+    const long long row_of_page = static_cast<long long>(page) * a.n_kv_heads * a.page.d + at;
+    const long long out0 = static_cast<long long>(token) * a.n_kv_heads * HD;
+    const int end = min(2 * a.n_kv_heads, (part + 1) * a.part_rows);
+#pragma unroll 1
+    for (int row0 = part * a.part_rows; row0 < end; row0 += kReadRows * kWide) {
+        using Raw = std::conditional_t<Q4, uint32_t, uint2>;
+        Raw raw[kReadRows];
+        __half scale[kReadRows];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    n[b] = __fmul_rn(static_cast<float>(static_cast<int>(w >> (8 * b) & 15) - 8), s);
-                    n[4 + b] = __fmul_rn(static_cast<float>(static_cast<int>(w >> (8 * b + 4) & 15) - 8), s);
-                }
-                lo = make_float4(n[0], n[1], n[2], n[3]);
-                hi = make_float4(n[4], n[5], n[6], n[7]);
+        for (int i = 0; i < kReadRows; ++i) {  // keys of all heads, then values; past the end: the last row again
+            const int row = min(row0 + i * kWide + lane / kLanes, end - 1);
+            const bool is_v = row >= a.n_kv_heads;
+            const long long r = row_of_page + static_cast<long long>(is_v ? row - a.n_kv_heads : row) * a.page.d;
+            const void *cache = is_v ? a.v_cache : a.k_cache;
+            if constexpr (Q4) {
+                raw[i] = __ldcs(reinterpret_cast<const uint32_t *>(static_cast<const uint8_t *>(cache) + r * (HD / 2)) + c / 8 * 4 + c % 4);
+                scale[i] = __ldg((is_v ? a.v_scale : a.k_scale) + r * (HD / 32) + c / 8);
+            } else {
+                raw[i] = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const __half *>(cache) + r * HD) + c);
             }
-            T *o = out + c / 4 * 32 + c % 4 * 4;
-            A::template store<true>(o, lo);
-            A::template store<true>(o + 16, hi);
-        } else {
-            if (stored) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(cache) + row * HD) + c);
-                const __half2 *p = reinterpret_cast<const __half2 *>(&u);
-                const float2 f0 = __half22float2(p[0]), f1 = __half22float2(p[1]), f2 = __half22float2(p[2]),
-                             f3 = __half22float2(p[3]);
-                lo = make_float4(f0.x, f0.y, f1.x, f1.y);
-                hi = make_float4(f2.x, f2.y, f3.x, f3.y);
+        }
+#pragma unroll
+        for (int i = 0; i < kReadRows; ++i) {
+            const int row = row0 + i * kWide + lane / kLanes;
+            if (row >= end) continue;
+            const bool is_v = row >= a.n_kv_heads;
+            T *out = static_cast<T *>(is_v ? a.v_out : a.k_out) + out0 + (is_v ? row - a.n_kv_heads : row) * HD;
+            float4 x;
+            if constexpr (Q4) {
+                const float d = __half2float(scale[i]);
+                const uint32_t w = c & 4 ? raw[i] >> 4 : raw[i];
+                auto code = [&](int b) { return __fmul_rn(static_cast<float>(static_cast<int>(w >> (8 * b) & 15) - 8), d); };
+                x = make_float4(code(0), code(1), code(2), code(3));
+            } else {
+                x = Act<BMO_ACT_F16>::value(raw[i]);
             }
-            A::template store<true>(out + 8 * c, lo);
-            A::template store<true>(out + 8 * c + 4, hi);
+            if (!stored) x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            A::template store<true>(out + 4 * c, x);
         }
     }
 }
 
+// Rows of a warp: one round of loads, or more rounds once the warps are many (32 an SM keep their loads in flight).
+struct RowShare {
+    int part_rows, parts;
+    unsigned grid;
+};
+bool share_rows(int n, int rows, int round, int warps_per_cta, RowShare &out) {
+    constexpr int kManyWarps = 148 * 64;
+    const int rounds = (rows + round - 1) / round;
+    const long long per = static_cast<long long>(n) * rounds / kManyWarps;
+    out.parts = per < 1 ? rounds : per < rounds ? static_cast<int>((rounds + per - 1) / per) : 1;
+    out.part_rows = (rounds + out.parts - 1) / out.parts * round;
+    const long long grid = (static_cast<long long>(n) * out.parts + warps_per_cta - 1) / warps_per_cta;
+    out.grid = static_cast<unsigned>(grid);
+    return grid <= 0x7fffffff;
+}
+
 template <int HD, bool Q4>
 cudaError_t append_act(PagedAppendArgs a, int act, cudaStream_t s) {
-    // Rows of a warp: one round of loads, or more rounds (fewer angles computed
-    // twice) once the warps are many: 32 an SM keep its loads in flight.
-    constexpr int kRound = kAppendRows * (128 / HD), kManyWarps = 148 * 32;
-    const int rows = a.n_heads + 2 * a.n_kv_heads;
-    const long long rounds = static_cast<long long>(a.n) * ((rows + kRound - 1) / kRound);
-    const int per = static_cast<int>(rounds / kManyWarps < 1 ? 1 : rounds / kManyWarps);
-    a.part_rows = per * kRound < rows ? per * kRound : rows;
-    a.parts = (rows + a.part_rows - 1) / a.part_rows;
-    const long long warps = static_cast<long long>(a.n) * a.parts;
-    const long long grid = (warps + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
-    if (grid > 0x7fffffff) return cudaErrorInvalidValue;
-    const unsigned g = static_cast<unsigned>(grid);
+    RowShare r;
+    if (!share_rows(a.n, a.n_heads + 2 * a.n_kv_heads, kAppendRows * (128 / HD), kAppendThreads / 32, r)) return cudaErrorInvalidValue;
+    a.part_rows = r.part_rows;
+    a.parts = r.parts;
+    const unsigned g = r.grid;
     auto run = [&](auto type) {
         constexpr int kAct = decltype(type)::value;
         using T = typename Act<kAct>::T;
@@ -537,12 +646,14 @@ cudaError_t append_act(PagedAppendArgs a, int act, cudaStream_t s) {
 }
 
 template <int HD, bool Q4>
-cudaError_t read_act(const PagedReadArgs &a, int act, cudaStream_t s) {
-    const int items = 2 * a.n_kv_heads * (HD / 8);
-    const int threads = items < kReadThreads ? (items + 31) / 32 * 32 : kReadThreads;
-    if (act == BMO_ACT_F32) read_kernel<HD, Q4, BMO_ACT_F32><<<a.n, threads, 0, s>>>(a);
-    else if (act == BMO_ACT_F16) read_kernel<HD, Q4, BMO_ACT_F16><<<a.n, threads, 0, s>>>(a);
-    else read_kernel<HD, Q4, BMO_ACT_BF16><<<a.n, threads, 0, s>>>(a);
+cudaError_t read_act(PagedReadArgs a, int act, cudaStream_t s) {
+    RowShare r;
+    if (!share_rows(a.n, 2 * a.n_kv_heads, kReadRows * (128 / HD), kReadThreads / 32, r)) return cudaErrorInvalidValue;
+    a.part_rows = r.part_rows;
+    a.parts = r.parts;
+    if (act == BMO_ACT_F32) read_kernel<HD, Q4, BMO_ACT_F32><<<r.grid, kReadThreads, 0, s>>>(a);
+    else if (act == BMO_ACT_F16) read_kernel<HD, Q4, BMO_ACT_F16><<<r.grid, kReadThreads, 0, s>>>(a);
+    else read_kernel<HD, Q4, BMO_ACT_BF16><<<r.grid, kReadThreads, 0, s>>>(a);
     return cudaGetLastError();
 }
 
@@ -553,8 +664,17 @@ cudaError_t launch_paged_plan(const PagedPlanArgs &a, cudaStream_t s) {
     plan_kernel<<<1, kPlanThreads, 0, s>>>(a, list_here);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess || list_here) return e;
-    plan_list_kernel<<<(a.max_tokens + 255) / 256, 256, 0, s>>>(a);
-    return cudaGetLastError();
+    // its CTAs are set up while the plan runs
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((a.max_tokens + kListThreads - 1) / kListThreads);
+    cfg.blockDim = dim3(kListThreads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, plan_list_kernel, a);
 }
 
 cudaError_t launch_paged_append(const PagedAppendArgs &a, int head_dim, int kv_type, int act, cudaStream_t s) {

@@ -636,7 +636,7 @@ struct PaSmem {
     float o[kPieces][NH * HD];
     Head head[kPieces];
     int whole[kPieces];  // -1: no piece; bit 0: begins at the head's first tile, bit 1: ends at its last
-    int scan[kPaWarps];
+    int scan[kPaWarps], longest[kPaWarps];
     Head join_head[2];
     int join_n[2], join_c0[2];  // pieces that this CTA, last to arrive, joins; the first one's CTA
 };
@@ -646,6 +646,7 @@ constexpr int kMaxGrid = 640;
 __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -INFINITY : (m - kHead + log2f(l)) * kLn2; }
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : __frcp_rn(l); }
 
+constexpr uint32_t kJoinTiles = 4;
 constexpr int kJoinBatch = 16;  // pieces requested at a time
 
 // Release of the CTA's earlier writes (ordered by a barrier before it) and acquire of the others'.
@@ -701,8 +702,10 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     if (lane < 2) S.whole[2 * warp + lane] = -1;
     if (tid < 2) S.join_n[tid] = 0;
     uint32_t my_end = 0;  // up to 32 rows: of rows 0..lane, in every warp
+    uint32_t longest = 0;
     if (a.n_rows <= 32) {
         my_end = lane < a.n_rows ? row_tiles(lane) : 0;
+        longest = __reduce_max_sync(0xffffffffu, my_end);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t x = __shfl_up_sync(0xffffffffu, my_end, o);
@@ -714,9 +717,12 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         uint32_t sum = 0;
 #pragma unroll 1
         for (int r = r0; r < r1; ++r) {
-            sum += row_tiles(r);
+            const uint32_t n = row_tiles(r);
+            longest = max(longest, n);
+            sum += n;
             ends[r] = sum;
         }
+        longest = __reduce_max_sync(0xffffffffu, longest);
         uint32_t inc = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -724,7 +730,10 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             if (lane >= o) inc += x;
         }
         if (lane == 31) S.scan[warp] = inc;
+        if (lane == 0) S.longest[warp] = longest;
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kPaWarps; ++w) longest = max(longest, S.longest[w]);
         uint32_t before = inc - sum;
 #pragma unroll
         for (int w = 0; w < kPaWarps - 1; ++w) before += w < warp ? S.scan[w] : 0;
@@ -740,7 +749,12 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     const uint32_t per = max(1u, (total + gridDim.x * kPaWarps - 1) / (gridDim.x * kPaWarps));
     const uint32_t me = blockIdx.x * kPaWarps + warp;
     uint32_t u = static_cast<uint32_t>(min(static_cast<unsigned long long>(total), static_cast<unsigned long long>(me) * per));
-    const uint32_t u_end = u + min(per, total - u);
+    uint32_t u_end = u + min(per, total - u);
+    // Few, short heads: a head a CTA, so that none waits for other CTAs.  Joining
+    // through global memory takes about as long as kJoinTiles tiles one after another.
+    const uint32_t warp_tiles = (longest + kPaWarps - 1) / kPaWarps;
+    const bool apart = static_cast<uint32_t>(a.n_rows) * units <= gridDim.x && warp_tiles <= per + kJoinTiles;
+    if (apart) u = blockIdx.x, u_end = blockIdx.x < a.n_rows * units ? u + 1 : u;
 
     // rows without a position
 #pragma unroll 1
@@ -759,27 +773,39 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
 #pragma unroll 1
     while (u < u_end) {
         // ---- the head that tile u belongs to ----
-        const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
         int row;
-        if (few) {
-            row = __popc(__ballot_sync(0xffffffffu, lane < a.n_rows && my_end <= q));
+        uint32_t row0, span, unit, from, to;  // [0, kHeadCost) of a head stands for its other costs, then come its tiles
+        if (apart) {
+            row = pa_div(u, a.units);
+            unit = u - row * units;
+            row0 = 0;
+            u = u_end;
+            const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
+            span = row_end - (row ? row_prev : 0);
+            if (!span) break;
+            const uint32_t n = (span - R::kHeadCost + kPaWarps - 1) / kPaWarps;
+            from = min(warp * n + R::kHeadCost, span), to = min(from + n, span);
         } else {
-            int lo = 0, hi = a.n_rows - 1;
+            const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
+            if (few) {
+                row = __popc(__ballot_sync(0xffffffffu, lane < a.n_rows && my_end <= q));
+            } else {
+                int lo = 0, hi = a.n_rows - 1;
 #pragma unroll 1
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (ends[mid] > q) hi = mid;
-                else lo = mid + 1;
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (ends[mid] > q) hi = mid;
+                    else lo = mid + 1;
+                }
+                row = lo;
             }
-            row = lo;
+            const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
+            row0 = row ? row_prev : 0;
+            span = row_end - row0;
+            unit = (u - row0 * units) / span;
+            from = u - row0 * units - unit * span, to = min(span, from + (u_end - u));
+            u += to - from;
         }
-        const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
-        const uint32_t row0 = row ? row_prev : 0;
-        // [0, kHeadCost) of a head stands for its other costs, then come its tiles
-        const uint32_t span = row_end - row0;
-        const uint32_t unit = (u - row0 * units) / span;
-        const uint32_t from = u - row0 * units - unit * span, to = min(span, from + (u_end - u));
-        u += to - from;
         const int tile0 = max(static_cast<int>(from) - R::kHeadCost, 0), tile1 = static_cast<int>(to) - R::kHeadCost;
         if (tile1 <= tile0) continue;
         Head hd;

@@ -53,6 +53,7 @@ struct PagedReadArgs {
     const __half *k_scale, *v_scale;
     void *k_out, *v_out;
     int n, n_kv_heads;
+    int parts, part_rows;  // as for the append
     long long n_slots;
     FastDiv page;
     int *status;

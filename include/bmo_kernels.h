@@ -170,7 +170,7 @@ BMO_API int bmo_k_sample_token(const float *logits_dev, int n, float temp, int t
  * fp16 scale planes [..][head_dim / 32] (kv_type 1).  Position p of request r
  * is in page table[r][p / page_size] at slot p % page_size; a "slot number"
  * is page * page_size + slot.  head_dim 64 or 128; page_size 1..65536;
- * n_pages * page_size below 2^31, max_blocks * page_size below 2^31 - 65535.
+ * n_pages * page_size and max_blocks * page_size below 2^31 - 65535.
  * No counterpart in the reference, which decodes one session. */
 
 /* Element types of the activations of the paged calls (q, k, v, outputs). */
