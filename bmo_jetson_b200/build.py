@@ -3,7 +3,9 @@
 CUDA sources are compiled by nvcc with ``-gencode arch=compute_100a,code=sm_100a``,
 host sources by g++; the shared library links the CUDA runtime statically so it
 does not depend on whichever libcudart a host process already loaded.
-Rebuilds only objects whose source or headers changed.
+Rebuilds only objects whose source or headers changed.  Where torch is
+installed, the torch binding of the paged cache is built beside it
+(bmo_jetson_b200/lib/_paged.so).
 
     python -m bmo_jetson_b200.build [--force] [-j N]
 """
@@ -21,6 +23,9 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "lib", "obj")
 LIB = os.path.join(HERE, "lib", "libbmo.so")
+# torch binding of the paged cache (bmo_jetson_b200/paged.py): an extension module, built where torch is installed
+BINDING_SRC = os.path.join(HERE, "binding", "paged_torch.cpp")
+BINDING = os.path.join(HERE, "lib", "_paged.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CXX = "/usr/bin/g++"
 CUDA_INC = "/usr/local/cuda/include"
@@ -64,6 +69,27 @@ def _compile(cmd):
     return r.stderr
 
 
+def build_binding(force: bool = False):
+    """Builds the torch binding; None where torch or Python's headers are missing."""
+    import importlib.util
+    import sysconfig
+    spec = importlib.util.find_spec("torch")  # not imported: the paths are enough
+    py = sysconfig.get_paths()["include"]
+    if spec is None or not spec.submodule_search_locations or not os.path.exists(os.path.join(py, "Python.h")):
+        return None
+    t = list(spec.submodule_search_locations)[0]
+    deps = [BINDING_SRC, os.path.join(ROOT, "include", "bmo_kernels.h")]
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps):
+        return BINDING
+    os.makedirs(os.path.dirname(BINDING), exist_ok=True)
+    tmp = BINDING + ".tmp"
+    _compile([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", f"-I{ROOT}/include",
+              f"-I{t}/include", f"-I{t}/include/torch/csrc/api/include", f"-I{py}", f"-I{CUDA_INC}", BINDING_SRC, "-o", tmp,
+              f"-L{t}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
     os.makedirs(OBJ, exist_ok=True)
     cu, cpp = _sources()
@@ -96,6 +122,7 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
         _compile([NVCC] + ARCH + ["-shared", "-ccbin", CXX, "-o", tmp] + objs +
                  ["-cudart", "static", "-lpthread", "-ldl", "-Xlinker", "--no-undefined"])
         os.replace(tmp, LIB)
+    build_binding(force)
     return LIB
 
 

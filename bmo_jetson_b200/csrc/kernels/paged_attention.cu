@@ -399,7 +399,7 @@ struct Q4Rows {
     static constexpr int kKW = HD / 32;           // words of a key row a lane holds
     static constexpr int kVW = HD / 64;           // words of a value row a lane holds
     uint32_t q[HD / 16][2];
-    float inv, bias[2];
+    float inv, bias[2][2];  // [chain][column]
     float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
     float vs[kSub][2];
     // B fragments of the query: a lane splits 4 elements, elements 16..31 of a
@@ -415,12 +415,16 @@ struct Q4Rows {
         const QueryPart x = query_part(e, i < 4 ? 1.0f : 0.0625f);
         inv = x.inv * qscale;
         const float weight = i < 4 ? 1.0f : 16.0f;
-        float sum_hi = weight * ((__half2float(x.hi[0]) + __half2float(x.hi[1])) + (__half2float(x.hi[2]) + __half2float(x.hi[3])));
-        float sum_lo = weight * ((__half2float(x.lo[0]) + __half2float(x.lo[1])) + (__half2float(x.lo[2]) + __half2float(x.lo[3])));
+        // sums of the elements that each of the two chains of products takes
+        float sum[2][2] = {{weight * (__half2float(x.hi[0]) + __half2float(x.hi[2])), weight * (__half2float(x.lo[0]) + __half2float(x.lo[2]))},
+                           {weight * (__half2float(x.hi[1]) + __half2float(x.hi[3])), weight * (__half2float(x.lo[1]) + __half2float(x.lo[3]))}};
 #pragma unroll
-        for (int d = 1; d < 8; d <<= 1) {
-            sum_hi += __shfl_xor_sync(0xffffffffu, sum_hi, d);
-            sum_lo += __shfl_xor_sync(0xffffffffu, sum_lo, d);
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) sum[j / 2][j % 2] += __shfl_xor_sync(0xffffffffu, sum[j / 2][j % 2], d);
+            // columns 2t, 2t + 1 start at -8 2^-24 sum q of block t
+            const float of_t = __shfl_sync(0xffffffffu, sum[j / 2][j % 2], (8 * t) & 31);
+            bias[j / 2][j % 2] = t < kBlocks ? -4.76837158203125e-07f * of_t : 0.0f;
         }
         if (4 * lane < HD) {
             // word 4 (i % 4): codes of bytes 4 (i % 4).. : elements 0, 2 then 1, 3; low nibbles before high ones
@@ -428,10 +432,6 @@ struct Q4Rows {
             dst[0] = half_bits2(x.hi[0], x.hi[2]), dst[2] = half_bits2(x.hi[1], x.hi[3]);
             dst[16] = half_bits2(x.lo[0], x.lo[2]), dst[18] = half_bits2(x.lo[1], x.lo[3]);
         }
-        // the sums of columns 2t, 2t + 1 start at -8 2^-24 sum q of block t
-        bias[0] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum_hi, (8 * t) & 31);
-        bias[1] = -4.76837158203125e-07f * __shfl_sync(0xffffffffu, sum_lo, (8 * t) & 31);
-        if (t >= kBlocks) bias[0] = bias[1] = 0.0f;
         __syncwarp();
         // lane t holds bytes 4 w.. of block blk, w in [w0, w0 + kKW); column pair g / 2 is block g / 2
         const int blk = HD == 128 ? t : t >> 1, w0 = HD == 128 ? 0 : 2 * (t & 1);
@@ -532,9 +532,13 @@ struct Q4Rows {
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
             const uint32_t x = kr[0][w], y = kr[1][w], x8 = x >> 8, y8 = y >> 8;
-            if (w == 0) mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[0][0], q[0][1], bias[0], bias[1]);
-            else mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
-            mma16816(d, w == 0, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
+            if (w == 0) {
+                mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[0][0], q[0][1], bias[0][0], bias[0][1]);
+                mma16816(d, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[1][0], q[1][1], bias[1][0], bias[1][1]);
+            } else {
+                mma16816(c, x & kLo, y & kLo, x & kHi, y & kHi, q[2 * w][0], q[2 * w][1]);
+                mma16816(d, x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, q[2 * w + 1][0], q[2 * w + 1][1]);
+            }
         }
         // lanes past the row's blocks hold zero sums
         sc[0][0] = ((c[0] + d[0]) + (c[1] + d[1])) * (ks[0] * 16777216.0f);

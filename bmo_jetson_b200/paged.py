@@ -16,19 +16,32 @@ synchronise.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+import os
 from typing import Optional
 
 import torch
 
+from . import build as _build
 from .engine import KV_F16, KV_Q4_0, lib
 
 NO_PAGES, TABLE_FULL, NO_ROOM, BAD_INDEX = 1 << 5, 1 << 6, 1 << 7, 1 << 8
-_ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-# the current stream's handle, without making a Stream object (2 us a call)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
-    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+def _load():
+    """The extension module that checks tensors and calls the library (binding/paged_torch.cpp)."""
+    if not os.path.isfile(_build.BINDING) and _build.build_binding() is None:
+        raise ImportError("the torch binding of the paged cache needs torch's and Python's headers to be built")
+    spec = importlib.util.spec_from_file_location("_paged", _build.BINDING)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    L = lib()
+    m.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (L.bmo_k_paged_plan, L.bmo_k_paged_append, L.bmo_k_paged_read,
+                                                             L.bmo_k_paged_attention)))
+    return m
+
+
+_ext = _load()
 
 
 class _Book(ctypes.Structure):
@@ -41,17 +54,6 @@ class _Cache(ctypes.Structure):
                [(n, ctypes.c_int32) for n in ("n_layers", "n_kv_heads", "head_dim", "kv_type")]
 
 
-def _call(device, fn, *args) -> None:
-    """Runs a library call on `device` and its current stream."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _raw_stream(device.index))
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(device.index))
-    if rc != 0:
-        raise RuntimeError(f"{fn.__name__} rc={rc}")
-
-
 def _ints(t: torch.Tensor, name: str, device, numel: Optional[int] = None) -> int:
     """Address of a dense int32 tensor on `device`."""
     if t.dtype is not torch.int32 or t.device != device or not t.is_contiguous():
@@ -59,10 +61,6 @@ def _ints(t: torch.Tensor, name: str, device, numel: Optional[int] = None) -> in
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name}: {numel} entries, got {t.numel()}")
     return t.data_ptr()
-
-
-def _status(t: Optional[torch.Tensor], device) -> Optional[int]:
-    return None if t is None else _ints(t, "status", device, 1)
 
 
 class PageBook:
@@ -80,7 +78,7 @@ class PageBook:
         self._c = _Book(_ints(table, "table", self.device), _ints(lens, "lens", self.device, n_req),
                         _ints(free, "free", self.device), _ints(state, "state", self.device, 4), n_req, max_blocks,
                         free.numel(), self.page_size, self.window)
-        self._ref = ctypes.byref(self._c)
+        self._addr, self._dev = ctypes.addressof(self._c), self.device.index
 
     @classmethod
     def empty(cls, n_req: int, n_pages: int, page_size: int, max_blocks: int, window: int = 0,
@@ -99,13 +97,7 @@ class PageBook:
         offsets [n_req + 1] receive the list of new positions; the new
         lengths and state replace the book's unless lens_out / state_out are
         given.  state[2] != 0 after it: the step was refused, nothing changed."""
-        d, n_req = self.device, self._c.n_req
-        n = slot.numel()
-        _call(
-            d, lib().bmo_k_paged_plan, self._ref, _ints(n_new, "n_new", d, n_req), n, _ints(slot, "slot", d), _ints(pos, "pos", d, n),
-            _ints(req, "req", d, n), _ints(offsets, "offsets", d, n_req + 1),
-            self._c.lens if lens_out is None else _ints(lens_out, "lens_out", d, n_req),
-            self._c.state if state_out is None else _ints(state_out, "state_out", d, 4))
+        _ext.plan(self._addr, self._dev, n_new, slot, pos, req, offsets, lens_out, state_out)
 
 
 class PagedKV:
@@ -136,8 +128,14 @@ class PagedKV:
                 raise ValueError(f"{name}: a contiguous {dtype} tensor of {tuple(shape)} on {book.device}")
         self._c = _Cache(book._c, k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if q4 else None,
                          v_scale.data_ptr() if q4 else None, n_layers, n_kv, head_dim, self.kv_type)
-        self._ref = ctypes.byref(self._c)
-        self._scratch = {}  # by query heads
+        self._addr, self._dev = ctypes.addressof(self._c), book.device.index
+        # for any number of query heads (what is needed grows with the query heads of a key head up to 8)
+        self._scratch_bytes = max(lib().bmo_k_paged_attention_scratch_bytes(self._addr, g * n_kv) for g in (1, 8))
+        if self._scratch_bytes == 0:
+            raise ValueError(f"a cache of {n_kv} heads of {head_dim}, pages of {page_size}")
+        self._scratch = torch.zeros(self._scratch_bytes, dtype=torch.uint8, device=book.device)
+        torch.cuda.current_stream(book.device).synchronize()  # the calls may be on another stream
+        self._scratch_addr = self._scratch.data_ptr()
 
     @classmethod
     def empty(cls, book: PageBook, n_layers: int, n_kv_heads: int, head_dim: int, kv_type: int = KV_F16) -> "PagedKV":
@@ -149,49 +147,18 @@ class PagedKV:
         ks, vs = (torch.zeros(shape + (head_dim // 32,), dtype=torch.float16, device=book.device) for _ in range(2))
         return cls(book, k, v, k_scale=ks, v_scale=vs)
 
-    def _rows(self, t: torch.Tensor, name: str, n: int, dtype, heads: int):
-        """(address, row stride) of [n, heads, head_dim] rows whose heads are dense."""
-        if t.dtype is not dtype or t.device != self.book.device or t.shape != (n, heads, self.head_dim):
-            raise ValueError(f"{name}: {dtype} of {(n, heads, self.head_dim)} on {self.book.device}")
-        s = t.stride()
-        if s[2] != 1 or (heads > 1 and s[1] != self.head_dim):
-            raise ValueError(f"{name}: the heads of a row are contiguous")
-        return t.data_ptr(), s[0]
-
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, slot: torch.Tensor, *,
                pos: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
                q_out: Optional[torch.Tensor] = None, theta: float = 0.0,
                status: Optional[torch.Tensor] = None) -> None:
         """Stores k, v [n, n_kv_heads, head_dim] at slot[n] (bmo_k_paged_append);
         theta > 0 rotates k, and q into q_out, by the positions pos[n]."""
-        n, d = slot.numel(), self.book.device
-        act = _ACT.get(k.dtype)
-        if act is None:
-            raise ValueError(f"k: float32, float16 or bfloat16, got {k.dtype}")
-        kp, ks = self._rows(k, "k", n, k.dtype, self.n_kv_heads)
-        vp, vs = self._rows(v, "v", n, k.dtype, self.n_kv_heads)
-        qp = qs = qop = qos = heads = 0
-        if q is not None:
-            heads = q.shape[1]
-            qp, qs = self._rows(q, "q", n, k.dtype, heads)
-            qop, qos = self._rows(q_out, "q_out", n, k.dtype, heads)
-        _call(d, lib().bmo_k_paged_append, self._ref, layer, n, kp, ks, vp, vs, _ints(slot, "slot", d),
-              None if pos is None else _ints(pos, "pos", d, n), theta, qp or None, qs, heads, qop or None, qos, act,
-              _status(status, d))
+        _ext.append(self._addr, self._dev, layer, k, v, slot, pos, q, q_out, theta, status)
 
     def read(self, layer: int, slot: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,
              status: Optional[torch.Tensor] = None) -> None:
         """Rows at slot[n] as k_out, v_out [n, n_kv_heads, head_dim] (bmo_k_paged_read)."""
-        n, d = slot.numel(), self.book.device
-        act = _ACT.get(k_out.dtype)
-        if act is None:
-            raise ValueError(f"k_out: float32, float16 or bfloat16, got {k_out.dtype}")
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if not t.is_contiguous():
-                raise ValueError(f"{name}: contiguous")
-        kp, _ = self._rows(k_out, "k_out", n, k_out.dtype, self.n_kv_heads)
-        vp, _ = self._rows(v_out, "v_out", n, k_out.dtype, self.n_kv_heads)
-        _call(d, lib().bmo_k_paged_read, self._ref, layer, n, _ints(slot, "slot", d), kp, vp, act, _status(status, d))
+        _ext.read(self._addr, self._dev, layer, slot, k_out, v_out, status)
 
     def attention(self, layer: int, q: torch.Tensor, out: torch.Tensor, *, rows: Optional[torch.Tensor] = None,
                   row_lens: Optional[torch.Tensor] = None, scale: float = 0.0, lse: Optional[torch.Tensor] = None,
@@ -199,26 +166,5 @@ class PagedKV:
         """Attention of q [n, n_heads, head_dim] into out (bmo_k_paged_attention).
         Row i is a token of request rows[i] (default i) that attends to the first
         row_lens[i] positions (default all); lse [n, n_heads] fp32."""
-        n, heads, _ = q.shape
-        d = self.book.device
-        act = _ACT.get(q.dtype)
-        if act is None:
-            raise ValueError(f"q: float32, float16 or bfloat16, got {q.dtype}")
-        qp, qs = self._rows(q, "q", n, q.dtype, heads)
-        op, os_ = self._rows(out, "out", n, q.dtype, heads)
-        lp = None
-        if lse is not None:
-            if lse.dtype is not torch.float32 or lse.shape != (n, heads) or lse.device != d or not lse.is_contiguous():
-                raise ValueError(f"lse: contiguous float32 of {(n, heads)}")
-            lp = lse.data_ptr()
-        sc = self._scratch.get(heads)
-        if sc is None:
-            nbytes = lib().bmo_k_paged_attention_scratch_bytes(self._ref, heads)
-            if nbytes == 0:
-                raise ValueError(f"{heads} query heads over {self.n_kv_heads} key heads of {self.head_dim}")
-            sc = self._scratch[heads] = torch.zeros(nbytes, dtype=torch.uint8, device=d)
-            torch.cuda.current_stream(d).synchronize()  # later calls may be on another stream
-        _call(d, lib().bmo_k_paged_attention, self._ref, layer, n, qp, qs, heads,
-              None if rows is None else _ints(rows, "rows", d, n),
-              None if row_lens is None else _ints(row_lens, "row_lens", d, n), scale, op, os_, lp, act,
-              _status(status, d), sc.data_ptr(), sc.numel())
+        _ext.attention(self._addr, self._dev, layer, q, out, rows, row_lens, scale, lse, status, self._scratch_addr,
+                       self._scratch_bytes)
