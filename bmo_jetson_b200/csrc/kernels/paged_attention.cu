@@ -265,14 +265,14 @@ struct F16Rows {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) inv[nb] = 1.0f;
-#pragma unroll 1
-        for (int h0 = 0; h0 < n_heads; h0 += 4) {
-            float x[4][4];  // four heads' loads in flight
+        {
+            constexpr int h0 = 0;
+            float x[kHeads][4];  // all heads' loads in flight
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < kHeads; ++j)
                 if (h0 + j < n_heads) query_load<ACT, HD>(src, q0 + (h0 + j) * HD, lane, x[j]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kHeads; ++j) {
                 if (h0 + j >= n_heads) continue;
                 const QueryPart p = query_part(x[j]);
                 if (4 * lane < HD) {
@@ -282,7 +282,7 @@ struct F16Rows {
                 }
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
-                    if (h0 == 4 * nb && j == t) inv[nb] = p.inv * qscale;
+                    if (j == 4 * nb + t) inv[nb] = p.inv * qscale;
             }
         }
         __syncwarp();
@@ -705,16 +705,28 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     };
     if (lane < 2) S.whole[2 * warp + lane] = -1;
     if (tid < 2) S.join_n[tid] = 0;
-    uint32_t my_end = 0;  // up to 32 rows: of rows 0..lane, in every warp
+    // Up to 128 rows, in every warp: of rows 0 .. 4 lane + j, so that no warp waits for another.
+    uint32_t my_end[4] = {};
     uint32_t longest = 0;
-    if (a.n_rows <= 32) {
-        my_end = lane < a.n_rows ? row_tiles(lane) : 0;
-        longest = __reduce_max_sync(0xffffffffu, my_end);
+    const bool few = a.n_rows <= 128;
+    if (few) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (4 * lane + j < a.n_rows) my_end[j] = row_tiles(4 * lane + j);
+            longest = max(longest, my_end[j]);
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+#pragma unroll
+        for (int j = 1; j < 4; ++j) my_end[j] += my_end[j - 1];
+        uint32_t before = my_end[3];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t x = __shfl_up_sync(0xffffffffu, my_end, o);
-            if (lane >= o) my_end += x;
+            const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
         }
+        before -= my_end[3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) my_end[j] += before;
     } else {
         const int per_thread = (a.n_rows + kPaThreads - 1) / kPaThreads;
         const int r0 = tid * per_thread, r1 = min(a.n_rows, r0 + per_thread);
@@ -747,8 +759,11 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         __syncthreads();
     }
     if (bad) raise_error(a.status, kErrBadIndex);
-    const bool few = a.n_rows <= 32;
-    auto end_of = [&](int r) { return few ? __shfl_sync(0xffffffffu, my_end, r) : ends[r]; };
+    auto end_of = [&](int r) {
+        if (!few) return ends[r];
+        const uint32_t lo = r & 1 ? my_end[1] : my_end[0], hi = r & 1 ? my_end[3] : my_end[2];
+        return __shfl_sync(0xffffffffu, r & 2 ? hi : lo, r >> 2);
+    };
     const uint32_t total = end_of(a.n_rows - 1) * units;  // below 2^31 (checked by the entry point)
     const uint32_t per = max(1u, (total + gridDim.x * kPaWarps - 1) / (gridDim.x * kPaWarps));
     const uint32_t me = blockIdx.x * kPaWarps + warp;
@@ -792,7 +807,9 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         } else {
             const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
             if (few) {
-                row = __popc(__ballot_sync(0xffffffffu, lane < a.n_rows && my_end <= q));
+                row = 4 * __popc(__ballot_sync(0xffffffffu, my_end[3] <= q));  // below 4 * 32: q lies before the last row's end
+#pragma unroll
+                for (int j = 0; j < 3; ++j) row += __shfl_sync(0xffffffffu, my_end[j], row >> 2) <= q ? 1 : 0;
             } else {
                 int lo = 0, hi = a.n_rows - 1;
 #pragma unroll 1
@@ -1208,7 +1225,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const int n = S.join_n[joining], c0 = S.join_c0[joining];
         const Head h = S.join_head[joining];
         const int cols = h.heads * (HD / 4);                   // of 4 elements
-        const int parts = min(max(1, kPaThreads / cols), n);   // <= 8
+        const bool direct = n <= kJoinBatch;                   // one round of loads: no parts to put together
+        const int parts = direct ? 1 : min(max(1, kPaThreads / cols), n);  // <= 8
         const int part = tid / cols;
         if (tid < Smem::kPieces) S.whole[tid] = tid < parts ? (tid == 0 ? 1 : 0) | (tid == parts - 1 ? 2 : 0) : -1;
         if (tid == 0) S.head[0] = h;
@@ -1246,9 +1264,24 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         o.x += w * po[i].x, o.y += w * po[i].y, o.z += w * po[i].z, o.w += w * po[i].w;
                     }
                 }
-                *reinterpret_cast<float4 *>(&S.o[part][4 * c]) = o;
-                if (c % (HD / 4) == 0) S.m[part][hh] = top, S.l[part][hh] = l;
+                if (direct) {
+                    const float f = inverse_of(l);
+                    const long long out0 = h.row * a.out_stride + static_cast<long long>(h.head0) * HD + 4 * c;
+                    act_store<ACT>(a.out, out0, o.x * f);
+                    act_store<ACT>(a.out, out0 + 1, o.y * f);
+                    act_store<ACT>(a.out, out0 + 2, o.z * f);
+                    act_store<ACT>(a.out, out0 + 3, o.w * f);
+                    if (a.lse && c % (HD / 4) == 0)
+                        a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + hh] = lse_of(top, l);
+                } else {
+                    *reinterpret_cast<float4 *>(&S.o[part][4 * c]) = o;
+                    if (c % (HD / 4) == 0) S.m[part][hh] = top, S.l[part][hh] = l;
+                }
             }
+        }
+        if (direct) {
+            if (joining == 1) return;
+            if (tid < Smem::kPieces) S.whole[tid] = -1;
         }
         __syncthreads();
     }
