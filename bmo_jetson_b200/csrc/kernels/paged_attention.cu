@@ -666,6 +666,8 @@ struct Head {
     uint32_t first, n_tiles;   // its tiles on the line
 };
 
+constexpr int kMaxCluster = 8;  // no more than the slots of a CTA's pieces
+
 // Two pieces a warp: one that began before its part of the line, one that goes on after it.
 template <int HD, int NH>
 struct PaSmem {
@@ -674,6 +676,8 @@ struct PaSmem {
     float bm[kPaWarps][NH], bl[kPaWarps][NH];
     float m[kPieces][NH], l[kPieces][NH];
     float o[kPieces][NH * HD];
+    float cluster_m[kMaxCluster][NH], cluster_l[kMaxCluster][NH], cluster_o[kMaxCluster][NH * HD];  // of the cluster's CTAs, in its first
+    float weight[kPieces][NH], sum_m[NH], sum_l[NH];  // of the pieces that are joined
     Head head[kPieces];
     int whole[kPieces];  // -1: no piece; bit 0: begins at the head's first tile, bit 1: ends at its last
     int scan[kPaWarps], longest[kPaWarps];
@@ -687,7 +691,19 @@ __device__ __forceinline__ float lse_of(float m, float l) { return l == 0.0f ? -
 __device__ __forceinline__ float inverse_of(float l) { return l == 0.0f ? 0.0f : __frcp_rn(l); }
 
 constexpr uint32_t kJoinTiles = 4;
+constexpr int kClusterTiles = 3;  // most tiles of a warp
 constexpr int kJoinBatch = 16;  // pieces requested at a time
+
+// Store to the same variable of the cluster's first CTA.
+__device__ __forceinline__ void remote_store(float *p, float x) {
+    uint32_t to;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(to) : "r"(smem_addr(p)));
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(x) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // Release of the CTA's earlier writes (ordered by a barrier before it) and acquire of the others'.
 __device__ __forceinline__ int arrive(int *p) {
@@ -739,13 +755,24 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const int start = a.window > 0 ? max(0, len - a.window) : 0;
         return len > start ? (len + kTile - 1) / kTile - start / kTile + R::kHeadCost : 0;
     };
+    // A cluster a head (a.cluster CTAs, chosen by the launcher) or a line of tiles over all warps.
+    const int cluster = a.cluster;
+    int rank = 0, cluster_row = 0;
+    uint32_t cluster_span = 0;
+    if (cluster > 1) {
+        cluster_arrive_relaxed();  // waited for before another CTA's shared memory is written
+        rank = blockIdx.x % cluster;
+        cluster_row = pa_div(blockIdx.x / cluster, a.units);
+        cluster_span = row_tiles(cluster_row);
+    }
     if (lane < 2) S.whole[2 * warp + lane] = -1;
     if (tid < 2) S.join_n[tid] = 0;
     // Up to 128 rows, in every warp: of rows 0 .. 4 lane + j, so that no warp waits for another.
     uint32_t my_end[4] = {};
     uint32_t longest = 0;
     const bool few = a.n_rows <= 128;
-    if (few) {
+    if (cluster > 1) {
+    } else if (few) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (4 * lane + j < a.n_rows) my_end[j] = row_tiles(4 * lane + j);
@@ -800,27 +827,40 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const uint32_t lo = r & 1 ? my_end[1] : my_end[0], hi = r & 1 ? my_end[3] : my_end[2];
         return __shfl_sync(0xffffffffu, r & 2 ? hi : lo, r >> 2);
     };
-    const uint32_t total = end_of(a.n_rows - 1) * units;  // below 2^31 (checked by the entry point)
-    const uint32_t per = max(1u, (total + gridDim.x * kPaWarps - 1) / (gridDim.x * kPaWarps));
-    const uint32_t me = blockIdx.x * kPaWarps + warp;
-    uint32_t u = static_cast<uint32_t>(min(static_cast<unsigned long long>(total), static_cast<unsigned long long>(me) * per));
-    uint32_t u_end = u + min(per, total - u);
-    // Few, short heads: a head a CTA, so that none waits for other CTAs.  Joining
-    // through global memory takes about as long as kJoinTiles tiles one after another.
-    const uint32_t warp_tiles = (longest + kPaWarps - 1) / kPaWarps;
-    const bool apart = static_cast<uint32_t>(a.n_rows) * units <= gridDim.x && warp_tiles <= per + kJoinTiles;
-    if (apart) u = blockIdx.x, u_end = blockIdx.x < a.n_rows * units ? u + 1 : u;
+    uint32_t per = 0, u, u_end;
+    bool apart = cluster > 1;
+    if (apart) {
+        u = blockIdx.x / cluster, u_end = u + 1;
+        if (cluster_span == 0 && rank == 0) {  // a row without a position
+            const int unit = u - cluster_row * units, kh = pa_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
+            const int h0 = kh * group + chunk * NH, n = min(NH, group - chunk * NH);
+            for (int i = tid; i < n * HD; i += kPaThreads)
+                act_store<ACT>(a.out, cluster_row * a.out_stride + static_cast<long long>(h0) * HD + i, 0.0f);
+            if (a.lse && tid < n) a.lse[static_cast<long long>(cluster_row) * a.n_heads + h0 + tid] = -INFINITY;
+        }
+    } else {
+        const uint32_t total = end_of(a.n_rows - 1) * units;  // below 2^31 (checked by the entry point)
+        per = max(1u, (total + gridDim.x * kPaWarps - 1) / (gridDim.x * kPaWarps));
+        const uint32_t me = blockIdx.x * kPaWarps + warp;
+        u = static_cast<uint32_t>(min(static_cast<unsigned long long>(total), static_cast<unsigned long long>(me) * per));
+        u_end = u + min(per, total - u);
+        // Few, short heads: a head a CTA, so that none waits for other CTAs.  Joining
+        // through global memory takes about as long as kJoinTiles tiles one after another.
+        const uint32_t warp_tiles = (longest + kPaWarps - 1) / kPaWarps;
+        apart = static_cast<uint32_t>(a.n_rows) * units <= gridDim.x && warp_tiles <= per + kJoinTiles;
+        if (apart) u = blockIdx.x, u_end = blockIdx.x < a.n_rows * units ? u + 1 : u;
 
-    // rows without a position
+        // rows without a position
 #pragma unroll 1
-    for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
-        const uint32_t e0 = end_of(max(r - 1, 0)), e1 = end_of(r);
-        if (e1 != (r ? e0 : 0)) continue;
+        for (int r = blockIdx.x; r < a.n_rows; r += gridDim.x) {
+            const uint32_t e0 = end_of(max(r - 1, 0)), e1 = end_of(r);
+            if (e1 != (r ? e0 : 0)) continue;
 #pragma unroll 1
-        for (int i = tid; i < a.n_heads * HD; i += kPaThreads) act_store<ACT>(a.out, r * a.out_stride + i, 0.0f);
-        if (a.lse)
+            for (int i = tid; i < a.n_heads * HD; i += kPaThreads) act_store<ACT>(a.out, r * a.out_stride + i, 0.0f);
+            if (a.lse)
 #pragma unroll 1
-            for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
+                for (int h = tid; h < a.n_heads; h += kPaThreads) a.lse[static_cast<long long>(r) * a.n_heads + h] = -INFINITY;
+        }
     }
 
     R R_(a, ring + warp * R::kRing, lane);
@@ -835,11 +875,15 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             unit = u - row * units;
             row0 = 0;
             u = u_end;
-            const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
-            span = row_end - (row ? row_prev : 0);
+            if (cluster > 1) {
+                span = cluster_span;
+            } else {
+                const uint32_t row_end = end_of(row), row_prev = end_of(max(row - 1, 0));
+                span = row_end - (row ? row_prev : 0);
+            }
             if (!span) break;
-            const uint32_t n = (span - R::kHeadCost + kPaWarps - 1) / kPaWarps;
-            from = min(warp * n + R::kHeadCost, span), to = min(from + n, span);
+            const uint32_t warps = cluster * kPaWarps, n = (span - R::kHeadCost + warps - 1) / warps;
+            from = min((rank * kPaWarps + warp) * n + R::kHeadCost, span), to = min(from + n, span);
         } else {
             const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
             if (few) {
@@ -1189,7 +1233,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     // global memory; the last CTA to arrive puts all its parts back into the
     // slots and comes through here once more.
     constexpr int kPieceFloats = pa_piece_floats<R>;
-    int joining = -1;  // 0, 1: the slots hold that head's parts
+    int joining = -1;  // 0, 1: the slots hold that head's parts; 2: those of the cluster's CTAs
+    if (cluster > 1) cluster_wait();
     for (;;) {
         const int w = lane < Smem::kPieces ? S.whole[lane] : -1;
         uint32_t left = __ballot_sync(0xffffffffu, w >= 0);
@@ -1206,24 +1251,43 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             const bool begins = begin_bits >> first & 1, complete = begins && ends_at;
             const Head h = S.head[first];
             float *dst = a.part + (2 * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
+            const bool second = joining == 2;
+            const uint32_t pieces = all & (0xffffffffu >> (31 - last)) & (0xffffffffu << first);
+            if (4 * warp < NH) {  // what each piece counts: lane % 8 a piece, lane / 8 a head of four
+                static_assert(Smem::kPieces == 8, "a head's pieces are 8 lanes'");
+                const int k = lane & 7, hh = min(4 * warp + (lane >> 3), NH - 1);
+                const bool there = pieces >> k & 1;
+                const float m = there ? (second ? S.cluster_m[k][hh] : S.m[k][hh]) : -INFINITY;
+                float top = m;
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float f = m == top ? 1.0f : ex2(m - top);
+                float l = there ? f * (second ? S.cluster_l[k][hh] : S.l[k][hh]) : 0.0f;
+#pragma unroll
+                for (int d = 1; d < 8; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                S.weight[k][hh] = f;
+                if (k == 0) S.sum_m[hh] = top, S.sum_l[hh] = l;
+            }
+            __syncthreads();
+            const float *o = second ? S.cluster_o[0] : S.o[0];
 #pragma unroll 1
             for (int e = tid; e < h.heads * HD; e += kPaThreads) {
                 const int hh = e / HD;
-                float top = -INFINITY, l = 0.0f, x = 0.0f;
-#pragma unroll 1
-                for (int k = first; k <= last; ++k)
-                    if (all >> k & 1) top = fmaxf(top, S.m[k][hh]);
-#pragma unroll 1
-                for (int k = first; k <= last; ++k)
-                    if (all >> k & 1) {
-                        const float f = S.m[k][hh] == top ? 1.0f : ex2(S.m[k][hh] - top);
-                        l += f * S.l[k][hh];
-                        x += f * S.o[k][e];
-                    }
+                float x = 0.0f;
+#pragma unroll
+                for (int k = 0; k < Smem::kPieces; ++k)
+                    if (pieces >> k & 1) x += S.weight[k][hh] * o[k * NH * HD + e];
+                const float top = S.sum_m[hh], l = S.sum_l[hh];
                 if (complete) {
                     act_store<ACT>(a.out, h.row * a.out_stride + static_cast<long long>(h.head0) * HD + e, x * inverse_of(l));
                     if (a.lse && e % HD == 0)
                         a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + hh] = lse_of(top, l);
+                } else if (cluster > 1) {
+                    remote_store(&S.cluster_o[rank][e], x);
+                    if (e % HD == 0) {
+                        remote_store(&S.cluster_m[rank][hh], top);
+                        remote_store(&S.cluster_l[rank][hh], l);
+                    }
                 } else {
                     __stcg(dst + e, x);
                     if (e % HD == 0) {
@@ -1232,7 +1296,24 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                     }
                 }
             }
+            __syncthreads();
             if (!complete) open[begins ? 1 : 0] = first;
+        }
+        if (joining == 2) return;
+        if (cluster > 1) {
+            __syncwarp();
+            cluster_sync();
+            // the head's CTAs that had tiles: the first cluster_parts, all of them with one piece
+            const uint32_t tiles = cluster_span ? cluster_span - R::kHeadCost : 0, warps = cluster * kPaWarps;
+            const uint32_t cta_tiles = (tiles + warps - 1) / warps * kPaWarps;
+            const int cluster_parts = tiles > cta_tiles ? (tiles + cta_tiles - 1) / cta_tiles : 1;
+            if (rank || cluster_parts == 1) return;
+            if (tid < Smem::kPieces)
+                S.whole[tid] = tid < cluster_parts ? (tid == 0 ? 1 : 0) | (tid == cluster_parts - 1 ? 2 : 0) : -1;
+            if (tid == 0) S.head[0] = S.head[1];  // its own first piece, which begins the head
+            __syncthreads();
+            joining = 2;
+            continue;
         }
         if (joining < 0) {
             if (open[0] < 0 && open[1] < 0) return;
@@ -1260,8 +1341,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         const int n = S.join_n[joining], c0 = S.join_c0[joining];
         const Head h = S.join_head[joining];
         const int cols = h.heads * (HD / 4);                   // of 4 elements
-        const bool direct = n <= kJoinBatch;                   // one round of loads: no parts to put together
-        const int parts = direct ? 1 : min(max(1, kPaThreads / cols), n);  // <= 8
+        const int parts = min(max(1, kPaThreads / cols), n);  // <= 8
         const int part = tid / cols;
         if (tid < Smem::kPieces) S.whole[tid] = tid < parts ? (tid == 0 ? 1 : 0) | (tid == parts - 1 ? 2 : 0) : -1;
         if (tid == 0) S.head[0] = h;
@@ -1299,24 +1379,9 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                         o.x += w * po[i].x, o.y += w * po[i].y, o.z += w * po[i].z, o.w += w * po[i].w;
                     }
                 }
-                if (direct) {
-                    const float f = inverse_of(l);
-                    const long long out0 = h.row * a.out_stride + static_cast<long long>(h.head0) * HD + 4 * c;
-                    act_store<ACT>(a.out, out0, o.x * f);
-                    act_store<ACT>(a.out, out0 + 1, o.y * f);
-                    act_store<ACT>(a.out, out0 + 2, o.z * f);
-                    act_store<ACT>(a.out, out0 + 3, o.w * f);
-                    if (a.lse && c % (HD / 4) == 0)
-                        a.lse[static_cast<long long>(h.row) * a.n_heads + h.head0 + hh] = lse_of(top, l);
-                } else {
-                    *reinterpret_cast<float4 *>(&S.o[part][4 * c]) = o;
-                    if (c % (HD / 4) == 0) S.m[part][hh] = top, S.l[part][hh] = l;
-                }
+                *reinterpret_cast<float4 *>(&S.o[part][4 * c]) = o;
+                if (c % (HD / 4) == 0) S.m[part][hh] = top, S.l[part][hh] = l;
             }
-        }
-        if (direct) {
-            if (joining == 1) return;
-            if (tid < Smem::kPieces) S.whole[tid] = -1;
         }
         __syncthreads();
     }
@@ -1363,8 +1428,33 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     a.units = make_fast_div(a.n_kv_heads * chunks);
     a.cnt = static_cast<int *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
-    paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * a.n_rows, s>>>(a);
-    return cudaGetLastError();
+    const size_t smem = kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * a.n_rows;
+    // Few heads of bounded length: a cluster a head, whose CTAs join through
+    // shared memory instead of global memory (32 heads of 512 positions: 8.4 us
+    // against 9.7).  As many CTAs as give a warp a tile, if 3 tiles a warp are enough and the
+    // clusters find room at once: with all resident CTAs in clusters, 74 heads in
+    // clusters of 4 took 19 us, not 11.
+    const long long heads = static_cast<long long>(a.n_rows) * a.units.d;
+    const long long table = a.max_blocks * static_cast<long long>(a.page.d);
+    const long long tiles = (a.window > 0 && a.window < table ? a.window : table) / (16 * R::kSub);
+    a.cluster = 1;
+    while (a.cluster < kMaxCluster && tiles > kPaWarps * a.cluster && heads * 2 * a.cluster * 5 <= grid * 3) a.cluster *= 2;
+    if (tiles > kPaWarps * a.cluster * kClusterTiles || (a.cluster == 2 && R::kMinCtas < 3)) a.cluster = 1;
+    if (a.cluster == 1) {
+        paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, smem, s>>>(a);
+        return cudaGetLastError();
+    }
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = a.cluster, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(heads * a.cluster));
+    cfg.blockDim = dim3(kPaThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_attn_kernel<R, ACT, kAligned>, a);
 }
 
 template <class R>

@@ -73,6 +73,7 @@ struct PagedAttnArgs {
     int n_rows, n_heads, n_kv_heads;
     int group;                       // query heads of a key head (this and the next set by the launcher)
     FastDiv units, chunks;           // units of a row, of a key head
+    int cluster;                     // > 1: CTAs of a cluster that takes one head
     float qscale;                    // score scale * log2(e)
     int *status;
     // split rows: two partial results per CTA, one arrival counter per CTA

@@ -200,6 +200,18 @@ def test_attention_many_rows():
 
 
 @pytest.mark.parametrize("kv", ["f16", "q4_0"])
+@pytest.mark.parametrize("rows,kv_heads,longest", [(1, 1, 3000), (1, 32, 600), (13, 4, 90), (27, 4, 700), (55, 4, 300),
+                                                   (75, 2, 40), (200, 2, 70), (40, 16, 130)])
+def test_attention_shares_of_the_gpu(kv, rows, kv_heads, longest):
+    """Numbers of heads and lengths at which a head is given a cluster of 8, 4 or
+    2 CTAs, a CTA, or a part of the line of tiles."""
+    lens = np.random.default_rng(rows).integers(0, longest + 1, rows)
+    lens[0] = longest
+    check(Case(lens, kv_heads, 64, 16, kv, seed=rows), kv_heads)
+    check(Case(lens, kv_heads, 128, 20, kv, seed=rows + 1, window=longest // 2 + 1), kv_heads)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4_0"])
 def test_attention_several_tokens_of_a_request(kv):
     c = Case([50, 7, 130], 2, 128, 16, kv, window=64)
     check(c, 2, reqs=[2, 2, 2, 0, 1, 0, 2], lens=[128, 129, 130, 50, 0, 49, 128])
