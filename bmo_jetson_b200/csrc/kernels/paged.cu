@@ -24,10 +24,6 @@ FastDiv make_fast_div(uint32_t d) {
 
 namespace {
 
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f) {
-    return (__umulhi(n, f.mul) + n) >> f.shift;
-}
-
 // ---- plan ----
 //
 // Request r of length L with n new positions grows to L' = L + n (0 when it
@@ -43,7 +39,9 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f) {
 // launch (kPlanOneCta).  Where no request has more than kFew of anything, the usual
 // step, each thread writes what its request has.  Otherwise the thread that writes
 // an entry searches the prefix sums for its request, so entries are written
-// side by side whatever the requests' lengths are, kPlanBatch of a thread's in flight.
+// side by side whatever the requests' lengths are, kPlanBatch of a thread's in
+// flight.  64 requests of one position: 3.8 us, of which about 2 are the launch; 61
+// requests of up to 2999 new positions, both kernels: 11.9 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanOneCta = 8192;
 constexpr int kFew = 2;
@@ -425,8 +423,9 @@ using Act = typename ActOf<ACT>::type;
 // token needs each of the token's angles once, two a lane, in registers: cos
 // and sin in double, rounded to fp32 as the exact-order step's table.  The rows' loads are
 // requested kAppendRows at a time, the first ones before the angles are computed.
-// Warps take few rows each when there are few tokens (launch_paged_append), all of
-// a token's when there are many.
+// Warps take few rows each when there are few tokens (share_rows), all of a
+// token's when there are many.  23993 tokens of 32 + 2 x 8 rows of 128 in bf16
+// (590 MB): 103 us, 5.7 TB/s; one token of 96 rows: 3.3 us; 64 tokens into Q4_0: 5.7 us.
 constexpr int kAppendThreads = 128;
 constexpr int kAppendRows = 8;  // row slots of a lane in flight
 
@@ -604,7 +603,8 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(const __grid_constan
     }
 }
 
-// Rows of a warp: one round of loads, or more rounds once the warps are many (32 an SM keep their loads in flight).
+// Rows of a warp: one round of loads, or more rounds once the warps are many (64 an SM;
+// 16, 32 and 128 measured the same for the append and 0 to 2 us of 23 more for the read).
 struct RowShare {
     int part_rows, parts;
     unsigned grid;

@@ -9,30 +9,40 @@
 //
 // Every key and value is read once and used for a few query heads, so the
 // kernel is bound by memory; what has to be avoided is anything that keeps
-// loads from being in flight.  Rows go from global memory straight into the
-// registers in which the matrix instruction (mma.sync m16n8k16) takes its A
-// operand: the contraction runs over a permuted index, so a lane's 16
-// consecutive bytes are its fragment, and nothing is staged, transposed or
-// synchronised.  (tcgen05.mma would need the rows in shared memory in its
-// canonical layout, and 128 rows of which a decode step fills 2.)
+// loads from being in flight.  Both products are mma.sync m16n8k16 with the rows
+// as its A operand.  (tcgen05.mma would need them in shared memory in its
+// canonical layout, and 128 rows of B's side, of which a decode step fills 2.)
 //   scores: A = 16 positions x 16 elements of K, B = q
 //   values: A = 16 elements x 16 positions of V^T, B = the weights
 // B has 8 columns.  An fp32 factor x takes two of them, hi = fp16(x) and
 // lo = fp16(x - hi), so products with fp16 keys and values keep about 22 bits
-// (x is brought into fp16's range by a power of two first) and are summed in
-// fp32 by the tensor core.
-//   fp16 cache: columns 2t, 2t + 1 are head t of a group of 4 (or 2 x 4).
-//   Q4_0 cache: columns 2t, 2t + 1 are block t of head_dim: q is masked to the
-//   block, so the score comes out as one integer-code sum per block, which
-//   the block's scale multiplies in fp32; and the weight of a value's block is
-//   p times that block's scale.  Codes n - 8 are exact in fp16.
+// (x is brought into fp16's range by a power of two first); the tensor core
+// sums a tile in fp32, and tiles are added by fp32 additions.
+//
+// fp16 cache: columns 2t, 2t + 1 are head t of a group of 4 (or of 2 x 4).  The
+// contraction runs over a permuted index, so that 16 consecutive bytes of a
+// row are a lane's fragment: rows go from global memory straight into
+// registers, and nothing is staged.  64 sessions of up to 3000 positions, 32
+// heads of 128 (1.64 GB): 259 us, 6.3 TB/s, 0.98 of the measured copy.
+//
+// Q4_0 cache: columns 2t, 2t + 1 are block t of head_dim.  q is masked to the
+// block, so the score comes out as one sum over codes a block, which the
+// block's scale multiplies in fp32; and the weight of a value's block is p times that
+// block's scale.  Unpacking costs two instructions per two codes, on
+// half-rate pipes, and makes the kernel bound by instructions: registers go to the
+// arithmetic, and rows arrive in a ring in shared memory by asynchronous copies.  64
+// sessions of 1500 positions (442 MB): 100 us, 4.4 TB/s, the issue slots 60% and the
+// ALU pipe 51% busy; with the rows in registers 152 us.
 //
 // Work: a row's window is cut into tiles of kTile positions; (row, key head,
 // tile) in that order is a line of tiles of which every warp takes an equal,
 // contiguous part.  A head that lies within one warp's part is written at once.
 // Otherwise its pieces are joined in shared memory among the CTA's warps,
 // then through global memory by the last CTA to arrive, in the order of the
-// line, so the result does not depend on the order of arrival.
+// line, so the result does not depend on the order of arrival.  Nothing waits for
+// another CTA.  A call of few heads is bound by latency instead (its code
+// is fetched cold, then loads, two barriers and the join follow one another): there a head gets a
+// CTA or a cluster of CTAs of its own, chosen in pa_launch.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -53,8 +63,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 // of its two parts is exact to 2^-25 of the largest weight's 2^7.
 constexpr float kSlack = 8.0f, kHead = 7.0f;
 
-__device__ __forceinline__ uint32_t pa_div(uint32_t n, const FastDiv &f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -66,16 +74,6 @@ __device__ __forceinline__ uint4 ldg_stream16(const void *p) {
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
         : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const void *p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint32_t ldg_stream4(const void *p) {
-    uint32_t v;
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
 
@@ -762,7 +760,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     if (cluster > 1) {
         cluster_arrive_relaxed();  // waited for before another CTA's shared memory is written
         rank = blockIdx.x % cluster;
-        cluster_row = pa_div(blockIdx.x / cluster, a.units);
+        cluster_row = fast_div(blockIdx.x / cluster, a.units);
         cluster_span = row_tiles(cluster_row);
     }
     if (lane < 2) S.whole[2 * warp + lane] = -1;
@@ -832,7 +830,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
     if (apart) {
         u = blockIdx.x / cluster, u_end = u + 1;
         if (cluster_span == 0 && rank == 0) {  // a row without a position
-            const int unit = u - cluster_row * units, kh = pa_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
+            const int unit = u - cluster_row * units, kh = fast_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
             const int h0 = kh * group + chunk * NH, n = min(NH, group - chunk * NH);
             for (int i = tid; i < n * HD; i += kPaThreads)
                 act_store<ACT>(a.out, cluster_row * a.out_stride + static_cast<long long>(h0) * HD + i, 0.0f);
@@ -871,7 +869,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         int row;
         uint32_t row0, span, unit, from, to;  // [0, kHeadCost) of a head stands for its other costs, then come its tiles
         if (apart) {
-            row = pa_div(u, a.units);
+            row = fast_div(u, a.units);
             unit = u - row * units;
             row0 = 0;
             u = u_end;
@@ -885,7 +883,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             const uint32_t warps = cluster * kPaWarps, n = (span - R::kHeadCost + warps - 1) / warps;
             from = min((rank * kPaWarps + warp) * n + R::kHeadCost, span), to = min(from + n, span);
         } else {
-            const uint32_t q = pa_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
+            const uint32_t q = fast_div(u, a.units);  // row tiles before u's: u / units lies in [row0, end)
             if (few) {
                 row = 4 * __popc(__ballot_sync(0xffffffffu, my_end[3] <= q));  // below 4 * 32: q lies before the last row's end
 #pragma unroll
@@ -913,7 +911,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         hd.row = row;
         hd.n_tiles = span - R::kHeadCost;
         hd.first = row0 * units + unit * span + R::kHeadCost;
-        const int kh = pa_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
+        const int kh = fast_div(unit, a.chunks), chunk = unit - kh * a.chunks.d;
         hd.head0 = kh * group + chunk * NH;
         hd.heads = min(NH, group - chunk * NH);
         int req;
@@ -933,14 +931,14 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         auto refill = [&](int at) {
             walk = at;
             if constexpr (kAligned) {
-                const int p = at + 16 * lane, b = pa_div(p, a.page);
+                const int p = at + 16 * lane, b = fast_div(p, a.page);
                 const uint32_t r = first_row(b);
                 entry = r == kNoPage ? r : r + (p - b * a.page.d);
             } else {
                 entry = first_row(at + lane);
             }
         };
-        if (R::kRing > 0 || !kAligned) refill(kAligned ? pbase + tile0 * kTile : pa_div(max(start, pbase + tile0 * kTile), a.page));
+        if (R::kRing > 0 || !kAligned) refill(kAligned ? pbase + tile0 * kTile : fast_div(max(start, pbase + tile0 * kTile), a.page));
         float o[NB][kO][4], m[NB], l[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -985,8 +983,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 // lane i finds the row of the tile's position i (mod 16), the others get it from there
                 const int p = p0 + (lane & (kTile - 1));
                 const bool in = p >= start && p < len;
-                const int b = pa_div(p, a.page);
-                if (static_cast<int>(pa_div(min(p0 + kTile, len) - 1, a.page)) >= walk + 32) refill(pa_div(max(p0, start), a.page));
+                const int b = fast_div(p, a.page);
+                if (static_cast<int>(fast_div(min(p0 + kTile, len) - 1, a.page)) >= walk + 32) refill(fast_div(max(p0, start), a.page));
                 const uint32_t base = __shfl_sync(0xffffffffu, entry, in ? b - walk : 0);
                 const bool ok = in && base != kNoPage;
                 bad |= in && !ok;
@@ -1061,7 +1059,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         if constexpr (R::kRing == 0) {
             // Entries [b0, b0 + 32) of the block table, one a lane, and the next tile's
             // block and place in it.  (Rows found as for the other loop measured 270 us against 259.)
-            int block = pa_div(pbase + tile0 * kTile, a.page), b0 = block;
+            int block = fast_div(pbase + tile0 * kTile, a.page), b0 = block;
             uint32_t offset = pbase + tile0 * kTile - block * a.page.d;
             auto entries = [&] { return b0 + lane < a.max_blocks ? table[b0 + lane] : -1; };
             int entry = kAligned ? entries() : 0;

@@ -20,6 +20,9 @@ struct FastDiv {
     uint32_t d, mul, shift;
 };
 FastDiv make_fast_div(uint32_t d);
+#ifdef __CUDACC__
+__device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv &f) { return (__umulhi(n, f.mul) + n) >> f.shift; }
+#endif
 
 struct PagedPlanArgs {
     bmo_page_book book;
