@@ -77,7 +77,6 @@ __device__ __forceinline__ uint4 ldg_stream16(const void *p) {
     return v;
 }
 
-// c += A B, and c = A B + start.
 // Shared memory by 32-bit address.
 __device__ __forceinline__ uint4 lds16(uint32_t p) {
     uint4 v;
@@ -112,18 +111,16 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1, float start0, float start1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%10, %11, %10, %11};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(start0), "f"(start1));
-}
 // c = A B if first, else c += A B (first known at compile time).
 __device__ __forceinline__ void mma16816(float (&c)[4], bool first, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    if (first) mma16816(c, a0, a1, a2, a3, b0, b1, 0.0f, 0.0f);
-    else mma16816(c, a0, a1, a2, a3, b0, b1);
+    if (first)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%10, %10, %10, %10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        mma16816(c, a0, a1, a2, a3, b0, b1);
 }
 
 __device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
@@ -189,8 +186,8 @@ __device__ __forceinline__ void range_factor(float amax, float &mul, float &inv)
     inv = __int_as_float((ex - 10) << 23);
 }
 
-// 4 elements of a query head, split: times `weight` and the power of two that
-// brings the head into fp16's range; inv: that power's inverse.
+// 4 elements of a query head, split: times the power of two that brings the
+// head into fp16's range; inv: that power's inverse.
 struct QueryPart {
     __half hi[4], lo[4];
     float inv;
@@ -200,12 +197,11 @@ __device__ __forceinline__ void query_load(const void *src, long long at, int la
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = 4 * lane < HD ? act_load<ACT>(src, at + 4 * lane + i) : 0.0f;
 }
-__device__ __forceinline__ QueryPart query_part(const float (&x)[4], float weight = 1.0f) {
+__device__ __forceinline__ QueryPart query_part(const float (&x)[4]) {
     const float amax = warp_max(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
     QueryPart p;
     float mul;
     range_factor(amax, mul, p.inv);
-    mul *= weight;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float y = x[i] * mul;
@@ -400,36 +396,24 @@ struct Q4Rows {
     // where lanes that hold other blocks' codes read zeros.
     uint4 q[NB == 1 ? kKW : 1];
     uint32_t q_at, q_step;
-    float inv[NB], bias[NB][2][2];  // [chain][column]
+    float inv[NB];
     float vlim, vinv;  // power of two that bounds the value scales seen so far, and its inverse
     float vs[kSub][2];
-    // B fragments of the query: a lane splits 4 elements, elements 16..31 of a
-    // block divided by 16, and puts them where the lanes that hold their codes
-    // find their fragments as 16-byte words: buf[block][hi, lo][16] (pairs of halves).
+    // B fragments of the queries: a lane splits 4 elements of each and puts them
+    // where the lanes that hold their codes find their fragments as 16-byte
+    // words: buf[head][block][hi, lo][16] (pairs of halves).
     template <int ACT>
     __device__ __forceinline__ void load_q(const void *src, long long q0, int n_heads, float qscale, float *buf, int lane) {
         const int g = lane >> 2, t = lane & 3;
         const int i = lane & 7;  // elements 4i.. of block lane / 8
-        const float weight = i < 4 ? 1.0f : 16.0f;
         float e[NB][4];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)  // a head past n_heads: the first again, not used
             query_load<ACT, HD>(src, q0 + (nb < n_heads ? nb : 0) * HD, lane, e[nb]);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const QueryPart x = query_part(e[nb], i < 4 ? 1.0f : 0.0625f);
+            const QueryPart x = query_part(e[nb]);
             inv[nb] = x.inv * qscale;
-            // sums of the elements that each of the two chains of products takes
-            float sum[4] = {weight * (__half2float(x.hi[0]) + __half2float(x.hi[2])), weight * (__half2float(x.lo[0]) + __half2float(x.lo[2])),
-                            weight * (__half2float(x.hi[1]) + __half2float(x.hi[3])), weight * (__half2float(x.lo[1]) + __half2float(x.lo[3]))};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int d = 1; d < 8; d <<= 1) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], d);
-                // columns 2t, 2t + 1 start at -8 2^-24 sum q of block t
-                const float of_t = __shfl_sync(0xffffffffu, sum[j], (8 * t) & 31);
-                bias[nb][j / 2][j % 2] = t < kBlocks ? -4.76837158203125e-07f * of_t : 0.0f;
-            }
             if (4 * lane < HD) {
                 // word 4 (i % 4): codes of bytes 4 (i % 4).. : elements 0, 2 then 1, 3; low nibbles before high ones
                 uint32_t *dst = reinterpret_cast<uint32_t *>(buf + nb * HD) + (lane >> 3) * 32 + 4 * (i & 3) + (i >> 2);
@@ -441,11 +425,13 @@ struct Q4Rows {
         // lane t holds bytes 4 w.. of block blk, w in [w0, w0 + kKW); column pair g / 2 is block g / 2
         const int blk = HD == 128 ? t : t >> 1, w0 = HD == 128 ? 0 : 2 * (t & 1);
         const bool mine = (g >> 1) == blk;
-        q_at = mine ? smem_addr(buf) + 4 * (blk * 32 + (g & 1) * 16) + 16 * w0 : ring + 3 * kStage;
-        q_step = mine ? 4 * HD : 0;
+        const uint32_t at = smem_addr(buf) + 4 * (blk * 32 + (g & 1) * 16) + 16 * w0;
         if constexpr (NB == 1) {
 #pragma unroll
-            for (int w = 0; w < kKW; ++w) q[w] = lds16(q_at + 16 * w);
+            for (int w = 0; w < kKW; ++w) q[w] = mine ? lds16(at + 16 * w) : make_uint4(0, 0, 0, 0);
+        } else {
+            q_at = mine ? at : ring + 3 * kStage;
+            q_step = mine ? 4 * HD : 0;
         }
     }
     __device__ __forceinline__ uint4 fragment(int nb, int w) const {
@@ -459,7 +445,7 @@ struct Q4Rows {
     static constexpr int kTile = 16 * kSub, kRow = HD / 2, kScaleRow = 2 * kBlocks;
     static constexpr int kOffV = kTile * kRow, kOffKs = 2 * kOffV, kOffVs = kOffKs + kTile * kScaleRow;
     static constexpr int kStage = kOffVs + kTile * kScaleRow;
-    static constexpr int kRing = 3 * kStage + 64;  // bytes of a warp: the stages, and zeros
+    static constexpr int kRing = 3 * kStage + (NB > 1 ? 64 : 0);  // bytes of a warp: the stages, and zeros
     const char *kp, *vp, *sp;       // the lane's bytes of rows 0..15: codes of keys and values, scales of either
     uint32_t ring, to_k, to_v, to_s;  // where they go in a stage
     uint32_t at_k, at_ks, at_v, at_vs;  // what the lane reads of a stage
@@ -477,7 +463,7 @@ struct Q4Rows {
         at_ks = kOffKs + g * kScaleRow + 2 * (t % kBlocks);
         at_v = kOffV + swizzle(2 * t, 4 * kVW * g / 16) + 4 * kVW * g % 16;
         at_vs = kOffVs + g * kScaleRow + 2 * (t % kBlocks);
-        if (lane < 16) reinterpret_cast<uint32_t *>(warp_ring + 3 * kStage)[lane] = 0;
+        if (NB > 1 && lane < 16) reinterpret_cast<uint32_t *>(warp_ring + 3 * kStage)[lane] = 0;
     }
     // Byte of a 16-byte chunk of a value row; rows 1 and 8 on have the same swizzle.
     __device__ __forceinline__ static int swizzle(int row, int chunk) { return row * kRow + 16 * (kRow == 64 ? chunk ^ (row & 2) : chunk); }
@@ -517,10 +503,6 @@ struct Q4Rows {
             for (int i = 0; i < 2; ++i)
                 if (!(there >> (16 * s + key_pos(lane, i)) & 1)) vs[s][i] = 0.0f;
     }
-    // A: codes n as subnormal halves, n 2^-24 (low nibbles) and 16 n 2^-24 (high
-    // nibbles, whose q is divided by 16), so a code costs half a mask; the sums
-    // start at -8 sum q, which makes them those of n - 8.  (Not done for the values: there the
-    // offset would be summed over all positions and cost digits.)
     __device__ __forceinline__ void scores(float (&sc)[kSub][NB][2]) {
         const uint32_t base = stage == ring + 2 * kStage ? ring : stage + kStage;  // of the next tile
         uint32_t kr[kSub][2][kKW];
@@ -539,7 +521,6 @@ struct Q4Rows {
                 }
                 ks[s][i] = lds_half(base + at_ks + (16 * s + 8 * i) * kScaleRow);
             }
-        constexpr uint32_t kLo = 0x000f000fu, kHi = 0x00f000f0u;
         float c[kSub][NB][4], d[kSub][NB][4];  // two shorter chains
 #pragma unroll
         for (int w = 0; w < kKW; ++w) {
@@ -549,13 +530,8 @@ struct Q4Rows {
 #pragma unroll
                 for (int s = 0; s < kSub; ++s) {
                     const uint32_t x = kr[s][0][w], y = kr[s][1][w], x8 = x >> 8, y8 = y >> 8;
-                    if (w == 0) {
-                        mma16816(c[s][nb], x & kLo, y & kLo, x & kHi, y & kHi, u.x, u.y, bias[nb][0][0], bias[nb][0][1]);
-                        mma16816(d[s][nb], x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, u.z, u.w, bias[nb][1][0], bias[nb][1][1]);
-                    } else {
-                        mma16816(c[s][nb], x & kLo, y & kLo, x & kHi, y & kHi, u.x, u.y);
-                        mma16816(d[s][nb], x8 & kLo, y8 & kLo, x8 & kHi, y8 & kHi, u.z, u.w);
-                    }
+                    mma16816(c[s][nb], w == 0, codes_lo(x), codes_lo(y), codes_hi(x), codes_hi(y), u.x, u.y);
+                    mma16816(d[s][nb], w == 0, codes_lo(x8), codes_lo(y8), codes_hi(x8), codes_hi(y8), u.z, u.w);
                 }
             }
         }
@@ -564,10 +540,9 @@ struct Q4Rows {
         for (int s = 0; s < kSub; ++s)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const float scale = ks[s][i] * 16777216.0f;
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    float x = ((c[s][nb][2 * i] + d[s][nb][2 * i]) + (c[s][nb][2 * i + 1] + d[s][nb][2 * i + 1])) * scale;
+                    float x = ((c[s][nb][2 * i] + d[s][nb][2 * i]) + (c[s][nb][2 * i + 1] + d[s][nb][2 * i + 1])) * ks[s][i];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
                     sc[s][nb][i] = x * inv[nb];
