@@ -1226,7 +1226,8 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
             float *dst = a.part + (2 * blockIdx.x + (begins ? 1 : 0)) * kPieceFloats;
             const bool second = joining == 2;
             const uint32_t pieces = all & (0xffffffffu >> (31 - last)) & (0xffffffffu << first);
-            if (4 * warp < NH) {  // what each piece counts: lane % 8 a piece, lane / 8 a head of four
+            const bool pair = __popc(pieces) <= 2;  // weighted by each thread for itself
+            if (!pair && 4 * warp < NH) {  // what each piece counts: lane % 8 a piece, lane / 8 a head of four
                 static_assert(Smem::kPieces == 8, "a head's pieces are 8 lanes'");
                 const int k = lane & 7, hh = min(4 * warp + (lane >> 3), NH - 1);
                 const bool there = pieces >> k & 1;
@@ -1241,16 +1242,28 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                 S.weight[k][hh] = f;
                 if (k == 0) S.sum_m[hh] = top, S.sum_l[hh] = l;
             }
-            __syncthreads();
+            if (!pair) __syncthreads();
             const float *o = second ? S.cluster_o[0] : S.o[0];
 #pragma unroll 1
             for (int e = tid; e < h.heads * HD; e += kPaThreads) {
                 const int hh = e / HD;
-                float x = 0.0f;
+                float x = 0.0f, top, l;
+                if (pair) {
+                    const float m0 = second ? S.cluster_m[first][hh] : S.m[first][hh], m1 = second ? S.cluster_m[last][hh] : S.m[last][hh];
+                    top = fmaxf(m0, m1);
+                    const float f0 = m0 == top ? 1.0f : ex2(m0 - top), f1 = last == first ? 0.0f : m1 == top ? 1.0f : ex2(m1 - top);
+                    l = f0 * (second ? S.cluster_l[first][hh] : S.l[first][hh]);
+                    x = f0 * o[first * NH * HD + e];
+                    if (last != first) {
+                        l += f1 * (second ? S.cluster_l[last][hh] : S.l[last][hh]);
+                        x += f1 * o[last * NH * HD + e];
+                    }
+                } else {
 #pragma unroll
-                for (int k = 0; k < Smem::kPieces; ++k)
-                    if (pieces >> k & 1) x += S.weight[k][hh] * o[k * NH * HD + e];
-                const float top = S.sum_m[hh], l = S.sum_l[hh];
+                    for (int k = 0; k < Smem::kPieces; ++k)
+                        if (pieces >> k & 1) x += S.weight[k][hh] * o[k * NH * HD + e];
+                    top = S.sum_m[hh], l = S.sum_l[hh];
+                }
                 if (complete) {
                     act_store<ACT>(a.out, h.row * a.out_stride + static_cast<long long>(h.head0) * HD + e, x * inverse_of(l));
                     if (a.lse && e % HD == 0)
@@ -1269,7 +1282,7 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
                     }
                 }
             }
-            __syncthreads();
+            if (!pair) __syncthreads();
             if (!complete) open[begins ? 1 : 0] = first;
         }
         if (joining == 2) return;
