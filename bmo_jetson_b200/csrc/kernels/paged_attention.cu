@@ -23,7 +23,7 @@
 // contraction runs over a permuted index, so that 16 consecutive bytes of a
 // row are a lane's fragment: rows go from global memory straight into
 // registers, and nothing is staged.  64 sessions of up to 3000 positions, 32
-// heads of 128 (1.64 GB): 259 us, 6.3 TB/s, 0.98 of the measured copy.
+// heads of 128 (1.64 GB): 259 to 264 us, 6.2 to 6.3 TB/s, 0.97 of the measured copy.
 //
 // Q4_0 cache: columns 2t, 2t + 1 are block t of head_dim.  q is masked to the
 // block, so the score comes out as one sum over codes a block, which the
@@ -31,8 +31,8 @@
 // block's scale.  Unpacking costs two instructions per two codes, on
 // half-rate pipes, and makes the kernel bound by instructions: registers go to the
 // arithmetic, and rows arrive in a ring in shared memory by asynchronous copies.  64
-// sessions of 1500 positions (442 MB): 100 us, 4.4 TB/s, the issue slots 60% and the
-// ALU pipe 51% busy; with the rows in registers 152 us.
+// sessions of 1500 positions (442 MB): 100 to 105 us, 4.2 to 4.4 TB/s, the issue
+// slots 62% busy; the rows in registers took 152 us, the ring alone brought 111.
 //
 // Work: a row's window is cut into tiles of kTile positions; (row, key head,
 // tile) in that order is a line of tiles of which every warp takes an equal,
@@ -1416,10 +1416,10 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
     const size_t smem = kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * a.n_rows;
     // Few heads of bounded length: a cluster a head, whose CTAs join through
-    // shared memory instead of global memory (32 heads of 512 positions: 8.4 us
-    // against 9.7).  As many CTAs as give a warp a tile, if 3 tiles a warp are enough and the
+    // shared memory instead of global memory (32 heads of 512 positions: 8.3 us
+    // against 10.7).  As many CTAs as give a warp a tile, if 3 tiles a warp are enough and the
     // clusters find room at once: with all resident CTAs in clusters, 74 heads in
-    // clusters of 4 took 19 us, not 11.
+    // clusters of 4 took 19.3 us, not 11.6.
     const long long heads = static_cast<long long>(a.n_rows) * a.units.d;
     const long long table = a.max_blocks * static_cast<long long>(a.page.d);
     const long long tiles = (a.window > 0 && a.window < table ? a.window : table) / (16 * R::kSub);
@@ -1452,7 +1452,7 @@ template <class F>
 auto pa_variant(int head_dim, int kv_type, int group, F f) {
     // Query heads that share a key head are taken together as far as their sums fit the
     // registers: most of the work is on the codes (4 query heads of 128 a key
-    // head: 99 us one by one, 73 in pairs).
+    // head, 64 sessions of 1500: 99 us one by one, 72 to 77 in pairs).
     if (kv_type == kKvQ4_0 && head_dim == 128)
         return group > 1 ? f(PaVariant<Q4Rows<128, 2>>{}) : f(PaVariant<Q4Rows<128, 1>>{});
     if (kv_type == kKvQ4_0)
