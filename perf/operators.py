@@ -225,9 +225,6 @@ def prepare(case, seed):
         need = sum(_cdiv(n + max(0, m), ps) + 1 for n, m in zip(lens, new))
         blocks = max(_cdiv(n + max(0, m), ps) for n, m in zip(lens, new)) + 1
         s |= _book(case, lens, 2 * need + 5, blocks, gen)
-        # the rest of the pool is others': pages that a step gives back stay clear of the ring's entries
-        # that it takes, so a pass can be repeated from the same lengths and state
-        s["book"][1] = need
         tokens = sum(max(0, m) for m in new)
         tokens += tokens // 8 + 3  # room for more than this step's
         s["n_new"] = _int(new)
@@ -459,6 +456,5 @@ def exact(case, seed):
         pos = s["pos"].cpu().numpy()
         q, k = _exact_turn(q, pos), _exact_turn(k, pos)
     # a Q4_0 block's codes are defined by 32-bit operations: its rows have no value in 64 bits
-    if case["kv"] == "q4_0":
-        return {"k": None, "v": None, "q": q} if case["rope"] else None
-    return {"k": k, "v": v} | ({"q": q} if case["rope"] else {})
+    got = {"k": None, "v": None} if case["kv"] == "q4_0" else {"k": k, "v": v}
+    return got | ({"q": q} if case["rope"] else {})
