@@ -33,6 +33,13 @@ namespace {
 // ends.  Prefix sums over the requests place each of these in the ring of free
 // pages and in the list of new positions.
 //
+// Lengths and state can go to other buffers than they come from, so the caller
+// may drop a plan and make it, or another, again from the old ones.  Table
+// cells before nb(L) are not written, later ones are stale, so the table needs
+// nothing for that; but pages given back past the ring's end overwrite its
+// first entries, those that the step takes.  Their earlier pages are kept in
+// book.undo, and a plan that begins at the same state reads them from there.
+//
 // What bounds it is latency: a few dependent loads and block barriers over a
 // few KB, so one CTA does all of it and no second launch follows, unless
 // there are so many new positions that one SM would take longer than the
@@ -163,6 +170,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
     const bmo_page_book &b = a.book;
     const int tid = threadIdx.x, ps = b.page_size, n_pages = b.n_pages;
     const int head = b.state[0], count = b.state[1];
+    // the ring entries that the last plan has overwritten, if it began at this state
+    int *const kept = b.undo ? b.undo + 4 : nullptr, *const written = b.undo ? kept + n_pages : nullptr;
+    int redo = 0;
+    if (b.undo) {  // loaded together: the start is a chain of loads as it is
+        const int head0 = b.undo[0], count0 = b.undo[1], n = b.undo[2];
+        if (head0 == head && count0 == count) redo = n;
+    }
     const bool one = b.n_req <= kPlanThreads;  // each thread has one request at most
 
     // ---- totals, and whether the step can be served ----
@@ -207,8 +221,28 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
     }
     const bool ok = bad == 0;
     const int n_add = ok ? static_cast<int>(all_add) : 0;
-    auto ring_at = [&](long long i) { return (static_cast<long long>(head) + i) % n_pages; };
+    auto ring_at = [&](long long i) {  // i <= count + all_give <= 2 n_pages
+        long long at = head + i;
+        if (at >= n_pages) at -= n_pages;
+        if (at >= n_pages) at -= n_pages;
+        return at;
+    };
     auto cell = [&](int r, int block) { return static_cast<long long>(r) * b.max_blocks + block; };
+    if (!ok || redo < 0 || redo > n_pages) redo = 0;
+    if (redo) {  // the plan was dropped, unless the caller has written the ring anew
+        bool same = true;
+        for (int i = tid; i < redo; i += kPlanThreads) same &= b.free_pages[ring_at(i)] == written[i];
+        if (!__syncthreads_and(same)) redo = 0;
+    }
+    auto take_page = [&](long long i) { return i < redo ? kept[i] : b.free_pages[ring_at(i)]; };
+    auto give_page = [&](long long i, int page) {  // i-th given back; every page has been taken
+        const long long over = count + i - n_pages;  // past the end: the entry of the ring's start
+        if (over >= 0 && b.undo) {
+            if (over >= redo) kept[over] = b.free_pages[ring_at(over)];
+            written[over] = page;
+        }
+        b.free_pages[ring_at(count + i)] = page;
+    };
 
     if (few && ok) {
         const int r = tid;
@@ -216,7 +250,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
 #pragma unroll
         for (int j = 0; j < kFew; ++j)
             if (j < it.take) {
-                taken[j] = b.free_pages[ring_at(end.take - it.take + j)];
+                taken[j] = take_page(end.take - it.take + j);
                 b.table[cell(r, it.have + j)] = taken[j];
             }
         int given[kFew];
@@ -237,7 +271,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
         __syncthreads();  // every page is taken before one is given back into the ring
 #pragma unroll
         for (int j = 0; j < kFew; ++j)
-            if (j < it.give) b.free_pages[ring_at(count + static_cast<long long>(end.give - it.give) + j)] = given[j];
+            if (j < it.give) give_page(end.give - it.give + j, given[j]);
         if (r < b.n_req) a.lens_out[r] = it.after;
     } else {
         // new pages and the list of new positions, kPlanThreads requests at a time
@@ -256,7 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
             plan_fill<PlanCell>(
                 s_end, nr, total.take,
                 [&](int i, int w, int j) {
-                    return PlanCell{cell(r0 + w, (s_len[w] + ps - 1) / ps + j), b.free_pages[ring_at(take0 + i)]};
+                    return PlanCell{cell(r0 + w, (s_len[w] + ps - 1) / ps + j), take_page(take0 + i)};
                 },
                 [&](int, PlanCell c) { b.table[c.at] = c.page; });
             __syncthreads();
@@ -293,13 +327,16 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
                 __syncthreads();
                 plan_fill<int>(
                     s_end, nr, total.give, [&](int, int w, int j) { return b.table[cell(r0 + w, s_first[w] + j)]; },
-                    [&](int i, int page) { b.free_pages[ring_at(count + give0 + i)] = page; });
+                    [&](int i, int page) { give_page(give0 + i, page); });
                 __syncthreads();
                 give0 += total.give;
             }
             if (r < b.n_req) a.lens_out[r] = ok ? it.after : b.lens[r];
         }
     }
+    // entries that the dropped plan has overwritten and this one has not
+    const int over = ok ? static_cast<int>(max(0ll, count + all_give - n_pages)) : 0;
+    for (int i = over + tid; i < redo; i += kPlanThreads) b.free_pages[ring_at(i)] = kept[i];
     if (tid == 0) a.offsets[b.n_req] = n_add;
     if (list_here)
         for (int i = n_add + tid; i < a.max_tokens; i += kPlanThreads) a.slot[i] = a.pos[i] = a.req[i] = -1;
@@ -308,6 +345,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PagedPlanArgs a, int
         a.state_out[1] = ok ? static_cast<int>(count - all_take + all_give) : count;
         a.state_out[2] = bad;
         a.state_out[3] = n_add;
+        if (ok && b.undo) b.undo[0] = head, b.undo[1] = count, b.undo[2] = over;
     }
 }
 

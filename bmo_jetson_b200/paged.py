@@ -46,7 +46,8 @@ _ext = _load()
 
 class _Book(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("table", "lens", "free_pages", "state")] + \
-               [(n, ctypes.c_int32) for n in ("n_req", "max_blocks", "n_pages", "page_size", "window")]
+               [(n, ctypes.c_int32) for n in ("n_req", "max_blocks", "n_pages", "page_size", "window")] + \
+               [("undo", ctypes.c_void_p)]
 
 
 class _Cache(ctypes.Structure):
@@ -66,7 +67,8 @@ def _ints(t: torch.Tensor, name: str, device, numel: Optional[int] = None) -> in
 class PageBook:
     """Block table [n_req, max_blocks], lengths [n_req], ring of free pages
     [n_pages] and state [4] (first free entry, free pages, status bits, new
-    positions of the last step): int32 tensors on one GPU."""
+    positions of the last step): int32 tensors on one GPU.  Keep one PageBook
+    for them: it also holds what lets its last plan be dropped and made again."""
 
     def __init__(self, table: torch.Tensor, lens: torch.Tensor, free: torch.Tensor, state: torch.Tensor, *,
                  page_size: int, window: int = 0):
@@ -78,6 +80,9 @@ class PageBook:
         self._c = _Book(_ints(table, "table", self.device), _ints(lens, "lens", self.device, n_req),
                         _ints(free, "free", self.device), _ints(state, "state", self.device, 4), n_req, max_blocks,
                         free.numel(), self.page_size, self.window)
+        self._undo = torch.zeros(4 + 2 * free.numel(), dtype=torch.int32, device=self.device)
+        torch.cuda.current_stream(self.device).synchronize()  # plans may be on another stream
+        self._c.undo = self._undo.data_ptr()
         self._addr, self._dev = ctypes.addressof(self._c), self.device.index
 
     @classmethod
@@ -96,7 +101,11 @@ class PageBook:
         request r, 0 leaves it, < 0 ends it.  slot, pos, req [max_tokens] and
         offsets [n_req + 1] receive the list of new positions; the new
         lengths and state replace the book's unless lens_out / state_out are
-        given.  state[2] != 0 after it: the step was refused, nothing changed."""
+        given.  The table and the ring change in place.  A plan into lens_out
+        and state_out may be dropped: the next one from the book's own, of this
+        step or another, is as if it had not been made (the last plan alone, by
+        this PageBook).  state[2] != 0 after it: the step was refused, nothing
+        changed."""
         _ext.plan(self._addr, self._dev, n_new, slot, pos, req, offsets, lens_out, state_out)
 
 

@@ -192,6 +192,7 @@ typedef struct bmo_page_book {
     int32_t *state;      /* [4]: first free entry of the ring, free pages, status bits, new positions of the step */
     int32_t n_req, max_blocks, n_pages, page_size;
     int32_t window; /* > 0: a token attends to the last `window` positions, its own included; 0: to all */
+    int32_t *undo;  /* [4 + 2 * n_pages], zero at first, or NULL: what lets a plan be made again (bmo_k_paged_plan) */
 } bmo_page_book;
 
 typedef struct bmo_paged_kv {
@@ -211,7 +212,14 @@ typedef struct bmo_paged_kv {
  * req_dev [max_tokens] is its slot number, position and request (-1 past the
  * last), offsets_dev [n_req + 1] is each request's first entry.
  * lens_out_dev [n_req] and state_out_dev [4] receive the new lengths and
- * state; they may be book->lens and book->state.  A step that cannot be
+ * state; they may be book->lens and book->state.  The table and the ring
+ * change in place.  With book->undo, a plan into other lens_out_dev and
+ * state_out_dev may be dropped: the next plan from the old lengths and state,
+ * of the same step or another, is as if it had not been made.  That holds
+ * for the last plan that was served, through the same undo buffer.  Without it
+ * (undo NULL) a plan's outputs have to be adopted: pages given back may have
+ * overwritten the ring's entries that the step took, and a second plan from
+ * the old state would hand out pages that are in use.  A step that cannot be
  * served changes nothing but state_out[2], which says why
  * (BMO_PAGED_* bits), and lists no positions.  n_req <= 65536. */
 BMO_API int bmo_k_paged_plan(const bmo_page_book *book, const int32_t *n_new_dev, int max_tokens, int32_t *slot_dev,
