@@ -174,6 +174,8 @@ class PagedKV:
                   status: Optional[torch.Tensor] = None) -> None:
         """Attention of q [n, n_heads, head_dim] into out (bmo_k_paged_attention).
         Row i is a token of request rows[i] (default i) that attends to the first
-        row_lens[i] positions (default all); lse [n, n_heads] fp32."""
+        row_lens[i] positions (default, and at most, the book's length); lse [n,
+        n_heads] fp32.  With a window, row_lens below the length before the last
+        plan can reach pages that were given back."""
         _ext.attention(self._addr, self._dev, layer, q, out, rows, row_lens, scale, lse, status, self._scratch_addr,
                        self._scratch_bytes)

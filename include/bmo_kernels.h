@@ -251,12 +251,18 @@ BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, in
  * [n_rows][n_heads][head_dim] attends to the last `window` (book.window; 0:
  * all) of the first row_len_dev[i] positions of request row_req_dev[i].
  * row_req_dev NULL: row i is request i; row_len_dev NULL: the request's
- * length.  So several rows may be tokens of one request.  Query head h reads
+ * length.  So several rows may be tokens of one request.  row_len_dev[i] is
+ * at most the request's length in book.lens, where lengths planned into a
+ * separate lens_out_dev have to be first; a larger one sets BMO_PAGED_BAD_INDEX
+ * and means that length.  With a window the caller sees to it that row_len_dev[i]
+ * is above the length that the request had before the last plan, or that
+ * its window begins in pages that were not given back before: those may be
+ * another request's.  Query head h reads
  * key head h / (n_heads / n_kv_heads); scale 0 means 1 / sqrt(head_dim).
  * out_dev [n_rows][n_heads][head_dim] in act_type; lse_dev (optional, fp32
  * [n_rows][n_heads]) receives log(sum(exp(score))).  A row of length 0 gives
- * zeros and -inf.  Rows are q_stride, out_stride elements apart.  Slots
- * past a request's length are never read.  Sums, maxima and products are fp32
+ * zeros and -inf.  Rows are q_stride, out_stride elements apart.  What
+ * lies in slots past a row's length, or before its window, has no part in its result.  Sums, maxima and products are fp32
  * (each fp32 factor as two fp16 parts); the result is the same from call to
  * call.  scratch_dev must be zero on the first call, is left reusable, and
  * serves one call at a time.  n_rows <= 4096, and n_rows * n_heads *

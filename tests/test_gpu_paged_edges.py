@@ -133,3 +133,19 @@ def test_plan_of_many_requests_with_long_lists(n_req, ps, window, most):
         new[rng.random(n_req) < 0.15] = -1
         s.sim = s.check(new, s.plan(new))
         s.adopt()
+
+
+# ---------------------------------------------------------------- lengths beyond a request's
+
+@pytest.mark.parametrize("kv", ["f16", "q4_0"])
+@pytest.mark.parametrize("window", [0, 8])
+def test_attention_row_len_above_the_requests(kv, window):
+    """A row length that the table's row has room for and the request does not hold:
+    reported, and the row attends to what the request holds, not to a page of another's."""
+    c = base.Case([20, 64], 1, 64, 16, kv, window=window)
+    c.cache.book.table[0, 2] = int(c.table[1, 3])  # stale: another request has the page now
+    q, out, lse, status = base.attend(c, 2, reqs=[0, 1, 0], lens=[40, 64, 20])
+    assert status == paged.BAD_INDEX
+    base.close(out, lse, c.attention(q.cpu().numpy(), reqs=[0, 1, 0], lens=[20, 64, 20]), base.vmax(c))
+    q, out, lse, status = base.attend(c, 2, reqs=[0, 1, 0], lens=[20, 64, 19])
+    assert status == 0
