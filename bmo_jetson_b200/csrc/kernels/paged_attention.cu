@@ -339,6 +339,11 @@ struct F16Rows {
         }
     }
     __device__ __forceinline__ void reset() {}
+    // Element d of a row is code(d) times scale(d / 32).
+    __device__ __forceinline__ static float code(const void *rows, long long row, int d) {
+        return __half2float(static_cast<const __half *>(rows)[row * HD + d]);
+    }
+    __device__ __forceinline__ static float scale(const __half *, long long, int) { return 1.0f; }
     // Adds the weighted values of the tile.  The tensor core's sum of a tile
     // starts from zero and is added in fp32: its own running sum is not rounded to nearest.
     __device__ __forceinline__ void values(const float (&w)[kSub][NB][2], float (&o)[NB][kO][4]) {
@@ -549,6 +554,14 @@ struct Q4Rows {
                 }
             }
     }
+    // Element d of a row is code(d) times scale(d / 32).
+    __device__ __forceinline__ static float code(const void *rows, long long row, int d) {
+        const int byte = static_cast<const uint8_t *>(rows)[row * (HD / 2) + d / 32 * 16 + d % 16];
+        return static_cast<float>((d % 32 < 16 ? byte & 15 : byte >> 4) - 8);
+    }
+    __device__ __forceinline__ static float scale(const __half *scales, long long row, int block) {
+        return __half2float(scales[row * kBlocks + block]);
+    }
     __device__ __forceinline__ void reset() { stage = ring, vlim = 5.9604644775390625e-08f, vinv = 16777216.0f; }  // 2^-24, 2^24
     // Whether a value scale of part s passes the bound of what a weight may be multiplied by.
     __device__ __forceinline__ bool value_range(int s) {
@@ -705,6 +718,74 @@ constexpr size_t kFixedSmem = (sizeof(PaSmem<HD, NH>) + 15) / 16 * 16;
 // A piece in global memory: [heads][HD] sums, then the maxima and the weights' sums; 16-byte multiples.
 template <class R>
 constexpr int pa_piece_floats = (R::kHeads * (R::HD + 2) + 3) / 4 * 4;
+
+// The heads [head0, head0 + heads) of `row` that have NaN in them once more, over
+// positions [p0, p1), from the formula, by one warp: their sums (dst), maxima and
+// weights' sums.  The two parts of a factor are added as two products, and with
+// an infinite key or value these can be of opposite signs, or 0 times infinity.
+// Whatever that spoils ends as NaN (rows that hold NaN come here, too).  Sums in
+// double: speed does not matter.
+template <class R, int ACT>
+__device__ __noinline__ void exact_piece(const PagedAttnArgs &a, int row, int head0, int heads, int req, int p0, int p1,
+                                         float *dst, float *dst_m, float *dst_l) {
+    const int lane = threadIdx.x & 31;
+    constexpr int HD = R::HD;
+    const int *table = a.table + static_cast<long long>(req) * a.max_blocks;
+    const int kh = head0 / a.group;
+    auto row_of = [&](int p) -> long long {  // -1: not there
+        if (p >= p1) return -1;
+        const uint32_t b = fast_div(p, a.page), page = table[b];
+        return page < static_cast<uint32_t>(a.n_pages) ? (page * a.n_kv_heads + kh) * a.page.d + (p - b * a.page.d) : -1ll;
+    };
+#pragma unroll 1
+    for (int h = 0; h < heads; ++h, dst += HD) {
+        __syncwarp();
+        float sum = dst_l[h];  // NaN if an element is
+#pragma unroll
+        for (int i = 0; i < HD; i += 32) sum += dst[i + lane];
+        if (!__any_sync(0xffffffffu, sum != sum)) continue;
+        const long long q = row * a.q_stride + static_cast<long long>(head0 + h) * HD;
+        auto score = [&](long long r) {
+            double x = 0.0, block = 0.0;
+#pragma unroll 1
+            for (int d = 0; d < HD; ++d) {
+                block += static_cast<double>(act_load<ACT>(a.q, q + d)) * static_cast<double>(R::code(a.k, r, d));
+                if (d % 32 == 31) x += block * static_cast<double>(R::scale(a.k_scale, r, d / 32)), block = 0.0;
+            }
+            return static_cast<float>(x * static_cast<double>(a.qscale));
+        };
+        float m = -INFINITY;
+#pragma unroll 1
+        for (int p = p0 + lane; p < p1; p += 32) {
+            const long long r = row_of(p);
+            if (r >= 0) m = fmaxf(m, score(r));
+        }
+        m = warp_max(m);
+        const float ref = m == -INFINITY ? 0.0f : m - kHead;
+        double l = 0.0, o[HD / 32] = {};
+#pragma unroll 1
+        for (int first = p0; first < p1; first += 32) {
+            const long long mine = row_of(first + lane);
+            const float w_mine = mine >= 0 ? ex2(score(mine) - ref) : 0.0f;
+            l += w_mine;
+#pragma unroll 1
+            for (int j = 0; j < 32; ++j) {
+                const float w = __shfl_sync(0xffffffffu, w_mine, j);
+                const long long r = __shfl_sync(0xffffffffu, mine, j);
+                if (r < 0) continue;
+#pragma unroll
+                for (int i = 0; i < HD / 32; ++i)
+                    o[i] += static_cast<double>(w) * static_cast<double>(R::code(a.v, r, lane + 32 * i) * R::scale(a.v_scale, r, i));
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) dst[lane + 32 * i] = static_cast<float>(o[i]);
+        if (lane == 0) dst_m[h] = m, dst_l[h] = static_cast<float>(l);
+    }
+}
 
 template <class R, int ACT, bool kAligned>
 __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(const __grid_constant__ PagedAttnArgs a) {
@@ -1167,21 +1248,28 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         }
         float *dst = whole ? buf : S.o[slot], *dst_m = whole ? S.bm[warp] : S.m[slot], *dst_l = whole ? S.bl[warp] : S.l[slot];
         __syncwarp();
+        float sum = 0.0f;  // NaN if an element is
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int h = R::head_of(nb, lane);
             if (h >= hd.heads) continue;
+            sum += l[nb];
             if (R_.owns(lane)) {
 #pragma unroll
                 for (int run = 0; run < R::kRuns; ++run)
 #pragma unroll
-                    for (int i = 0; i < R::kRunLen; i += 4)
-                        *reinterpret_cast<float4 *>(dst + h * HD + R::run_start(run, lane) + i) =
-                            make_float4(R_.element(o[nb], run, i), R_.element(o[nb], run, i + 1),
-                                        R_.element(o[nb], run, i + 2), R_.element(o[nb], run, i + 3));
+                    for (int i = 0; i < R::kRunLen; i += 4) {
+                        const float4 x = make_float4(R_.element(o[nb], run, i), R_.element(o[nb], run, i + 1),
+                                                     R_.element(o[nb], run, i + 2), R_.element(o[nb], run, i + 3));
+                        *reinterpret_cast<float4 *>(dst + h * HD + R::run_start(run, lane) + i) = x;
+                        sum += (x.x + x.y) + (x.z + x.w);
+                    }
             }
             if (g == 0 && (R::kRing == 0 || t == 0)) dst_m[h] = m[nb], dst_l[h] = l[nb];
         }
+        if (__any_sync(0xffffffffu, sum != sum))
+            exact_piece<R, ACT>(a, row, hd.head0, hd.heads, req, max(start, pbase + tile0 * kTile),
+                                min(len, pbase + tile1 * kTile), dst, dst_m, dst_l);
         __syncwarp();
         if (whole) {
             const long long out0 = row * a.out_stride + static_cast<long long>(hd.head0) * HD + lane;

@@ -263,7 +263,9 @@ BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, in
  * [n_rows][n_heads]) receives log(sum(exp(score))).  A row of length 0 gives
  * zeros and -inf.  Rows are q_stride, out_stride elements apart.  What
  * lies in slots past a row's length, or before its window, has no part in its result.  Sums, maxima and products are fp32
- * (each fp32 factor as two fp16 parts); the result is the same from call to
+ * (each fp32 factor as two fp16 parts; heads that meet an infinite or NaN
+ * element are computed from the formula instead, in which a block of a Q4_0 key
+ * is its scale times the sum of its codes' products); the result is the same from call to
  * call.  scratch_dev must be zero on the first call, is left reusable, and
  * serves one call at a time.  n_rows <= 4096, and n_rows * n_heads *
  * (max_blocks * page_size / 16 + 4) below 2^31.  status_dev as above. */

@@ -149,3 +149,172 @@ def test_attention_row_len_above_the_requests(kv, window):
     base.close(out, lse, c.attention(q.cpu().numpy(), reqs=[0, 1, 0], lens=[20, 64, 20]), base.vmax(c))
     q, out, lse, status = base.attend(c, 2, reqs=[0, 1, 0], lens=[20, 64, 19])
     assert status == 0
+
+
+# ---------------------------------------------------------------- infinite rows
+
+class Rows:
+    """One request on pages of 16 in order, its rows as given: k, v [positions, kv_heads, hd].
+    Q4_0: packed, then `edit(codes and scales of k, of v)` may change them."""
+
+    def __init__(self, k, v, kv="f16", edit=None, more=(), window=0):
+        n, kv_heads, hd = k.shape
+        pages = -(-n // 16)
+        lens = [n] + list(more)
+
+        def paged_rows(x):  # [1, page, head, slot, row]
+            y = np.zeros((pages * 16,) + x.shape[1:], x.dtype)
+            y[:n] = x
+            return np.ascontiguousarray(y.reshape(pages, 16, *x.shape[1:]).transpose(0, 2, 1, 3)[None])
+
+        table = np.tile(np.arange(pages), (len(lens), 1))
+        book = paged.PageBook(i32(table), i32(lens), i32(np.arange(pages)), i32([0, 0, 0, 0]), page_size=16, window=window)
+        self.kv_heads, self.hd, self.window, self.lens = kv_heads, hd, window, lens
+        if kv == "f16":
+            k, v = k.astype(np.float16), v.astype(np.float16)
+            self.k, self.v = k.astype(np.float64), v.astype(np.float64)
+            self.k_scale = np.ones(k.shape[:2] + (hd // 32,))
+            self.cache = paged.PagedKV(book, *(torch.from_numpy(paged_rows(x)).to(DEV) for x in (k, v)))
+        else:
+            (kn, ks), (vn, vs) = base.pack(k.astype(np.float32)), base.pack(v.astype(np.float32))
+            if edit:
+                edit((kn, ks), (vn, vs))
+            with np.errstate(invalid="ignore"):
+                self.k, self.v = base.unpack(kn, np.ones_like(ks)), base.unpack(vn, vs)
+            self.k_scale = ks.astype(np.float64)
+            t = [torch.from_numpy(paged_rows(x)).to(DEV) for x in (kn, vn, ks, vs)]
+            self.cache = paged.PagedKV(book, t[0], t[1], k_scale=t[2], v_scale=t[3])
+
+    def run(self, q, rows=None):
+        out = torch.full_like(q, 7.0)
+        lse = torch.full(q.shape[:2], 7.0, device=DEV)
+        self.cache.attention(0, q, out, lse=lse, rows=rows)
+        return out.double().cpu().numpy(), lse.double().cpu().numpy()
+
+    def want(self, q, n=None):
+        """(out, lse, largest score error) of one row in 64 bits; products of zero and infinity are NaN.
+        A block of 32 of a key counts as its scale times the sum of its codes' products."""
+        q = np.asarray(q.double().cpu().numpy())
+        n = self.lens[0] if n is None else n
+        lo = max(0, n - self.window) if self.window else 0
+        k, ks, v = self.k[lo:n], self.k_scale[lo:n], self.v[lo:n]
+        heads = q.shape[0]
+        out, lse, off = np.zeros((heads, self.hd)), np.zeros(heads), np.zeros(heads)
+        with np.errstate(invalid="ignore", over="ignore"):
+            for h in range(heads):
+                g = h // (heads // self.kv_heads)
+                s = ((k[:, g] * q[h]).reshape(len(k), -1, 32).sum(-1) * ks[:, g]).sum(-1) / math.sqrt(self.hd)
+                a = (np.abs(k[:, g] * q[h]).reshape(len(k), -1, 32).sum(-1) * np.abs(ks[:, g])).sum(-1)
+                off[h] = 2.0 ** -20 * np.max(a[np.isfinite(a)], initial=0.0) / math.sqrt(self.hd)
+                p = np.exp(s - s.max())
+                lse[h] = s.max() + np.log(p.sum())
+                out[h] = (p[:, None] * v[:, g])[p != 0].sum(0) / p.sum()
+        return out, lse, off
+
+
+def check_edges(got, want, vmax, dtype=torch.float32):
+    (out, lse), (want_out, want_lse, off) = got, want
+    np.testing.assert_array_equal(np.isnan(out), np.isnan(want_out))
+    there = ~np.isnan(want_out)
+    np.testing.assert_array_equal(np.isinf(out[there]), np.isinf(want_out[there]))
+    inf = np.isinf(want_out)
+    np.testing.assert_array_equal(out[inf], want_out[inf])
+    fin = np.isfinite(want_out)
+    tol = (2 * off[:, None] + 2.0 ** -19) * vmax + base.HALF_UNIT[dtype] * np.abs(np.where(fin, want_out, 0)) + 2.0 ** -25
+    assert (np.abs(out[fin] - want_out[fin]) <= tol[fin]).all()
+    ok = np.isfinite(want_lse)
+    assert not np.isfinite(lse[~ok]).any()
+    bound = off + 2.0 ** -19 + 2.0 ** -22 * np.abs(np.where(ok, want_lse, 0))
+    assert (np.abs(lse[ok] - want_lse[ok]) <= bound[ok]).all()
+
+
+def finite_max(x):
+    return float(np.max(np.abs(x[np.isfinite(x)])))
+
+
+# positions, key heads, query heads, head_dim, window: a CTA or a cluster a head, parts of heads joined, shared heads
+SHAPES = [(1, 1, 1, 64, 0), (40, 2, 2, 128, 0), (700, 3, 12, 128, 300), (700, 1, 5, 64, 0), (9000, 1, 2, 128, 0),
+          (2500, 2, 24, 64, 0)]
+
+
+@pytest.mark.parametrize("n,kv_heads,heads,hd,window", SHAPES[1:])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_attention_infinite_f16_keys(n, kv_heads, heads, hd, window, dtype):
+    """A key of -inf score has weight 0; heads that give it the score +inf, or meet a zero, are NaN."""
+    rng = np.random.default_rng(n + heads)
+    k, v = (rng.normal(0, 1, (n, kv_heads, hd)) for _ in range(2))
+    q = rng.normal(0, 1, (heads, hd))
+    for at in {n - 1, max(0, n - 20), n // 2}:
+        d = rng.integers(0, hd)
+        k[at, :, d] = np.inf
+        q[:, d] = -np.abs(q[:, d]) - 0.1
+        if at == n // 2:
+            q[-1, d] *= -1
+    q = torch.from_numpy(q.astype(np.float32)).to(dtype).to(DEV)
+    r = Rows(k, v, window=window)
+    out, lse = r.run(q[None])
+    want = r.want(q)
+    assert np.isfinite(want[0][:-1]).all()
+    check_edges((out[0], lse[0]), want, finite_max(r.v), dtype)
+
+
+@pytest.mark.parametrize("n,kv_heads,heads,hd,window", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_infinite_f16_values(n, kv_heads, heads, hd, window, dtype):
+    """An infinite value makes its element infinite, two of opposite signs make it NaN, the others stay."""
+    rng = np.random.default_rng(n + heads)
+    k, v = (rng.normal(0, 1, (n, kv_heads, hd)) for _ in range(2))
+    v[n - 1, :, 3] = np.inf
+    v[max(0, n - 9), 0, 40] = -np.inf
+    if n > 1:
+        v[n - 1, -1, 17], v[n - 2, -1, 17] = np.inf, -np.inf
+    q = torch.from_numpy(rng.normal(0, 1, (heads, hd)).astype(np.float32)).to(dtype).to(DEV)
+    r = Rows(k, v, window=window)
+    out, lse = r.run(q[None])
+    check_edges((out[0], lse[0]), r.want(q), finite_max(r.v), dtype)
+
+
+@pytest.mark.parametrize("n,kv_heads,heads,hd,window", SHAPES)
+def test_attention_infinite_q4_scales(n, kv_heads, heads, hd, window):
+    rng = np.random.default_rng(n + heads)
+    k, v = (rng.normal(0, 1, (n, kv_heads, hd)) for _ in range(2))
+    q = rng.normal(0, 1, (heads, hd))
+    q[:, 32:64] = np.abs(q[:, 32:64]) + 0.1
+    q = torch.from_numpy(q.astype(np.float32)).to(DEV)
+
+    def value(_, vals):
+        vals[1][n - 1, :, 1] = np.inf
+
+    def key_low(keys, _):  # every element -8 * inf: the score is -inf
+        keys[0][n - 1, :, 16:32] = 0
+        keys[1][n - 1, :, 1] = np.inf
+
+    def key_any(keys, _):  # a block counts by the sign of its sum
+        keys[1][n - 1, :, 0] = np.inf
+
+    for edit in (value, key_low, key_any):
+        r = Rows(k, v, "q4_0", edit, window=window)
+        out, lse = r.run(q[None])
+        want = r.want(q)
+        if edit is not value and n == 1:
+            continue  # a lone key of score -inf: nothing to attend to
+        check_edges((out[0], lse[0]), want, finite_max(r.v))
+
+
+def test_attention_over_rows_that_append_made_infinite():
+    """Keys past fp16's range are stored as infinities."""
+    cache = paged.PagedKV.empty(paged.PageBook.empty(1, 4, 16, 4), 1, 1, 64)
+    k = torch.randn(20, 1, 64, device=DEV)
+    k[7, 0, 5] = 1e5
+    v = torch.randn(20, 1, 64, device=DEV)
+    cache.append(0, k, v, i32(np.arange(20)))
+    cache.book.table[0, :2] = i32([0, 1])
+    cache.book.lens[0] = 20
+    q = torch.randn(1, 2, 64, device=DEV)
+    q[0, :, 5] = -0.25
+    out = torch.empty_like(q)
+    cache.attention(0, q, out)
+    left = [i for i in range(20) if i != 7]
+    kk, vv = k.half().double()[left, 0], v.half().double()[left, 0]
+    want = torch.softmax(q[0].double() @ kk.T / 8, -1) @ vv
+    assert (out[0].double() - want).abs().max() < 2.0 ** -15
