@@ -14,10 +14,13 @@
 // canonical layout, and 128 rows of B's side, of which a decode step fills 2.)
 //   scores: A = 16 positions x 16 elements of K, B = q
 //   values: A = 16 elements x 16 positions of V^T, B = the weights
-// B has 8 columns.  An fp32 factor x takes two of them, hi = fp16(x) and
-// lo = fp16(x - hi), so products with fp16 keys and values keep about 22 bits
-// (x is brought into fp16's range by a power of two first); the tensor core
-// sums a tile in fp32, and tiles are added by fp32 additions.
+// B has 8 columns.  An fp32 factor x, brought into fp16's range by a power of
+// two, takes two of them: hi = fp16(x) and lo = fp16(2^11 (x - hi)), whose sum is
+// divided by 2^11 when the two are added.  So products with fp16 keys and values
+// keep 22 bits of x, relative to x itself down to 2^-14 and to 2^-36 absolute
+// below (an unscaled lo would end at 2^-25: weights 2^-32 of the largest would
+// count as nothing, some 2^-15 of a row of 131072).  The
+// tensor core sums a tile in fp32, and tiles are added by fp32 additions.
 //
 // fp16 cache: columns 2t, 2t + 1 are head t of a group of 4 (or of 2 x 4).  The
 // contraction runs over a permuted index, so that 16 consecutive bytes of a
@@ -58,10 +61,12 @@ namespace {
 constexpr int kPaWarps = 4;
 constexpr int kPaThreads = 32 * kPaWarps;
 constexpr float kLn2 = 0.6931471805599453f;
-// Weights are e^(s - m) * 2^7 in fp16; the maximum m is raised only when a
-// score passes it by more than 2^8, so a weight is below 2^15 and the sum
-// of its two parts is exact to 2^-25 of the largest weight's 2^7.
+// Weights are e^(s - m) * 2^7 in two fp16 parts; the maximum m is raised only
+// when a score passes it by more than 2^8, so a weight is below 2^15.  Of n
+// weights the parts leave out 2^-22 of each and n 2^-43 of the largest.
 constexpr float kSlack = 8.0f, kHead = 7.0f;
+// The second part of a factor is held times kLo.
+constexpr float kLo = 2048.0f, kLoInv = 1.0f / 2048.0f;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -135,7 +140,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 __device__ __forceinline__ void split_half2(float x, float y, uint32_t &px, uint32_t &py) {  // (hi, lo) of x, of y
     const __half2 hi = __floats2half2_rn(x, y);
     const float2 f = __half22float2(hi);
-    const __half2 lo = __floats2half2_rn(x - f.x, y - f.y);
+    const __half2 lo = __floats2half2_rn((x - f.x) * kLo, (y - f.y) * kLo);
     const uint32_t h = *reinterpret_cast<const uint32_t *>(&hi), l = *reinterpret_cast<const uint32_t *>(&lo);
     px = __byte_perm(h, l, 0x5410);
     py = __byte_perm(h, l, 0x7632);
@@ -206,7 +211,7 @@ __device__ __forceinline__ QueryPart query_part(const float (&x)[4]) {
     for (int i = 0; i < 4; ++i) {
         const float y = x[i] * mul;
         p.hi[i] = __float2half_rn(y);
-        p.lo[i] = __float2half_rn(y - __half2float(p.hi[i]));
+        p.lo[i] = __float2half_rn((y - __half2float(p.hi[i])) * kLo);
     }
     return p;
 }
@@ -334,8 +339,8 @@ struct F16Rows {
                 mma16816(c, j == 0, x.x, y.x, x.y, y.y, q[nb][2 * j][0], q[nb][2 * j][1]);
                 mma16816(d, j == 0, x.z, y.z, x.w, y.w, q[nb][2 * j + 1][0], q[nb][2 * j + 1][1]);
             }
-            sc[nb][0] = ((c[0] + d[0]) + (c[1] + d[1])) * inv[nb];
-            sc[nb][1] = ((c[2] + d[2]) + (c[3] + d[3])) * inv[nb];
+            sc[nb][0] = __fmaf_rn(c[1] + d[1], kLoInv, c[0] + d[0]) * inv[nb];
+            sc[nb][1] = __fmaf_rn(c[3] + d[3], kLoInv, c[2] + d[2]) * inv[nb];
         }
     }
     __device__ __forceinline__ void reset() {}
@@ -381,7 +386,7 @@ struct F16Rows {
     __device__ __forceinline__ static int run_start(int run, int lane) { return 64 * run + 8 * (lane >> 2); }
     __device__ __forceinline__ float element(const float (&o)[kO][4], int run, int i) const {
         const float *c = o[4 * run + i / 2];
-        return i % 2 ? c[2] + c[3] : c[0] + c[1];
+        return i % 2 ? __fmaf_rn(c[3], kLoInv, c[2]) : __fmaf_rn(c[1], kLoInv, c[0]);
     }
 };
 
@@ -547,7 +552,7 @@ struct Q4Rows {
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    float x = ((c[s][nb][2 * i] + d[s][nb][2 * i]) + (c[s][nb][2 * i + 1] + d[s][nb][2 * i + 1])) * ks[s][i];
+                    float x = __fmaf_rn(c[s][nb][2 * i + 1] + d[s][nb][2 * i + 1], kLoInv, c[s][nb][2 * i] + d[s][nb][2 * i]) * ks[s][i];
                     x += __shfl_xor_sync(0xffffffffu, x, 1);
                     x += __shfl_xor_sync(0xffffffffu, x, 2);
                     sc[s][nb][i] = x * inv[nb];
@@ -642,7 +647,7 @@ struct Q4Rows {
     }
     __device__ __forceinline__ float element(const float (&o)[kO][4], int run, int i) const {
         const float *c = o[i];
-        return (run ? c[2] + c[3] : c[0] + c[1]) * vlim;
+        return (run ? __fmaf_rn(c[3], kLoInv, c[2]) : __fmaf_rn(c[1], kLoInv, c[0])) * vlim;
     }
 };
 

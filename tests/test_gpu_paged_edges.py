@@ -318,3 +318,66 @@ def test_attention_over_rows_that_append_made_infinite():
     kk, vv = k.half().double()[left, 0], v.half().double()[left, 0]
     want = torch.softmax(q[0].double() @ kk.T / 8, -1) @ vv
     assert (out[0].double() - want).abs().max() < 2.0 ** -15
+
+
+# ---------------------------------------------------------------- weights, scales and queries of very different sizes
+#
+# Both parts of a factor x = hi + lo / 2^11 keep it to 2^-22 relative, and to
+# 2^-36 absolute where that is more (lo's last bit, 2^-24, halved and divided by
+# 2^11).  A weight is held times 2^7 or more over the largest of its piece, so
+# n weights are off by n 2^-43 of the largest besides; with Q4_0 scales, which
+# are brought below 1 by a power of two up to 4 times the largest, codes up
+# to 8, by n 2^-42 of the largest |v|.
+
+@pytest.mark.parametrize("kv", ["f16", "q4_0"])
+@pytest.mark.parametrize("rows,bits", [(1, 32.0), (2048, 32.0), (2048, 28.5), (1, 36.0)])
+def test_attention_many_small_weights(kv, rows, bits):
+    """One position 2^bits above 65535 others of equal weight, a warp walking few of them or all.
+    Scores are exact but for two roundings of some 36 (2^-18 of a weight)."""
+    n, hd = 65536, 64
+    k, v = np.zeros((n, 1, hd)), np.ones((n, 1, hd))
+    k[0, 0, 0], v[0] = 8.0, 0.0
+    r = Rows(k, v, kv)
+    assert (r.k * r.k_scale[..., :1] == k).all() and (r.v == v).all()
+    q = torch.zeros(rows, 1, hd, device=DEV)
+    q[:, 0, 0] = bits * math.log(2.0)  # scale 1 / 8
+    out, _ = r.run(q, rows=i32(np.zeros(rows)))
+    p = math.exp(-float(q[0, 0, 0]))
+    want = (n - 1) * p / (1 + (n - 1) * p)
+    assert np.max(np.abs(out - want)) <= 2.0 ** -16 * want + n * 2.0 ** -42
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("group", [1, 2, 4])
+def test_attention_q4_blocks_of_unequal_scales(hd, group):
+    """Each block of 32 elements is as exact as its own values ask for."""
+    n = 40
+    rng = np.random.default_rng(hd + group)
+    k, v = (rng.normal(0, 1, (n, 2, hd)) for _ in range(2))
+    v[:, :, :32] *= 2.0 ** 9
+    v[:, :, 32:64] *= 2.0 ** -11
+    r = Rows(k, v, "q4_0")
+    q = torch.from_numpy(rng.normal(0, 0.01, (2 * group, hd)).astype(np.float32)).to(DEV)
+    (out, _), (want, _, off) = r.run(q[None]), r.want(q)
+    top = np.abs(r.v).max()
+    for b in range(hd // 32):
+        e = slice(32 * b, 32 * b + 32)
+        vmax = np.abs(r.v[:, :, e]).max()
+        tol = (2 * off[:, None] + 2.0 ** -19) * vmax + n * 2.0 ** -42 * top
+        assert (np.abs(out[0] - want)[:, e] <= tol).all(), b
+
+
+@pytest.mark.parametrize("kv", ["f16", "q4_0"])
+@pytest.mark.parametrize("heads", [1, 4, 8])
+def test_attention_query_with_one_large_element(kv, heads):
+    """A query element 2^24 times the others, whose keys are 0: the others keep their bits.
+    2^-46 of the large one, over 128 elements, is below the bound of 2^-20 sum |q k|."""
+    rng = np.random.default_rng(heads)
+    k, v = (rng.normal(0, 1, (3, 1, 128)) for _ in range(2))
+    k[:, :, 0] = 0
+    q = rng.normal(0, 1, (heads, 128))
+    q[:, 0] = 2.0 ** 24
+    r = Rows(k, v, kv)
+    q = torch.from_numpy(q.astype(np.float32)).to(DEV)
+    out, lse = r.run(q[None])
+    check_edges((out[0], lse[0]), r.want(q), finite_max(r.v))
