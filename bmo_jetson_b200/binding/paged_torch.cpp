@@ -137,6 +137,9 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Rows v = rows(a[4], "v", dev, tokens, c->n_kv_heads, c->head_dim, type);
         Rows q{nullptr, 0}, qo{nullptr, 0};
         int64_t heads = 0;
+        const double theta = number(a[9]);
+        if (a[7] != Py_None && theta == 0.0) refuse("theta", "above 0 where q is to be rotated");
+        if (a[7] == Py_None && a[8] != Py_None) refuse("q_out", "without q");
         if (a[7] != Py_None) {
             const at::Tensor &query = tensor(a[7], "q");
             if (query.dim() != 3) refuse("q", "[n, heads, head_dim]");
@@ -145,7 +148,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             qo = rows(a[8], "q_out", dev, tokens, heads, c->head_dim, type);
         }
         return g_append(c, layer_of(a[2]), count(tokens, "slot"), k.p, k.stride, v.p, v.stride, ints(a[5], "slot", dev, -1),
-                        ints(a[6], "pos", dev, tokens, true), static_cast<float>(number(a[9])), q.p, q.stride,
+                        ints(a[6], "pos", dev, tokens, true), static_cast<float>(theta), q.p, q.stride,
                         count(heads, "q"), qo.p, qo.stride, act, ints(a[10], "status", dev, 1, true), stream);
     });
 }

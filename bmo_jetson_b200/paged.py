@@ -9,8 +9,8 @@ synchronise.
 
     book = PageBook.empty(n_req, n_pages, page_size, max_blocks, window=512)
     kv = PagedKV.empty(book, n_layers, n_kv_heads, head_dim)
-    book.plan(n_new, slot, pos, req, offsets)             # once a step
-    kv.append(layer, k, v, slot, pos=pos, q=q, q_out=q)   # each layer
+    book.plan(n_new, slot, pos, req, offsets)  # once a step
+    kv.append(layer, k, v, slot, pos=pos, q=q, q_out=q, theta=10000.0)  # each layer
     kv.attention(layer, q, out)
 """
 from __future__ import annotations
@@ -161,7 +161,8 @@ class PagedKV:
                q_out: Optional[torch.Tensor] = None, theta: float = 0.0,
                status: Optional[torch.Tensor] = None) -> None:
         """Stores k, v [n, n_kv_heads, head_dim] at slot[n] (bmo_k_paged_append);
-        theta > 0 rotates k, and q into q_out, by the positions pos[n]."""
+        theta > 0 rotates k, and q into q_out, by the positions pos[n]; with
+        theta 0 nothing is rotated, pos is not read and q is refused."""
         _ext.append(self._addr, self._dev, layer, k, v, slot, pos, q, q_out, theta, status)
 
     def read(self, layer: int, slot: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor,

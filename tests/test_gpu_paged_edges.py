@@ -381,3 +381,16 @@ def test_attention_query_with_one_large_element(kv, heads):
     q = torch.from_numpy(q.astype(np.float32)).to(DEV)
     out, lse = r.run(q[None])
     check_edges((out[0], lse[0]), r.want(q), finite_max(r.v))
+
+
+# ---------------------------------------------------------------- arguments
+
+def test_append_with_queries_names_theta():
+    book = paged.PageBook.empty(1, 4, 16, 4)
+    cache = paged.PagedKV.empty(book, 1, 1, 64)
+    x = torch.randn(2, 1, 64, device=DEV)
+    with pytest.raises(ValueError, match="theta"):
+        cache.append(0, x, x, i32([0, 1]), pos=i32([0, 1]), q=x, q_out=x)
+    with pytest.raises(ValueError, match="q_out"):
+        cache.append(0, x, x, i32([0, 1]), pos=i32([0, 1]), q_out=x, theta=1e4)
+
