@@ -81,10 +81,13 @@ int layer_of(PyObject *o) {
     const long long v = integer(o);
     return v < 0 || v > INT32_MAX ? -1 : static_cast<int>(v);  // the library refuses -1
 }
-double number(PyObject *o) {
+// 0 has a meaning of its own in theta and scale: what rounds to it is refused.
+float number(PyObject *o, const char *name) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) throw Raised{};
-    return v;
+    const float f = static_cast<float>(v);
+    if (f == 0.0f && v != 0.0) refuse(name, "too small for float32");
+    return f;
 }
 int count(int64_t n, const char *name) {
     if (n > INT32_MAX) refuse(name, "too many rows");
@@ -137,8 +140,8 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Rows v = rows(a[4], "v", dev, tokens, c->n_kv_heads, c->head_dim, type);
         Rows q{nullptr, 0}, qo{nullptr, 0};
         int64_t heads = 0;
-        const double theta = number(a[9]);
-        if (a[7] != Py_None && theta == 0.0) refuse("theta", "above 0 where q is to be rotated");
+        const float theta = number(a[9], "theta");
+        if (a[7] != Py_None && theta == 0.0f) refuse("theta", "above 0 where q is to be rotated");
         if (a[7] == Py_None && a[8] != Py_None) refuse("q_out", "without q");
         if (a[7] != Py_None) {
             const at::Tensor &query = tensor(a[7], "q");
@@ -148,7 +151,7 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
             qo = rows(a[8], "q_out", dev, tokens, heads, c->head_dim, type);
         }
         return g_append(c, layer_of(a[2]), count(tokens, "slot"), k.p, k.stride, v.p, v.stride, ints(a[5], "slot", dev, -1),
-                        ints(a[6], "pos", dev, tokens, true), static_cast<float>(theta), q.p, q.stride,
+                        ints(a[6], "pos", dev, tokens, true), theta, q.p, q.stride,
                         count(heads, "q"), qo.p, qo.stride, act, ints(a[10], "status", dev, 1, true), stream);
     });
 }
@@ -190,7 +193,7 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
         }
         return g_attention(c, layer_of(a[2]), count(tokens, "q"), q.p, q.stride, count(heads, "q"),
                            ints(a[5], "rows", dev, tokens, true), ints(a[6], "row_lens", dev, tokens, true),
-                           static_cast<float>(number(a[7])), out.p, out.stride, lse, act,
+                           number(a[7], "scale"), out.p, out.stride, lse, act,
                            ints(a[9], "status", dev, 1, true), reinterpret_cast<void *>(integer(a[10])),
                            static_cast<size_t>(integer(a[11])), stream);
     });

@@ -394,3 +394,14 @@ def test_append_with_queries_names_theta():
     with pytest.raises(ValueError, match="q_out"):
         cache.append(0, x, x, i32([0, 1]), pos=i32([0, 1]), q_out=x, theta=1e4)
 
+
+
+@pytest.mark.parametrize("value", [1e-50, -1e-60])
+def test_scale_and_theta_below_fp32(value):
+    """What fp32 rounds to 0 is not taken for 0, which means 1 / sqrt(head_dim), or no rotation."""
+    c = base.Case([5], 1, 64, 16)
+    q = torch.randn(1, 1, 64, device=DEV)
+    with pytest.raises(ValueError, match="scale"):
+        c.cache.attention(0, q, torch.empty_like(q), scale=value)
+    with pytest.raises(ValueError, match="theta"):
+        c.cache.append(0, q, q, i32([0]), pos=i32([0]), theta=value)
