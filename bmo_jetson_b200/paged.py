@@ -76,6 +76,9 @@ class PageBook:
             raise ValueError("table: [n_req, max_blocks] on a GPU")
         self.table, self.lens, self.free, self.state = table, lens, free, state
         self.page_size, self.window, self.device = int(page_size), int(window), table.device
+        # the C struct has 32 bits for them
+        if not 1 <= self.page_size <= 65536 or not 0 <= self.window < 1 << 31:
+            raise ValueError(f"pages of 1 to 65536 positions, a window from 0 on: got {page_size}, {window}")
         n_req, max_blocks = table.shape
         self._c = _Book(_ints(table, "table", self.device), _ints(lens, "lens", self.device, n_req),
                         _ints(free, "free", self.device), _ints(state, "state", self.device, 4), n_req, max_blocks,

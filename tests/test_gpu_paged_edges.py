@@ -405,3 +405,11 @@ def test_scale_and_theta_below_fp32(value):
         c.cache.attention(0, q, torch.empty_like(q), scale=value)
     with pytest.raises(ValueError, match="theta"):
         c.cache.append(0, q, q, i32([0]), pos=i32([0]), theta=value)
+
+
+
+@pytest.mark.parametrize("kw", [dict(page_size=2 ** 32 + 16), dict(page_size=16, window=2 ** 32), dict(page_size=0),
+                                dict(page_size=65537), dict(page_size=16, window=-1)])
+def test_book_sizes_out_of_range(kw):
+    with pytest.raises(ValueError):
+        paged.PageBook(i32([[-1]]), i32([0]), i32([0]), i32([0, 1, 0, 0]), **kw)
