@@ -97,15 +97,22 @@ class PagedSessions:
         i32 = {"dtype": torch.int32, "device": self.book.device}
         self.lists = [torch.empty(n_req, **i32) for _ in range(3)]
         self.offsets = torch.empty(n_req + 1, **i32)
+        self.status = torch.zeros(1, **i32)  # of all frames since it was looked at
 
     def frame(self, x: torch.Tensor, new: Sequence[int]) -> torch.Tensor:
         """One frame: new[r] 1 for a session that gets a position, 0 for an idle
         one, -1 for one that ends.  x [n, dim]: the hidden states of the n sessions
-        that get a position, in order; returns theirs after the last layer."""
+        that get a position, in order; returns theirs after the last layer, NaN if
+        the frame was refused (refused() says why; the sessions are as before it)."""
         n = sum(1 for v in new if v > 0)
+        if len(new) != self.book.lens.numel() or any(v > 1 for v in new):
+            raise ValueError(f"new: 1, 0 or -1 for each of {self.book.lens.numel()} sessions")
+        if x.shape[0] != n:
+            raise ValueError(f"x: a row for each of the {n} sessions that get a position, got {x.shape[0]}")
         slot, pos, req = (t[:n] for t in self.lists)
         self.book.plan(torch.tensor(new, dtype=torch.int32).to(self.book.device, non_blocking=True), slot, pos, req,
                        self.offsets)
+        self.status |= self.book.state[2]
         if n == 0:
             return x
         for i, layer in enumerate(self.layers):
@@ -113,7 +120,7 @@ class PagedSessions:
             x = layer.o(a, resid=x)
             h = layer.ffn_in(x, gamma=layer.gamma2)
             x = layer.ffn_out(h, resid=x)
-        return x
+        return torch.where(self.book.state[2] == 0, x, torch.nan)  # without waiting for the plan
 
     def attend(self, i: int, qkv: torch.Tensor, slot: torch.Tensor, pos: torch.Tensor, req: torch.Tensor) -> torch.Tensor:
         """Layer i's attention of the projection's rows (q | k | v), which are rotated and stored on the way."""
@@ -128,8 +135,12 @@ class PagedSessions:
         return a
 
     def refused(self) -> int:
-        """Status bits of the last frame's plan (0: it was served); synchronises."""
-        return int(self.book.state[2])
+        """Status bits of the plans since the last call of this (0: all frames were served); synchronises."""
+        self.status |= self.book.state[2]
+        bits = int(self.status)
+        self.status.zero_()
+        self.book.state[2] = 0
+        return bits
 
 
 def main(argv=None) -> int:
@@ -154,8 +165,7 @@ def main(argv=None) -> int:
                       pages, a.page_size, window=a.window, kv_type=KV_F16 if a.kv == "f16" else KV_Q4_0)
     rng = np.random.default_rng(a.seed)
     x = torch.randn(a.sessions, a.dim, device="cuda")
-    rows, refused = 0, 0
-    t0 = 0.0
+    rows, t0 = 0, 0.0
     for f in range(a.frames + 3):
         if f == 3:  # the first frames size scratch buffers
             torch.cuda.synchronize()
