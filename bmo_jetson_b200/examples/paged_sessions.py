@@ -160,9 +160,10 @@ def main(argv=None) -> int:
     if not 1 <= a.sessions <= 64 or a.dim % a.heads or a.dim // a.heads not in (64, 128) or a.heads % a.kv_heads:
         ap.error("1 to 64 sessions, heads of 64 or 128, a multiple of the key heads")
     hd = a.dim // a.heads
-    pages = a.sessions * (-(-a.window // a.page_size) + 2)
+    longest = a.frames + 3
+    pages = a.sessions * (-(-(a.window or longest) // a.page_size) + 2)
     s = PagedSessions(random_layers(a.layers, a.dim, a.kv_heads * hd, a.ffn, a.seed), a.heads, a.kv_heads, hd, a.sessions,
-                      pages, a.page_size, window=a.window, kv_type=KV_F16 if a.kv == "f16" else KV_Q4_0)
+                      pages, a.page_size, longest, window=a.window, kv_type=KV_F16 if a.kv == "f16" else KV_Q4_0)
     rng = np.random.default_rng(a.seed)
     x = torch.randn(a.sessions, a.dim, device="cuda")
     rows, t0 = 0, 0.0

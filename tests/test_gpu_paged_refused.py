@@ -30,3 +30,8 @@ def test_frame_takes_a_position_a_session():
     with pytest.raises(ValueError):
         s.frame(x, [1, 0])
     assert s.refused() == 0 and s.book.lens.tolist() == [0, 0]
+
+
+def test_example_command_without_a_window():
+    assert ex.main(["--sessions", "3", "--frames", "40", "--layers", "1", "--dim", "128", "--heads", "2", "--kv-heads", "1",
+                    "--ffn", "256", "--window", "0"]) == 0
