@@ -3,9 +3,10 @@
 CUDA sources are compiled by nvcc with ``-gencode arch=compute_100a,code=sm_100a``,
 host sources by g++; the shared library links the CUDA runtime statically so it
 does not depend on whichever libcudart a host process already loaded.
-Rebuilds only objects whose source or headers changed.  Where torch is
-installed, the torch binding of the paged cache is built beside it
-(bmo_jetson_b200/lib/_paged.so).
+Rebuilds only objects whose source or headers changed.  Where torch with CUDA
+and Python's headers are installed, the torch binding of the paged cache is
+built beside it (bmo_jetson_b200/lib/_paged.<tag>.so, the tag made of torch's and
+Python's versions and of the sources).
 
     python -m bmo_jetson_b200.build [--force] [-j N]
 """
@@ -14,9 +15,12 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import glob
+import hashlib
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -25,7 +29,6 @@ OBJ = os.path.join(HERE, "lib", "obj")
 LIB = os.path.join(HERE, "lib", "libbmo.so")
 # torch binding of the paged cache (bmo_jetson_b200/paged.py): an extension module, built where torch is installed
 BINDING_SRC = os.path.join(HERE, "binding", "paged_torch.cpp")
-BINDING = os.path.join(HERE, "lib", "_paged.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CXX = "/usr/bin/g++"
 CUDA_INC = "/usr/local/cuda/include"
@@ -69,25 +72,42 @@ def _compile(cmd):
     return r.stderr
 
 
-def build_binding(force: bool = False):
-    """Builds the torch binding; None where torch or Python's headers are missing."""
-    import importlib.util
-    import sysconfig
-    spec = importlib.util.find_spec("torch")  # not imported: the paths are enough
-    py = sysconfig.get_paths()["include"]
-    if spec is None or not spec.submodule_search_locations or not os.path.exists(os.path.join(py, "Python.h")):
+def _torch_dir():
+    """Where torch is installed, found without importing it; None: it is not."""
+    spec = importlib.util.find_spec("torch")
+    return list(spec.submodule_search_locations)[0] if spec and spec.submodule_search_locations else None
+
+
+def binding_path():
+    """The torch binding for this torch, this Python and these sources: its file, built or not.
+    None where it cannot be built: no torch, a torch without CUDA, or no headers."""
+    t, py = _torch_dir(), sysconfig.get_paths()["include"]
+    if t is None:
         return None
-    t = list(spec.submodule_search_locations)[0]
-    deps = [BINDING_SRC, os.path.join(ROOT, "include", "bmo_kernels.h")]
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= max(os.path.getmtime(d) for d in deps):
-        return BINDING
-    os.makedirs(os.path.dirname(BINDING), exist_ok=True)
-    tmp = BINDING + ".tmp"
+    needs = [os.path.join(t, "include", "c10", "cuda", "CUDAGuard.h"), os.path.join(t, "lib", "libc10_cuda.so"),
+             os.path.join(t, "version.py"), os.path.join(py, "Python.h"), os.path.join(CUDA_INC, "cuda_runtime_api.h")]
+    if not all(os.path.isfile(n) for n in needs):
+        return None
+    tag = hashlib.sha256(str(sysconfig.get_config_var("SOABI")).encode())
+    for f in (needs[2], BINDING_SRC, os.path.join(ROOT, "include", "bmo_kernels.h")):
+        with open(f, "rb") as src:
+            tag.update(src.read())
+    return os.path.join(HERE, "lib", f"_paged.{tag.hexdigest()[:12]}.so")
+
+
+def build_binding(force: bool = False):
+    """Builds the torch binding unless its file is there; None where it cannot be built."""
+    so = binding_path()
+    if so is None or (os.path.exists(so) and not force):
+        return so
+    t, py = _torch_dir(), sysconfig.get_paths()["include"]
+    os.makedirs(os.path.dirname(so), exist_ok=True)
+    tmp = f"{so}.{os.getpid()}.tmp"
     _compile([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall", f"-I{ROOT}/include",
               f"-I{t}/include", f"-I{t}/include/torch/csrc/api/include", f"-I{py}", f"-I{CUDA_INC}", BINDING_SRC, "-o", tmp,
               f"-L{t}/lib", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
-    os.replace(tmp, BINDING)
-    return BINDING
+    os.replace(tmp, so)
+    return so
 
 
 def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
@@ -122,7 +142,10 @@ def build(force: bool = False, jobs: int = 0, verbose: bool = False) -> str:
         _compile([NVCC] + ARCH + ["-shared", "-ccbin", CXX, "-o", tmp] + objs +
                  ["-cudart", "static", "-lpthread", "-ldl", "-Xlinker", "--no-undefined"])
         os.replace(tmp, LIB)
-    build_binding(force)
+    binding = build_binding(force)
+    for old in glob.glob(os.path.join(HERE, "lib", "_paged*.so")):  # of sources or versions that are no more
+        if old != binding:
+            os.remove(old)
     return LIB
 
 

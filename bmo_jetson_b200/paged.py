@@ -17,7 +17,6 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
-import os
 from typing import Optional
 
 import torch
@@ -30,9 +29,10 @@ NO_PAGES, TABLE_FULL, NO_ROOM, BAD_INDEX = 1 << 5, 1 << 6, 1 << 7, 1 << 8
 
 def _load():
     """The extension module that checks tensors and calls the library (binding/paged_torch.cpp)."""
-    if not os.path.isfile(_build.BINDING) and _build.build_binding() is None:
-        raise ImportError("the torch binding of the paged cache needs torch's and Python's headers to be built")
-    spec = importlib.util.spec_from_file_location("_paged", _build.BINDING)
+    so = _build.build_binding()
+    if so is None:
+        raise ImportError("the torch binding of the paged cache needs a torch with CUDA, and torch's, Python's and CUDA's headers")
+    spec = importlib.util.spec_from_file_location("_paged", so)
     m = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(m)
     L = lib()
