@@ -1510,13 +1510,15 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     // shared memory instead of global memory (32 heads of 512 positions: 8.3 us
     // against 10.7).  As many CTAs as give a warp a tile, if 3 tiles a warp are enough and the
     // clusters find room at once: with all resident CTAs in clusters, 74 heads in
-    // clusters of 4 took 19.3 us, not 11.6.
+    // clusters of 4 took 19.3 us, not 11.6.  Pairs of CTAs (45 to 88 heads of 150 to
+    // 380 positions): Q4_0 8.0 to 10.6 us against 8.6 to 10.7 on the line, 8 query heads of
+    // 128 a key head in fp16 12 to 15 against 11 to 22.
     const long long heads = static_cast<long long>(a.n_rows) * a.units.d;
     const long long table = a.max_blocks * static_cast<long long>(a.page.d);
     const long long tiles = (a.window > 0 && a.window < table ? a.window : table) / (16 * R::kSub);
     a.cluster = 1;
     while (a.cluster < kMaxCluster && tiles > kPaWarps * a.cluster && heads * 2 * a.cluster * 5 <= grid * 3) a.cluster *= 2;
-    if (tiles > kPaWarps * a.cluster * kClusterTiles || (a.cluster == 2 && R::kMinCtas < 3)) a.cluster = 1;
+    if (tiles > kPaWarps * a.cluster * kClusterTiles) a.cluster = 1;
     if (a.cluster == 1) {
         paged_attn_kernel<R, ACT, kAligned><<<grid, kPaThreads, smem, s>>>(a);
         return cudaGetLastError();

@@ -413,3 +413,14 @@ def test_scale_and_theta_below_fp32(value):
 def test_book_sizes_out_of_range(kw):
     with pytest.raises(ValueError):
         paged.PageBook(i32([[-1]]), i32([0]), i32([0]), i32([0, 1, 0, 0]), **kw)
+
+
+# ---------------------------------------------------------------- a pair of CTAs a head
+
+@pytest.mark.parametrize("kv,hd,group", [("f16", 128, 8), ("f16", 64, 8), ("f16", 128, 1), ("q4_0", 128, 2), ("q4_0", 64, 4)])
+@pytest.mark.parametrize("ps", [16, 20])
+def test_attention_pairs_of_ctas(kv, hd, group, ps):
+    """48 to 80 key heads of up to 380 positions: two CTAs each, of which a short row leaves one idle."""
+    for rows, n in ((6, 380), (10, 250)):
+        lens = [n, 0, 1, n // 3] + [n] * (rows - 4)
+        base.check(base.Case(lens, 8, hd, ps, kv, seed=rows, window=n), 8 * group)
