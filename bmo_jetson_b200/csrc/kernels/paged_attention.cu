@@ -264,25 +264,22 @@ struct F16Rows {
         const int g = lane >> 2, t = lane & 3;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) inv[nb] = 1.0f;
-        {
-            constexpr int h0 = 0;
-            float x[kHeads][4];  // all heads' loads in flight
+        float x[kHeads][4];  // all heads' loads in flight
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j)
-                if (h0 + j < n_heads) query_load<ACT, HD>(src, q0 + (h0 + j) * HD, lane, x[j]);
+        for (int j = 0; j < kHeads; ++j)
+            if (j < n_heads) query_load<ACT, HD>(src, q0 + j * HD, lane, x[j]);
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j) {
-                if (h0 + j >= n_heads) continue;
-                const QueryPart p = query_part(x[j]);
-                if (4 * lane < HD) {
-                    uint2 *dst = reinterpret_cast<uint2 *>(buf + (h0 + j) * HD) + lane;
-                    dst[0] = make_uint2(half_bits2(p.hi[0], p.hi[1]), half_bits2(p.hi[2], p.hi[3]));
-                    dst[HD / 4] = make_uint2(half_bits2(p.lo[0], p.lo[1]), half_bits2(p.lo[2], p.lo[3]));
-                }
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-                    if (j == 4 * nb + t) inv[nb] = p.inv * qscale;
+        for (int j = 0; j < kHeads; ++j) {
+            if (j >= n_heads) continue;
+            const QueryPart p = query_part(x[j]);
+            if (4 * lane < HD) {
+                uint2 *dst = reinterpret_cast<uint2 *>(buf + j * HD) + lane;
+                dst[0] = make_uint2(half_bits2(p.hi[0], p.hi[1]), half_bits2(p.hi[2], p.hi[3]));
+                dst[HD / 4] = make_uint2(half_bits2(p.lo[0], p.lo[1]), half_bits2(p.lo[2], p.lo[3]));
             }
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (j == 4 * nb + t) inv[nb] = p.inv * qscale;
         }
         __syncwarp();
 #pragma unroll
@@ -1116,100 +1113,54 @@ __global__ void __launch_bounds__(kPaThreads, R::kMinCtas) paged_attn_kernel(con
         };
         uint32_t there = 0;  // positions attended to of the tile requested last
         if constexpr (R::kRing == 0) {
-            // Entries [b0, b0 + 32) of the block table, one a lane, and the next tile's
-            // block and place in it.  (Rows found as for the other loop measured 270 us against 259.)
+            // Step `tile` uses the rows requested in the step before and requests the next
+            // tile's.  Aligned pages are walked here, by block and place in it, from entries
+            // [b0, b0 + 32) of the block table, one a lane: rows found by locate() measured 270 us against 259.
             int block = fast_div(pbase + tile0 * kTile, a.page), b0 = block;
             uint32_t offset = pbase + tile0 * kTile - block * a.page.d;
-            auto entries = [&] { return b0 + lane < a.max_blocks ? table[b0 + lane] : -1; };
-            int entry = kAligned ? entries() : 0;
-        uint32_t there[1] = {};  // positions attended to of the tiles requested
-        // Step `tile` uses the rows requested kAhead steps before and requests
-        // those of kAhead tiles later; the first kAhead steps only request.
+            auto pages = [&] { return b0 + lane < a.max_blocks ? table[b0 + lane] : -1; };
+            int page_of = kAligned ? pages() : 0;
 #pragma unroll 1
-        for (int tile = tile0 - 1; tile < tile1; ++tile) {
-            const uint32_t now = there[0];
-            float sc[R::kSub][NB][2];
-            if (now) {
+            for (int tile = tile0 - 1; tile < tile1; ++tile) {
+                const uint32_t now = there;
+                if (now) {
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
+                    for (int s = 0; s < R::kSub; ++s) R_.load_v(s, P[s]);
 #pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
-                if (now != kAll) {
-#pragma unroll
-                    for (int s = 0; s < R::kSub; ++s)
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int i = 0; i < 2; ++i)
-                                if (!(now >> (16 * s + key_pos(lane, i)) & 1)) sc[s][nb][i] = -INFINITY;
+                    for (int s = 0; s < R::kSub; ++s) R_.scores(s, sc[s]);
+                    mask_scores(now);
                 }
-            }
-            there[0] = 0;
-            if (tile + 1 < tile1) {
-                uint32_t mask;
-                if constexpr (kAligned) {
-                    const int p0 = pbase + (tile + 1) * kTile;
-                    mask = kAll;
-                    if (p0 < start) mask &= kAll << (start - p0);
-                    if (p0 + kTile > len) mask &= kAll >> (p0 + kTile - len);
+                there = 0;
+                if (tile + 1 < tile1) {
+                    if constexpr (kAligned) {
+                        const int p0 = pbase + (tile + 1) * kTile;
+                        there = kAll;
+                        if (p0 < start) there &= kAll << (start - p0);
+                        if (p0 + kTile > len) there &= kAll >> (p0 + kTile - len);
 #pragma unroll
-                    for (int s = 0; s < R::kSub; ++s) {
-                        if (block >= b0 + 32) b0 = block, entry = entries();
-                        const int page = __shfl_sync(0xffffffffu, entry, block - b0);
-                        const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
-                        P[s].first = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + offset : 0;
-                        if (!ok) {
-                            bad |= (mask >> (16 * s) & 0xffff) != 0;
-                            mask &= ~(0xffffu << (16 * s));
+                        for (int s = 0; s < R::kSub; ++s) {
+                            if (block >= b0 + 32) b0 = block, page_of = pages();
+                            const int page = __shfl_sync(0xffffffffu, page_of, block - b0);
+                            const bool ok = static_cast<uint32_t>(page) < static_cast<uint32_t>(a.n_pages);
+                            P[s].first = ok ? (static_cast<uint32_t>(page) * a.n_kv_heads + kh) * a.page.d + offset : 0;
+                            if (!ok) {
+                                bad |= (there >> (16 * s) & 0xffff) != 0;
+                                there &= ~(0xffffu << (16 * s));
+                            }
+                            offset += 16;
+                            if (offset == a.page.d) offset = 0, ++block;
                         }
-                        offset += 16;
-                        if (offset == a.page.d) offset = 0, ++block;
+                    } else {
+                        there = locate(tile + 1);
                     }
-                } else {
-                    mask = locate(tile + 1);
+#pragma unroll
+                    for (int s = 0; s < R::kSub; ++s) R_.load_k(s, P[s]);
                 }
-                there[0] = mask;
-#pragma unroll
-                for (int s = 0; s < R::kSub; ++s) R_.load_k(s, P[s]);
+                if (!now) continue;
+                if (now != kAll) R_.clear_values(now, lane);
+                weigh();
+                R_.values(sc, o);
             }
-            if (!now) {
-                continue;
-            }
-            bool rise = false;
-#pragma unroll
-            for (int s = 0; s < R::kSub; ++s)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) rise |= fmaxf(sc[s][nb][0], sc[s][nb][1]) > m[nb] + kSlack;
-            if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    float x = m[nb];
-#pragma unroll
-                    for (int s = 0; s < R::kSub; ++s) x = fmaxf(x, fmaxf(sc[s][nb][0], sc[s][nb][1]));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    const float f = x == -INFINITY ? 1.0f : ex2(m[nb] - x);
-                    m[nb] = x;
-                    l[nb] *= f;
-#pragma unroll
-                    for (int j = 0; j < kO; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[nb][j][i] *= f;
-                }
-            }
-            if (now != kAll) R_.clear_values(now, lane);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                const float ref = m[nb] == -INFINITY ? 0.0f : m[nb] - kHead;
-#pragma unroll
-                for (int s = 0; s < R::kSub; ++s) {
-                    sc[s][nb][0] = ex2(sc[s][nb][0] - ref);
-                    sc[s][nb][1] = ex2(sc[s][nb][1] - ref);
-                    l[nb] += sc[s][nb][0] + sc[s][nb][1];
-                }
-            }
-            R_.values(sc, o);
-        }
         } else {
             // Step `tile` requests the rows of two tiles later, forms the next
             // tile's scores and adds its own values: two independent streams of arithmetic.
