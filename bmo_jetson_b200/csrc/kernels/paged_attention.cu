@@ -150,8 +150,9 @@ __device__ __forceinline__ uint32_t half_bits2(__half a, __half b) {
     return *reinterpret_cast<const uint32_t *>(&p);
 }
 
-// Codes 0..15 at bits 0-3 and 16-19 (or 4-7 and 20-23) of w as halves n - 8:
-// the code is placed in the mantissa of 1024 and the offset taken away.
+// Codes 0..15 at bits 0-3 and 16-19 (or 4-7 and 20-23) of w as halves n - 8,
+// by the usual way from a small integer to a float: its bits are placed in the
+// mantissa of a power of two, 1024, which is taken away with the offset.
 __device__ __forceinline__ uint32_t codes_lo(uint32_t w) {
     uint32_t m;
     asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(m) : "r"(w));  // (w & mask) | 1024.0
