@@ -48,8 +48,9 @@ namespace {
 // step, each thread writes what its request has.  Otherwise the thread that writes
 // an entry searches the prefix sums for its request, so entries are written
 // side by side whatever the requests' lengths are, kPlanBatch of a thread's in
-// flight.  64 requests of one position: 3.7 us, of which about 2 are the launch; 61
-// requests of up to 2999 new positions, both kernels: 11.6 us.
+// flight.  64 requests of one position: 3.9 us, of which about 2 are the launch; 61
+// requests of up to 2999 new positions, made again over a dropped plan, both
+// kernels: 12.8 to 13.4 us.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanOneCta = 8192;
 constexpr int kFew = 2;
@@ -464,7 +465,8 @@ using Act = typename ActOf<ACT>::type;
 // requested kAppendRows at a time, the first ones before the angles are computed.
 // Warps take few rows each when there are few tokens (share_rows), all of a
 // token's when there are many.  23993 tokens of 32 + 2 x 8 rows of 128 in bf16
-// (590 MB): 103 us, 5.7 TB/s; one token of 96 rows: 3.3 us; 64 tokens into Q4_0: 5.7 us.
+// (590 MB): 103 us, 5.7 TB/s; one token of 96 rows: 3.1 us; 64 tokens into Q4_0: 5.5 us.
+// The 23993 tokens into Q4_0 (519 MB): 235 us, 2.2 TB/s, bound by the packing's chain.
 constexpr int kAppendThreads = 128;
 constexpr int kAppendRows = 8;  // row slots of a lane in flight
 
@@ -579,7 +581,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
 
 // ---- read ----
 //
-// Bound by its bytes, most of them written when codes become floats.  A lane
+// fp16 rows are bound by their bytes (23993 rows of 2 x 8 heads of 128: 33.8 us,
+// 5.8 TB/s).  2999 Q4_0 rows of 2 x 32 heads to fp32 (112 MB): 23 us, 4.9 TB/s; writing
+// the floats alone, 98 MB, takes 14.7 us, so that is not the writes' bound.  A lane
 // makes 4 consecutive elements, so a warp writes whole lines; two lanes read the
 // same 4 bytes of codes, one for the low nibbles and one for the high ones.  Rows are shared out over
 // warps as for the append.

@@ -32,10 +32,11 @@
 // block, so the score comes out as one sum over codes a block, which the
 // block's scale multiplies in fp32; and the weight of a value's block is p times that
 // block's scale.  Unpacking costs two instructions per two codes, on
-// half-rate pipes, and makes the kernel bound by instructions: registers go to the
-// arithmetic, and rows arrive in a ring in shared memory by asynchronous copies.  64
-// sessions of 1500 positions (442 MB): 100 to 105 us, 4.2 to 4.4 TB/s, the issue
-// slots 62% busy; the rows in registers took 152 us, the ring alone brought 111.
+// half-rate pipes, and makes the kernel bound by instructions and their latencies at
+// three warps a scheduler: registers go to the arithmetic, and rows arrive in a ring in
+// shared memory by asynchronous copies.  64 sessions of 1500 positions (442 MB): 104 to
+// 106 us, 4.2 TB/s, the issue slots 62% busy; the rows in registers took 152 us, the
+// ring alone brought 111.
 //
 // Work: a row's window is cut into tiles of kTile positions; (row, key head,
 // tile) in that order is a line of tiles of which every warp takes an equal,
@@ -727,7 +728,8 @@ constexpr int pa_piece_floats = (R::kHeads * (R::HD + 2) + 3) / 4 * 4;
 // weights' sums.  The two parts of a factor are added as two products, and with
 // an infinite key or value these can be of opposite signs, or 0 times infinity.
 // Whatever that spoils ends as NaN (rows that hold NaN come here, too).  Sums in
-// double: speed does not matter.
+// double: speed does not matter.  Looking for NaN costs a call of small heads 0.1 to
+// 0.2 us of 8, 64 sessions of 16 tiles a head 0.4 of 47, long heads nothing.
 template <class R, int ACT>
 __device__ __noinline__ void exact_piece(const PagedAttnArgs &a, int row, int head0, int heads, int req, int p0, int p1,
                                          float *dst, float *dst_m, float *dst_l) {
@@ -1459,7 +1461,7 @@ cudaError_t pa_launch(PagedAttnArgs &a, void *scratch, size_t scratch_bytes, cud
     a.part = reinterpret_cast<float *>(static_cast<char *>(scratch) + (4 * kMaxGrid + 255) / 256 * 256);
     const size_t smem = kFixedSmem<R::HD, R::kHeads> + kPaWarps * R::kRing + 4 * a.n_rows;
     // Few heads of bounded length: a cluster a head, whose CTAs join through
-    // shared memory instead of global memory (32 heads of 512 positions: 8.3 us
+    // shared memory instead of global memory (32 heads of 512 positions: 8.3 to 8.6 us
     // against 10.7).  As many CTAs as give a warp a tile, if 3 tiles a warp are enough and the
     // clusters find room at once: with all resident CTAs in clusters, 74 heads in
     // clusters of 4 took 19.3 us, not 11.6.  Pairs of CTAs (45 to 88 heads of 150 to
@@ -1497,7 +1499,7 @@ template <class F>
 auto pa_variant(int head_dim, int kv_type, int group, F f) {
     // Query heads that share a key head are taken together as far as their sums fit the
     // registers: most of the work is on the codes (4 query heads of 128 a key
-    // head, 64 sessions of 1500: 99 us one by one, 72 to 77 in pairs).
+    // head, 64 sessions of 1500: 99 us one by one, 77 in pairs).
     if (kv_type == kKvQ4_0 && head_dim == 128)
         return group > 1 ? f(PaVariant<Q4Rows<128, 2>>{}) : f(PaVariant<Q4Rows<128, 1>>{});
     if (kv_type == kKvQ4_0)

@@ -240,7 +240,7 @@ BMO_API int bmo_k_paged_append(const bmo_paged_kv *cache, int layer, int n, cons
                                long long q_out_stride, int act_type, int *status_dev, void *stream);
 
 /* Reads the rows at slot_dev[0, n) of `layer` back: k_out_dev, v_out_dev
- * [n][n_kv_heads][head_dim], dense, in act_type; slot -1 and slots outside
+ * [n][n_kv_heads][head_dim], dense and aligned to 4 elements, in act_type; slot -1 and slots outside
  * the cache read as zeros (the latter set BMO_PAGED_BAD_INDEX). */
 BMO_API int bmo_k_paged_read(const bmo_paged_kv *cache, int layer, int n, const int32_t *slot_dev, void *k_out_dev,
                              void *v_out_dev, int act_type, int *status_dev, void *stream);
@@ -266,7 +266,8 @@ BMO_API size_t bmo_k_paged_attention_scratch_bytes(const bmo_paged_kv *cache, in
  * (each fp32 factor as two fp16 parts; heads that meet an infinite or NaN
  * element are computed from the formula instead, in which a block of a Q4_0 key
  * is its scale times the sum of its codes' products); the result is the same from call to
- * call.  scratch_dev must be zero on the first call, is left reusable, and
+ * call.  A row of one position gives the stored value, rounded or packed, where
+ * a ring's attention (bmo_k_decode_attention) gives v as it came.  scratch_dev must be zero on the first call, is left reusable, and
  * serves one call at a time.  n_rows <= 4096, and n_rows * n_heads *
  * (max_blocks * page_size / 16 + 4) below 2^31.  status_dev as above. */
 BMO_API int bmo_k_paged_attention(const bmo_paged_kv *cache, int layer, int n_rows, const void *q_dev,

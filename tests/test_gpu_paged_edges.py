@@ -424,3 +424,13 @@ def test_attention_pairs_of_ctas(kv, hd, group, ps):
     for rows, n in ((6, 380), (10, 250)):
         lens = [n, 0, 1, n // 3] + [n] * (rows - 4)
         base.check(base.Case(lens, 8, hd, ps, kv, seed=rows, window=n), 8 * group)
+
+
+def test_plan_without_undo():
+    """The undo buffer may be left out: plans that are adopted are served as before."""
+    n_req, n_pages, ps, window, first, second, most = REPEATED["histories"]
+    s = Steps(n_req, n_pages, ps, 120, window, most)
+    s.book._c.undo = None
+    for new in (first, [-1] * n_req, second, [1, 0, -1, 1, 1], [3, 50, 9, 0, 0]):
+        s.sim = s.check(new, s.plan(new))
+        s.adopt()
