@@ -395,7 +395,6 @@ def test_append_with_queries_names_theta():
         cache.append(0, x, x, i32([0, 1]), pos=i32([0, 1]), q_out=x, theta=1e4)
 
 
-
 @pytest.mark.parametrize("value", [1e-50, -1e-60])
 def test_scale_and_theta_below_fp32(value):
     """What fp32 rounds to 0 is not taken for 0, which means 1 / sqrt(head_dim), or no rotation."""
@@ -405,7 +404,6 @@ def test_scale_and_theta_below_fp32(value):
         c.cache.attention(0, q, torch.empty_like(q), scale=value)
     with pytest.raises(ValueError, match="theta"):
         c.cache.append(0, q, q, i32([0]), pos=i32([0]), theta=value)
-
 
 
 @pytest.mark.parametrize("kw", [dict(page_size=2 ** 32 + 16), dict(page_size=16, window=2 ** 32), dict(page_size=0),
